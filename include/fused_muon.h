@@ -169,6 +169,55 @@ int fm_muon_apply(void* param, int dtype, const void* update, int64_t n, float d
                   void* stream);
 
 /*
+ * AdamW over a list of tensors, in place, in as few launches as the list
+ * needs (one for up to 640 tensors):
+ *   m = lerp(m, g, w1);  v = lerp(v, g*g, w2)
+ *   p = p * decay + alpha * m / (eps + sqrt(v))
+ * with w1 = 1 - beta1, w2 = 1 - beta2, decay = 1 - lr*wd and, per tensor,
+ * alpha = -lr * sqrt(1 - beta2^t) / (1 - beta1^t).  dtype (FM_DT_F32 / BF16 /
+ * F16) is the parameters' and gradients' type; moment_dtype is the same, or
+ * FM_DT_F32 beside 16-bit parameters.  With equal types every op rounds to that
+ * type as the reference's torch ops do (bit-identical results); 16-bit
+ * parameters with fp32 moments are computed in fp32 and rounded once.  The
+ * list is read during the call (host memory); tensors with n = 0 are skipped
+ * and the tensors must not overlap.
+ * Replaces: muon_fused/optimizer.py:165-200 (nine torch ops per tensor).
+ */
+typedef struct {
+  void* param;
+  const void* grad;
+  void* moment1;
+  void* moment2;
+  int64_t n;
+  float alpha;
+} fm_adamw_tensor;
+int fm_adamw(const fm_adamw_tensor* tensors, int64_t count, int dtype, int moment_dtype,
+             float decay, float w1, float w2, float eps, void* stream);
+
+/*
+ * Decay + neuron-wise normalised update of `count` matrices of one shape
+ * (rows = output neurons), in place.  With u the matrix's bf16 update:
+ *   s_i = mean_j u_ij^2;  v_i = beta2 v_i + (1 - beta2) s_i
+ *   r_i = 1 / (sqrt(v_i) + eps);  F = |diag(r) u|_F
+ *   p_ij = p_ij * decay - step / (F + 1e-7) * r_i * u_ij
+ * with decay = 1 - lr*wd and step = lr * 0.2 * sqrt(rows * cols).  param has
+ * type dtype (FM_DT_F32 / BF16 / F16) and, like update, rows x cols contiguous
+ * elements; row_moment holds rows floats.  workspace: at least
+ * fm_normed_workspace_size() bytes, 256-byte aligned.  The list is read during
+ * the call; the matrices must not overlap.
+ * Replaces: nothing; it stands beside fm_muon_apply.
+ */
+typedef struct {
+  void* param;
+  const void* update;
+  float* row_moment;
+} fm_normed_matrix;
+int fm_normed_workspace_size(int64_t count, int64_t rows, uint64_t* bytes);
+int fm_muon_apply_normed(const fm_normed_matrix* mats, int64_t count, int64_t rows, int64_t cols,
+                         int dtype, float decay, float step, float beta2, float eps,
+                         void* workspace, uint64_t workspace_bytes, void* stream);
+
+/*
  * GEMM kernel selection for all later calls in the process:
  * 0 = automatic: a single-matrix call (fm_fused_newton_schulz, the
  *     allocation-free form) whose lower-triangle 128x128 tiles fit on the SMs

@@ -8,6 +8,7 @@ from __future__ import annotations
 
 import ctypes
 import os
+import struct
 import threading
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
@@ -38,11 +39,21 @@ SIGNATURES = {
     "fm_fused_newton_schulz_noalloc": (_c_int, [_vp, _c_int, _i64, _i64, _i64, _vp, _c_int, _vp]),
     "fm_muon_momentum": (_c_int, [_vp, _vp, _vp, _i64, _c_int, ctypes.c_float, _c_int, _vp]),
     "fm_muon_apply": (_c_int, [_vp, _c_int, _vp, _i64, ctypes.c_float, ctypes.c_float, _vp]),
+    "fm_adamw": (_c_int, [_vp, _i64, _c_int, _c_int, ctypes.c_float, ctypes.c_float,
+                          ctypes.c_float, ctypes.c_float, _vp]),
+    "fm_normed_workspace_size": (_c_int, [_i64, _i64, ctypes.POINTER(_u64)]),
+    "fm_muon_apply_normed": (_c_int, [_vp, _i64, _i64, _i64, _c_int, ctypes.c_float,
+                                      ctypes.c_float, ctypes.c_float, ctypes.c_float, _vp, _u64,
+                                      _vp]),
     "fm_set_gemm_path": (_c_int, [_c_int]),
     "fm_stage_timing": (_c_int, [_c_int]),
     "fm_stage_times": (_c_int, [ctypes.POINTER(ctypes.c_float), ctypes.POINTER(_c_int)]),
     "fm_launch_count": (_c_int, [ctypes.POINTER(ctypes.c_uint64)]),
 }
+
+# fm_adamw_tensor and fm_normed_matrix as struct formats (native alignment).
+ADAMW_TENSOR = struct.Struct("@PPPPqf4x")
+NORMED_MATRIX = struct.Struct("@PPP")
 
 _lib = None
 _lock = threading.Lock()

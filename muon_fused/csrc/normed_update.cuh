@@ -1,0 +1,194 @@
+// Decay + neuron-wise normalised update of same-shape matrices (rows = output
+// neurons, u = the bf16 orthogonalised update):
+//
+//   s_i = mean_j u_ij²             v_i = b2·v_i + (1-b2)·s_i
+//   r_i = 1 / (sqrt(v_i) + eps)    F = ‖diag(r)·u‖_F = sqrt(Σ_i cols·s_i·r_i²)
+//   p_ij = p_ij·(1 - lr·wd) - lr·0.2·sqrt(rows·cols)/(F + 1e-7) · r_i · u_ij
+//
+// F needs only the row sums, so two passes over u and one over p suffice:
+//   normed_rows   one row per warp (or block): Σ u², v, r and the block's share of F²
+//   normed_apply  p, walking the matrix backwards so that the rows of u read
+//                 last by normed_rows are still in L2
+// HBM bounds both.  All statistics are fp32; p is rounded once.  Sums run in a
+// fixed order (no atomics), so results repeat bit for bit.
+#pragma once
+#include <cstdint>
+
+#include "fm_ptx.cuh"
+#include "muon_elementwise.cuh"
+#include "ns_prep.cuh"
+
+namespace fm {
+
+constexpr int kNormedThreads = 256;
+constexpr int kNormedList = 64;        // matrices per launch
+constexpr int kNormedMaxBlocks = 1184; // row blocks per matrix = F² partials per matrix
+
+struct NormedEntry {
+  void* p;
+  const __nv_bfloat16* u;
+  float* v;
+};
+
+struct NormedArgs {
+  NormedEntry e[kNormedList];
+  long long rows, cols;
+  float* rinv;      // rows floats per matrix
+  float* partials;  // kNormedMaxBlocks per matrix
+  int row_blocks;
+  float decay, step, beta2, eps;  // step = lr·0.2·sqrt(rows·cols)
+};
+
+__device__ __forceinline__ float bf16x8_sumsq(uint4 u, float acc) {
+  const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float2 f = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&w[i]));
+    acc = fmaf(f.x, f.x, acc);
+    acc = fmaf(f.y, f.y, acc);
+  }
+  return acc;
+}
+
+// Σ u² over one row by `width` threads (t = 0..width-1): elements up to the
+// first 16-byte boundary, 16-byte loads, the rest.
+__device__ __forceinline__ float row_sumsq(const __nv_bfloat16* row, long long cols, int t,
+                                           int width) {
+  const long long mis = (reinterpret_cast<uintptr_t>(row) & 15) / 2;
+  const long long head = mis ? min(cols, 8 - mis) : 0;
+  const long long vecs = (cols - head) / 8;
+  const uint4* q = reinterpret_cast<const uint4*>(row + head);
+  float acc[4] = {0.f, 0.f, 0.f, 0.f};
+  long long i = t;
+  for (; i + 3ll * width < vecs; i += 4ll * width) {
+    uint4 a[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) a[k] = __ldg(q + i + static_cast<long long>(k) * width);
+#pragma unroll
+    for (int k = 0; k < 4; ++k) acc[k] = bf16x8_sumsq(a[k], acc[k]);
+  }
+  for (; i < vecs; i += width) acc[0] = bf16x8_sumsq(__ldg(q + i), acc[0]);
+  if (t < head) {
+    const float x = __bfloat162float(row[t]);
+    acc[1] = fmaf(x, x, acc[1]);
+  }
+  const long long tail = head + vecs * 8;
+  if (tail + t < cols) {
+    const float x = __bfloat162float(row[tail + t]);
+    acc[2] = fmaf(x, x, acc[2]);
+  }
+  return (acc[0] + acc[1]) + (acc[2] + acc[3]);
+}
+
+// TPR threads per row: a warp where a row is short, the block where it is long.
+template <int TPR>
+__global__ void __launch_bounds__(kNormedThreads)
+    normed_rows_kernel(const __grid_constant__ NormedArgs a) {
+  constexpr int kPer = kNormedThreads / TPR;  // rows per block and round
+  __shared__ float s_part[kNormedThreads / 32];
+  pdl_wait();
+  const NormedEntry e = a.e[blockIdx.y];
+  float* rinv = a.rinv + a.rows * blockIdx.y;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int sub = threadIdx.x / TPR, t = threadIdx.x % TPR;
+  float f2 = 0.f;  // this thread's rows' share of F² (thread t == 0 of each row)
+  for (long long r0 = static_cast<long long>(blockIdx.x) * kPer; r0 < a.rows;
+       r0 += static_cast<long long>(gridDim.x) * kPer) {
+    const long long r = r0 + sub;
+    const bool ok = r < a.rows;
+    float s = ok ? row_sumsq(e.u + r * a.cols, a.cols, t, TPR) : 0.f;
+    s = warp_sum(s);
+    if constexpr (TPR > 32) {
+      __syncthreads();
+      if (lane == 0) s_part[warp] = s;
+      __syncthreads();
+      s = 0.f;
+#pragma unroll
+      for (int w = 0; w < TPR / 32; ++w) s += s_part[w];
+    }
+    if (ok && t == 0) {
+      const float v = fmaf(a.beta2, e.v[r], (1.f - a.beta2) * (s / static_cast<float>(a.cols)));
+      e.v[r] = v;
+      const float ri = 1.f / (sqrtf(v) + a.eps);
+      rinv[r] = ri;
+      f2 = fmaf(s * ri, ri, f2);
+    }
+  }
+  f2 = warp_sum(f2);
+  __syncthreads();
+  if (lane == 0) s_part[warp] = f2;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    float x = 0.f;
+#pragma unroll
+    for (int w = 0; w < kNormedThreads / 32; ++w) x += s_part[w];
+    a.partials[static_cast<long long>(blockIdx.y) * kNormedMaxBlocks + blockIdx.x] = x;
+  }
+}
+
+template <typename T>
+__global__ void __launch_bounds__(kNormedThreads)
+    normed_apply_kernel(const __grid_constant__ NormedArgs a) {
+  __shared__ float s_part[kNormedThreads / 32];
+  pdl_wait();
+  const NormedEntry e = a.e[blockIdx.y];
+  T* p = static_cast<T*>(e.p);
+  const float* rinv = a.rinv + a.rows * blockIdx.y;
+  const float* part = a.partials + static_cast<long long>(blockIdx.y) * kNormedMaxBlocks;
+  float f2 = 0.f;
+  for (int i = threadIdx.x; i < a.row_blocks; i += kNormedThreads) f2 += part[i];
+  f2 = warp_sum(f2);
+  if ((threadIdx.x & 31) == 0) s_part[threadIdx.x >> 5] = f2;
+  __syncthreads();
+  f2 = 0.f;
+#pragma unroll
+  for (int w = 0; w < kNormedThreads / 32; ++w) f2 += s_part[w];
+  const float eta = -a.step / (sqrtf(f2) + 1e-7f);
+
+  const long long n = a.rows * a.cols;
+  const long long chunks = (n + 7) / 8;
+  const bool vec = aligned16(p) && aligned16(e.u);
+  for (long long b = blockIdx.x; b * kNormedThreads < chunks; b += gridDim.x) {
+    const long long c = chunks - 1 - (b * kNormedThreads + threadIdx.x);
+    if (c < 0) continue;
+    const long long i0 = c * 8;
+    const int cnt = static_cast<int>(min(8ll, n - i0));
+    // 32-bit division where it is enough: the 64-bit one costs more than the chunk's arithmetic
+    long long row = n <= 0xffffffffll ? static_cast<unsigned>(i0) / static_cast<unsigned>(a.cols)
+                                      : i0 / a.cols;
+    long long left = (row + 1) * a.cols - i0;  // elements of the chunk's first row from i0 on
+    float x[8], u[8];
+    const bool full = vec && cnt == 8;
+    if (full) {
+      load8(p + i0, true, x);
+      load8(e.u + i0, true, u);
+    } else {
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        x[k] = k < cnt ? to_f(p[i0 + k]) : 0.f;
+        u[k] = k < cnt ? __bfloat162float(e.u[i0 + k]) : 0.f;
+      }
+    }
+    float f = eta * rinv[row];
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      if (k < cnt) {
+        if (left == 0) {
+          left = a.cols;
+          f = eta * rinv[++row];
+        }
+        --left;
+        x[k] = fmaf(f, u[k], __fmul_rn(x[k], a.decay));
+      }
+    }
+    if (full) {
+      store8(p + i0, true, x);
+    } else {
+#pragma unroll
+      for (int k = 0; k < 8; ++k)
+        if (k < cnt) p[i0 + k] = from_f<T>(x[k]);
+    }
+  }
+}
+
+}  // namespace fm

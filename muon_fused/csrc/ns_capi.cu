@@ -23,7 +23,9 @@
 #include "ns_gemm_sm100.cuh"
 #include "ns_fused_sm100.cuh"
 #include "ns_fused2_sm100.cuh"
+#include "adamw_list.cuh"
 #include "muon_elementwise.cuh"
+#include "normed_update.cuh"
 #include "ns_prep.cuh"
 
 namespace fm {
@@ -721,6 +723,99 @@ int ns_run(const void* G, int dtype, long long batch, long long rows, long long 
   return FM_OK;
 }
 
+template <typename T, typename M, int CAP>
+int adamw_launch(const fm_adamw_tensor* ts, int64_t count, float decay, float w1, float w2,
+                 float eps, cudaStream_t st) {
+  constexpr long long kMaxChunks = 1ll << 30;  // blocks per launch (grid.x limit 2^31 - 1)
+  AdamTable<CAP> t;
+  t.decay = decay;
+  t.w1 = w1;
+  t.w2 = w2;
+  t.eps = eps;
+  int64_t i = 0;
+  long long done = 0;  // chunks of tensor i already launched
+  while (i < count) {
+    long long chunks = 0;
+    t.count = 0;
+    while (i < count && t.count < CAP && chunks < kMaxChunks) {
+      const fm_adamw_tensor& x = ts[i];
+      const long long off = done * kAdamChunk;
+      const long long need = (x.n - off + kAdamChunk - 1) / kAdamChunk;
+      const long long take = std::min(need, kMaxChunks - chunks);
+      if (take > 0) {
+        AdamEntry& e = t.e[t.count++];
+        e.p = static_cast<T*>(x.param) + off;
+        e.g = static_cast<const T*>(x.grad) + off;
+        e.m = static_cast<M*>(x.moment1) + off;
+        e.v = static_cast<M*>(x.moment2) + off;
+        e.n = std::min<long long>(x.n - off, take * kAdamChunk);
+        e.alpha = x.alpha;
+        e.first = unsigned(chunks);
+        chunks += take;
+      }
+      if (take == need) {
+        ++i;
+        done = 0;
+      } else {
+        done += take;
+      }
+    }
+    if (chunks == 0) break;
+    adamw_list_kernel<T, M, CAP><<<unsigned(chunks), kAdamThreads, 0, st>>>(t);
+    FM_CUDA(cudaGetLastError());
+    note_launch();
+  }
+  return FM_OK;
+}
+
+template <typename T, typename M>
+int adamw_any(const fm_adamw_tensor* ts, int64_t count, float decay, float w1, float w2, float eps,
+              cudaStream_t st) {
+  return count <= kAdamSmall ? adamw_launch<T, M, kAdamSmall>(ts, count, decay, w1, w2, eps, st)
+                             : adamw_launch<T, M, kAdamLarge>(ts, count, decay, w1, w2, eps, st);
+}
+
+template <typename T>
+int normed_launch(const DeviceState& ds, const fm_normed_matrix* mats, int64_t count,
+                  long long rows, long long cols, float decay, float step, float beta2, float eps,
+                  float* ws, cudaStream_t st) {
+  // Matrices per pair of launches: few enough that their updates stay in L2
+  // between the row pass and the apply pass.
+  constexpr long long kL2Keep = 64ll << 20;
+  const long long group = std::max<long long>(
+      1, std::min<long long>(kNormedList, kL2Keep / std::max<long long>(1, 2 * rows * cols)));
+  // A warp per row up to 4096 columns (16 loads of 16 bytes a lane), a block per longer row.
+  const bool wide = cols > 4096;
+  const long long per = wide ? 1 : kNormedThreads / 32;
+  const long long chunks = (rows * cols + 7) / 8;
+  for (int64_t i = 0; i < count; i += group) {
+    const int k = int(std::min<long long>(group, count - i));
+    NormedArgs a;
+    for (int j = 0; j < k; ++j) {
+      a.e[j].p = mats[i + j].param;
+      a.e[j].u = static_cast<const __nv_bfloat16*>(mats[i + j].update);
+      a.e[j].v = mats[i + j].row_moment;
+    }
+    a.rows = rows;
+    a.cols = cols;
+    a.rinv = ws + i * rows;
+    a.partials = ws + count * rows + i * kNormedMaxBlocks;
+    a.row_blocks = int(std::min<long long>(kNormedMaxBlocks, (rows + per - 1) / per));
+    a.decay = decay;
+    a.step = step;
+    a.beta2 = beta2;
+    a.eps = eps;
+    const dim3 g1(unsigned(a.row_blocks), unsigned(k));
+    const long long want = (chunks + kNormedThreads - 1) / kNormedThreads;
+    const dim3 g2(unsigned(std::min<long long>(want, ds.sm_count * 8ll)), unsigned(k));
+    FM_CUDA(wide ? launch_pdl(normed_rows_kernel<kNormedThreads>, g1, dim3(kNormedThreads), 0, st,
+                              false, a)
+                 : launch_pdl(normed_rows_kernel<32>, g1, dim3(kNormedThreads), 0, st, false, a));
+    FM_CUDA(launch_pdl(normed_apply_kernel<T>, g2, dim3(kNormedThreads), 0, st, false, a));
+  }
+  return FM_OK;
+}
+
 }  // namespace
 }  // namespace fm
 
@@ -890,6 +985,81 @@ int fm_muon_apply(void* param, int dtype, const void* update, int64_t n, float d
   FM_CUDA(cudaGetLastError());
   note_launch();
   return FM_OK;
+}
+
+int fm_adamw(const fm_adamw_tensor* tensors, int64_t count, int dtype, int moment_dtype,
+             float decay, float w1, float w2, float eps, void* stream) {
+  if (count < 0) return fail(FM_E_INVALID, "negative tensor count");
+  if (count == 0) return FM_OK;
+  if (!tensors) return fail(FM_E_INVALID, "null pointer argument");
+  if (dtype != FM_DT_F32 && dtype != FM_DT_BF16 && dtype != FM_DT_F16)
+    return fail(FM_E_INVALID, "fm_adamw: unsupported dtype %d", dtype);
+  if (moment_dtype != dtype && moment_dtype != FM_DT_F32)
+    return fail(FM_E_INVALID, "fm_adamw: moments must have the parameters' type or fp32, got %d",
+                moment_dtype);
+  for (int64_t i = 0; i < count; ++i) {
+    const fm_adamw_tensor& t = tensors[i];
+    if (t.n < 0) return fail(FM_E_INVALID, "fm_adamw: tensor %lld has a negative size", (long long)i);
+    if (t.n > 0 && (!t.param || !t.grad || !t.moment1 || !t.moment2))
+      return fail(FM_E_INVALID, "fm_adamw: tensor %lld has a null pointer", (long long)i);
+  }
+  DeviceState* ds;
+  if (int rc = device_state(&ds)) return rc;
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  const bool f32m = moment_dtype == FM_DT_F32;
+  switch (dtype) {
+    case FM_DT_F32:
+      return adamw_any<float, float>(tensors, count, decay, w1, w2, eps, st);
+    case FM_DT_BF16:
+      return f32m ? adamw_any<__nv_bfloat16, float>(tensors, count, decay, w1, w2, eps, st)
+                  : adamw_any<__nv_bfloat16, __nv_bfloat16>(tensors, count, decay, w1, w2, eps, st);
+    default:
+      return f32m ? adamw_any<__half, float>(tensors, count, decay, w1, w2, eps, st)
+                  : adamw_any<__half, __half>(tensors, count, decay, w1, w2, eps, st);
+  }
+}
+
+int fm_normed_workspace_size(int64_t count, int64_t rows, uint64_t* bytes) {
+  if (!bytes) return fail(FM_E_INVALID, "bytes is null");
+  if (count < 0 || rows < 0 || count > (1 << 20) || rows > (1ll << 40))
+    return fail(FM_E_INVALID, "count %lld / rows %lld out of range", (long long)count, (long long)rows);
+  *bytes = uint64_t(count) * (uint64_t(rows) + kNormedMaxBlocks) * 4;
+  return FM_OK;
+}
+
+int fm_muon_apply_normed(const fm_normed_matrix* mats, int64_t count, int64_t rows, int64_t cols,
+                         int dtype, float decay, float step, float beta2, float eps,
+                         void* workspace, uint64_t workspace_bytes, void* stream) {
+  if (count < 0 || rows < 0 || cols < 0) return fail(FM_E_INVALID, "negative size");
+  if (count == 0 || rows == 0 || cols == 0) return FM_OK;
+  if (!mats || !workspace) return fail(FM_E_INVALID, "null pointer argument");
+  if (rows > (1ll << 40) || cols > (1ll << 40) / rows)
+    return fail(FM_E_INVALID, "matrix %lld x %lld too large", (long long)rows, (long long)cols);
+  if ((reinterpret_cast<uintptr_t>(workspace) & 255) != 0)
+    return fail(FM_E_INVALID, "workspace must be 256-byte aligned");
+  uint64_t need = 0;
+  if (int rc = fm_normed_workspace_size(count, rows, &need)) return rc;
+  if (workspace_bytes < need)
+    return fail(FM_E_WORKSPACE, "workspace too small: need %llu bytes, got %llu",
+                (unsigned long long)need, (unsigned long long)workspace_bytes);
+  if (dtype != FM_DT_F32 && dtype != FM_DT_BF16 && dtype != FM_DT_F16)
+    return fail(FM_E_INVALID, "fm_muon_apply_normed: unsupported dtype %d", dtype);
+  for (int64_t i = 0; i < count; ++i)
+    if (!mats[i].param || !mats[i].update || !mats[i].row_moment)
+      return fail(FM_E_INVALID, "fm_muon_apply_normed: matrix %lld has a null pointer", (long long)i);
+  DeviceState* ds;
+  if (int rc = device_state(&ds)) return rc;
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  float* ws = static_cast<float*>(workspace);
+  switch (dtype) {
+    case FM_DT_F32:
+      return normed_launch<float>(*ds, mats, count, rows, cols, decay, step, beta2, eps, ws, st);
+    case FM_DT_BF16:
+      return normed_launch<__nv_bfloat16>(*ds, mats, count, rows, cols, decay, step, beta2, eps, ws,
+                                          st);
+    default:
+      return normed_launch<__half>(*ds, mats, count, rows, cols, decay, step, beta2, eps, ws, st);
+  }
 }
 
 int fm_set_gemm_path(int path) {

@@ -1,0 +1,225 @@
+"""Operators of the optimizer step around Newton-Schulz.
+
+``fused_adamw``          AdamW over a list of tensors in one launch;
+``fused_normed_update``  weight decay + neuron-wise normalised update of
+                         same-shape matrices.
+
+Both update their tensors in place on torch's current CUDA stream, never
+synchronise the host and raise ``RuntimeError`` on bad input.  They work on the
+tensors' values outside autograd (as an optimizer step under ``no_grad``) and
+bump the version counters of what they write, so a backward pass through values
+saved before the call fails instead of using the new ones.
+"""
+
+from __future__ import annotations
+
+import ctypes
+import math
+from collections.abc import Sequence
+
+import torch
+from torch.autograd.graph import increment_version
+
+from muon_fused import _lib
+from muon_fused._fused_muon_C import _check_cuda, _stream
+
+STEP_DTYPES = {torch.float32: _lib.FM_DT_F32, torch.bfloat16: _lib.FM_DT_BF16,
+               torch.float16: _lib.FM_DT_F16}
+
+
+def _check_list(tensors, name: str, count: int | None = None) -> list[torch.Tensor]:
+    if isinstance(tensors, torch.Tensor):
+        raise RuntimeError(f"{name} must be a list of tensors")
+    tensors = list(tensors)
+    if count is not None and len(tensors) != count:
+        raise RuntimeError(f"{name} must have one tensor per parameter, got {len(tensors)} "
+                           f"for {count}")
+    return tensors
+
+
+def _check_disjoint(*lists) -> None:
+    """No memory twice in one call: its elements would be updated in no order."""
+    spans = sorted((t.data_ptr(), t.data_ptr() + t.nbytes) for ts in lists for t in ts if t.numel())
+    for (_, end), (start, _) in zip(spans, spans[1:]):
+        if start < end:
+            raise RuntimeError("the tensors of one call must not overlap in memory")
+
+
+def adamw_launch(params, grads, moments1, moments2, alphas, lr: float, wd: float, betas,
+                 eps: float) -> None:
+    """The unchecked call: tensors of one device, one parameter type and one
+    moment type, all contiguous; ``alphas`` holds each tensor's -lr/scale."""
+    pack = _lib.ADAMW_TENSOR.pack
+    table = b"".join([
+        pack(p.data_ptr(), g.data_ptr(), m.data_ptr(), v.data_ptr(), p.numel(), a)
+        for p, g, m, v, a in zip(params, grads, moments1, moments2, alphas)])
+    p0 = params[0]
+    with torch.cuda.device(p0.device):
+        _lib.check(_lib.load().fm_adamw(
+            table, len(params), STEP_DTYPES[p0.dtype], STEP_DTYPES[moments1[0].dtype],
+            1 - lr * wd, 1 - betas[0], 1 - betas[1], eps, _stream(p0)), "fm_adamw")
+
+
+def adamw_alpha(lr: float, betas, step: int) -> float:
+    """-lr/scale, scale = (1 - b1^t)/sqrt(1 - b2^t) (reference optimizer.py:191-200)."""
+    return -lr / ((1 - betas[0] ** step) / (1 - betas[1] ** step) ** 0.5)
+
+
+def fused_adamw(
+    params: Sequence[torch.Tensor],
+    grads: Sequence[torch.Tensor],
+    moments1: Sequence[torch.Tensor],
+    moments2: Sequence[torch.Tensor],
+    steps: int | Sequence[int],
+    *,
+    lr: float,
+    wd: float = 0.1,
+    betas: tuple[float, float] = (0.9, 0.95),
+    eps: float = 1e-8,
+) -> None:
+    """AdamW step of every tensor of a list, in place::
+
+        m = lerp(m, g, 1 - b1);  v = lerp(v, g², 1 - b2)
+        p = p·(1 - lr·wd) - lr·sqrt(1 - b2^t)/(1 - b1^t) · m/(eps + sqrt(v))
+
+    Args:
+        params, grads: contiguous CUDA tensors (fp32, bf16 or fp16) on one
+            device; a gradient has its parameter's shape and type.
+        moments1, moments2: the running moments, of the parameter's type (every
+            op then rounds to it, as the optimizer's torch ops did) or fp32.
+        steps: the step count t >= 1 of each tensor (after this step), or one
+            for all.
+        lr, wd, betas, eps: as in :class:`FusedMuon`.
+
+    A list may mix types and sizes; tensors of zero elements are skipped.  No
+    two tensors may share memory.
+    """
+    params = _check_list(params, "params")
+    n = len(params)
+    grads = _check_list(grads, "grads", n)
+    moments1 = _check_list(moments1, "moments1", n)
+    moments2 = _check_list(moments2, "moments2", n)
+    steps = [steps] * n if isinstance(steps, int) else [int(s) for s in steps]
+    if len(steps) != n:
+        raise RuntimeError(f"steps must be an int or one per parameter, got {len(steps)} for {n}")
+    if any(s < 1 for s in steps):
+        raise RuntimeError("steps must be >= 1")
+    if not all(0.0 <= b < 1.0 for b in betas):
+        raise RuntimeError(f"betas must be in [0, 1), got {betas}")
+    if n == 0:
+        return
+    device = params[0].device
+    groups: dict[tuple, list[int]] = {}
+    for i, (p, g, m, v) in enumerate(zip(params, grads, moments1, moments2)):
+        if not (p.device == g.device == m.device == v.device == device):
+            raise RuntimeError("fused_adamw needs all tensors on one device")
+        _check_cuda(p, "params")
+        if p.dtype not in STEP_DTYPES or g.dtype != p.dtype:
+            raise RuntimeError(f"params and grads must be fp32, bf16 or fp16 of one type, got "
+                               f"{p.dtype} and {g.dtype}")
+        if m.dtype != v.dtype or m.dtype not in (p.dtype, torch.float32):
+            raise RuntimeError(f"moments must have the parameter's type or fp32, got {m.dtype} "
+                               f"and {v.dtype}")
+        if not (p.shape == g.shape == m.shape == v.shape):
+            raise RuntimeError("params, grads and moments must have the same shapes")
+        if not (p.is_contiguous() and g.is_contiguous() and m.is_contiguous()
+                and v.is_contiguous()):
+            raise RuntimeError("fused_adamw needs contiguous tensors")
+        if p.numel():
+            groups.setdefault((p.dtype, m.dtype), []).append(i)
+    _check_disjoint(params, grads, moments1, moments2)
+    for idx in groups.values():
+        adamw_launch([params[i] for i in idx], [grads[i] for i in idx],
+                     [moments1[i] for i in idx], [moments2[i] for i in idx],
+                     [adamw_alpha(lr, betas, steps[i]) for i in idx], lr, wd, betas, eps)
+    increment_version(params + moments1 + moments2)
+
+
+def normed_workspace_size(count: int, rows: int) -> int:
+    """Bytes of device workspace ``fused_normed_update`` needs for ``count`` matrices."""
+    out = ctypes.c_uint64(0)
+    _lib.check(_lib.load().fm_normed_workspace_size(int(count), int(rows), ctypes.byref(out)),
+               "fm_normed_workspace_size")
+    return int(out.value)
+
+
+def fused_normed_update(
+    params: Sequence[torch.Tensor],
+    updates: torch.Tensor | Sequence[torch.Tensor],
+    row_moments: Sequence[torch.Tensor],
+    *,
+    lr: float,
+    wd: float = 0.1,
+    beta2: float = 0.95,
+    eps: float = 1e-8,
+    workspace: torch.Tensor | None = None,
+) -> None:
+    """Decay + neuron-wise normalised update of same-shape matrices, in place.
+
+    For each matrix (rows = output neurons) with its orthogonalised update u::
+
+        s_i = mean_j u_ij²;  v_i = beta2·v_i + (1 - beta2)·s_i
+        r_i = 1/(sqrt(v_i) + eps);  F = ‖diag(r)·u‖_F
+        p_ij = p_ij·(1 - lr·wd) - lr·0.2·sqrt(rows·cols)/(F + 1e-7) · r_i·u_ij
+
+    so that every neuron moves at a rate of its own while the update's root
+    mean square stays 0.2·lr, the size Muon's learning-rate scale aims at.
+
+    Args:
+        params: contiguous CUDA parameters (fp32, bf16 or fp16) of one shape
+            and type; more than two dimensions are seen as (size(0), -1).
+        updates: a contiguous bf16 (count, rows, cols) tensor, or one bf16
+            tensor per parameter.
+        row_moments: an fp32 tensor of ``rows`` elements per parameter (v).
+        workspace: optional CUDA buffer of at least
+            ``normed_workspace_size(count, rows)`` bytes.
+    """
+    params = _check_list(params, "params")
+    n = len(params)
+    updates = list(updates.unbind(0)) if isinstance(updates, torch.Tensor) else list(updates)
+    updates = _check_list(updates, "updates", n)
+    row_moments = _check_list(row_moments, "row_moments", n)
+    if not 0.0 <= beta2 < 1.0:
+        raise RuntimeError(f"beta2 must be in [0, 1), got {beta2}")
+    if n == 0:
+        return
+    p0 = params[0]
+    _check_cuda(p0, "params")
+    if p0.dim() < 2:
+        raise RuntimeError("fused_normed_update needs matrices")
+    if p0.dtype not in STEP_DTYPES:
+        raise RuntimeError(f"params must be fp32, bf16 or fp16, got {p0.dtype}")
+    rows = p0.size(0)
+    cols = p0.numel() // rows if rows else 0
+    for p, u, v in zip(params, updates, row_moments):
+        if not (p.device == u.device == v.device == p0.device):
+            raise RuntimeError("fused_normed_update needs all tensors on one device")
+        if p.dtype != p0.dtype or p.shape != p0.shape:
+            raise RuntimeError("the params of one call must have one shape and type")
+        if u.dtype != torch.bfloat16 or u.numel() != p.numel() or (u.dim() and u.size(0) != rows):
+            raise RuntimeError("updates must be bf16 and shaped like the parameters")
+        if v.dtype != torch.float32 or v.shape != (rows,):
+            raise RuntimeError("row_moments must be fp32 vectors of one element per row")
+        if not (p.is_contiguous() and u.is_contiguous() and v.is_contiguous()):
+            raise RuntimeError("fused_normed_update needs contiguous tensors")
+    if p0.numel() == 0:
+        return
+    _check_disjoint(params, updates, row_moments)
+    need = normed_workspace_size(n, rows)
+    if workspace is None:
+        workspace = torch.empty(need, dtype=torch.uint8, device=p0.device)
+    else:
+        _check_cuda(workspace, "workspace")
+        if workspace.device != p0.device:
+            raise RuntimeError("workspace must be on the same device as the input")
+        if workspace.nbytes < need:  # as everywhere: too small is replaced
+            workspace = torch.empty(need, dtype=torch.uint8, device=p0.device)
+    pack = _lib.NORMED_MATRIX.pack
+    table = b"".join([pack(p.data_ptr(), u.data_ptr(), v.data_ptr())
+                      for p, u, v in zip(params, updates, row_moments)])
+    with torch.cuda.device(p0.device):
+        _lib.check(_lib.load().fm_muon_apply_normed(
+            table, n, rows, cols, STEP_DTYPES[p0.dtype], 1 - lr * wd,
+            lr * 0.2 * math.sqrt(rows * cols), beta2, eps, workspace.data_ptr(), workspace.nbytes,
+            _stream(p0)), "fm_muon_apply_normed")
+    increment_version(params + row_moments)
