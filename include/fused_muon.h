@@ -169,6 +169,24 @@ int fm_muon_apply(void* param, int dtype, const void* update, int64_t n, float d
                   void* stream);
 
 /*
+ * Newton-Schulz of each head of `batch` same-shape projections: a head is a
+ * block of rows / heads rows (dim 0: query, key and value projections) or of
+ * cols / heads columns (dim 1: output projection), at most 128 wide, and is
+ * normalised and orthogonalised by itself.  G, dtype, ldg and batch_stride_g
+ * as in fm_fused_newton_schulz_batched, except that fp16 is not rounded to bf16
+ * first; out: batch x rows x cols bf16, contiguous.  0 <= steps <= 8.  The
+ * products run in split fp16, so the result is the exact one up to its bf16
+ * rounding (the whole-matrix path iterates in bf16).
+ * workspace: at least fm_heads_workspace_size() bytes, 256-byte aligned.
+ * Replaces: nothing; the reference orthogonalises whole matrices only.
+ */
+int fm_heads_workspace_size(int64_t batch, int64_t rows, int64_t cols, int64_t heads, int dim,
+                            uint64_t* bytes);
+int fm_newton_schulz_heads(const void* G, int dtype, int64_t batch, int64_t rows, int64_t cols,
+                           int64_t ldg, int64_t batch_stride_g, int64_t heads, int dim, void* out,
+                           int steps, void* workspace, uint64_t workspace_bytes, void* stream);
+
+/*
  * AdamW over a list of tensors, in place, in as few launches as the list
  * needs (one for up to 640 tensors):
  *   m = lerp(m, g, w1);  v = lerp(v, g*g, w2)

@@ -113,6 +113,56 @@ def fused_newton_schulz_batched(G: torch.Tensor, steps: int = 5, workspace=None,
     return out
 
 
+def workspace_size_heads(batch: int, rows: int, cols: int, heads: int, dim: int = 0) -> int:
+    """Workspace bytes for ``batch`` (rows, cols) projections of ``heads`` heads."""
+    return _lib.workspace_bytes_heads(batch, rows, cols, heads, dim)
+
+
+def newton_schulz_heads(G: torch.Tensor, heads: int, steps: int = 5, dim: int = 0, workspace=None,
+                        out: torch.Tensor | None = None) -> torch.Tensor:
+    """Newton-Schulz of each head of a (rows, cols) or (batch, rows, cols)
+    projection (heads are blocks of rows, or of columns for dim=1); returns a
+    bf16 tensor of G's shape (or writes ``out``, contiguous, bf16, that shape)."""
+    _check_cuda(G, "G")
+    if G.dim() not in (2, 3):
+        raise RuntimeError("G must be 2D or 3D (batch, rows, cols)")
+    if G.dtype not in _DTYPE_CODE:
+        raise RuntimeError(f"unsupported dtype {G.dtype}; expected a floating type")
+    rows, cols = G.shape[-2:]
+    batch = G.shape[0] if G.dim() == 3 else 1
+    if out is None:
+        out = torch.empty(G.shape, dtype=torch.bfloat16, device=G.device)
+    elif (out.shape != G.shape or out.dtype != torch.bfloat16 or not out.is_contiguous()
+          or out.device != G.device):
+        raise RuntimeError("out must be a contiguous bf16 tensor shaped like G on its device")
+    elif out.untyped_storage().data_ptr() == G.untyped_storage().data_ptr():
+        raise RuntimeError("out must not share memory with G")
+    if G.numel() == 0:
+        return out
+    ld = G.stride(-2)
+    if (G.stride(-1) != 1 and cols > 1) or ld < cols or (
+            batch > 1 and G.stride(0) < (rows - 1) * ld + cols):
+        G = G.contiguous()
+        ld = cols
+    bs = G.stride(0) if G.dim() == 3 else 0
+    need = _lib.workspace_bytes_heads(batch, rows, cols, heads, dim)
+    if workspace is None:
+        workspace = torch.empty(need, dtype=torch.uint8, device=G.device)
+    else:
+        _check_cuda(workspace, "workspace")
+        if workspace.device != G.device:
+            raise RuntimeError("workspace must be on the same device as the input")
+        if workspace.nbytes < need:
+            workspace = torch.empty(need, dtype=torch.uint8, device=G.device)
+    with torch.cuda.device(G.device):
+        _lib.check(
+            _lib.load().fm_newton_schulz_heads(
+                G.data_ptr(), _DTYPE_CODE[G.dtype], batch, rows, cols, ld, bs, int(heads), int(dim),
+                out.data_ptr(), int(steps), workspace.data_ptr(), workspace.nbytes, _stream(G)),
+            "fm_newton_schulz_heads")
+    return out
+
+
 def newton_schulz_step(X: torch.Tensor, workspace=None) -> torch.Tensor:
     """One iteration on a normalised bf16 matrix: (aI + bA + cA²)·X, A = X·Xᵀ.
 

@@ -39,6 +39,9 @@ SIGNATURES = {
     "fm_fused_newton_schulz_noalloc": (_c_int, [_vp, _c_int, _i64, _i64, _i64, _vp, _c_int, _vp]),
     "fm_muon_momentum": (_c_int, [_vp, _vp, _vp, _i64, _c_int, ctypes.c_float, _c_int, _vp]),
     "fm_muon_apply": (_c_int, [_vp, _c_int, _vp, _i64, ctypes.c_float, ctypes.c_float, _vp]),
+    "fm_heads_workspace_size": (_c_int, [_i64, _i64, _i64, _i64, _c_int, ctypes.POINTER(_u64)]),
+    "fm_newton_schulz_heads": (_c_int, [_vp, _c_int, _i64, _i64, _i64, _i64, _i64, _i64, _c_int, _vp,
+                                        _c_int, _vp, _u64, _vp]),
     "fm_adamw": (_c_int, [_vp, _i64, _c_int, _c_int, ctypes.c_float, ctypes.c_float,
                           ctypes.c_float, ctypes.c_float, _vp]),
     "fm_normed_workspace_size": (_c_int, [_i64, _i64, ctypes.POINTER(_u64)]),
@@ -99,6 +102,13 @@ def workspace_bytes_batched(batch: int, rows: int, cols: int) -> int:
     out = ctypes.c_uint64(0)
     check(load().fm_workspace_size_batched(int(batch), int(rows), int(cols), ctypes.byref(out)),
           "fm_workspace_size_batched")
+    return int(out.value)
+
+
+def workspace_bytes_heads(batch: int, rows: int, cols: int, heads: int, dim: int) -> int:
+    out = ctypes.c_uint64(0)
+    check(load().fm_heads_workspace_size(int(batch), int(rows), int(cols), int(heads), int(dim),
+                                         ctypes.byref(out)), "fm_heads_workspace_size")
     return int(out.value)
 
 

@@ -19,7 +19,8 @@ CSRC = os.path.join(HERE, "csrc")
 LIB = os.path.join(HERE, "libfused_muon.so")
 SOURCES = ["ns_capi.cu"]
 DEPS = SOURCES + ["fm_ptx.cuh", "ns_gemm_sm100.cuh", "ns_gemm2_sm100.cuh", "ns_prep.cuh", "ns_fused_sm100.cuh", "ns_fused2_sm100.cuh",
-                  "muon_elementwise.cuh", "adamw_list.cuh", "normed_update.cuh"]
+                  "muon_elementwise.cuh", "adamw_list.cuh", "normed_update.cuh",
+                  "ns_heads_sm100.cuh"]
 HEADER = os.path.join(os.path.dirname(HERE), "include", "fused_muon.h")
 
 NVCC_FLAGS = [

@@ -26,6 +26,7 @@
 #include "adamw_list.cuh"
 #include "muon_elementwise.cuh"
 #include "normed_update.cuh"
+#include "ns_heads_sm100.cuh"
 #include "ns_prep.cuh"
 
 namespace fm {
@@ -114,6 +115,28 @@ void timer_end(long long start, cudaStream_t st) {
   cudaEventRecord(e, st);
 }
 
+// Shared-memory opt-in of every per-head kernel (ns_heads_sm100.cuh).
+template <int DP, bool HALF>
+int heads_setup_for() {
+  auto smem = [](const void* fn, int bytes) -> int {
+    FM_CUDA(cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
+    return FM_OK;
+  };
+  int rc;
+  if ((rc = smem((const void*)heads_gram_kernel<DP, false, HALF>, GramCfg<DP>::kSmem))) return rc;
+  if ((rc = smem((const void*)heads_gram_kernel<DP, true, HALF>, GramCfg<DP>::kSmem))) return rc;
+  if ((rc = smem((const void*)heads_iterate_kernel<DP, HALF>, IterCfg<DP>::kSmem))) return rc;
+  if ((rc = smem((const void*)heads_apply_kernel<DP, false, HALF>, ApplyCfg<DP>::kSmem))) return rc;
+  return smem((const void*)heads_apply_kernel<DP, true, HALF>, ApplyCfg<DP>::kSmem);
+}
+int heads_setup() {
+  int rc;
+  if ((rc = heads_setup_for<64, false>())) return rc;
+  if ((rc = heads_setup_for<64, true>())) return rc;
+  if ((rc = heads_setup_for<128, false>())) return rc;
+  return heads_setup_for<128, true>();
+}
+
 // Per-device set-up: SM count, smem opt-in for the GEMM kernels, address of
 // the device error word.  Runs once per device, with that device current.
 int device_state(DeviceState** out) {
@@ -151,6 +174,7 @@ int device_state(DeviceState** out) {
                                    FusedCfg<128>::kSmem));
       FM_CUDA(cudaFuncSetAttribute(ns_fused_pair_kernel,
                                    cudaFuncAttributeMaxDynamicSharedMemorySize, kPairSmemBytes));
+      if (int rc = heads_setup()) return rc;
       FM_CUDA(cudaGetSymbolAddress(reinterpret_cast<void**>(&s.err_word), g_device_error));
       if (!g_encode) {
         cudaDriverEntryPointQueryResult q;
@@ -723,6 +747,205 @@ int ns_run(const void* G, int dtype, long long batch, long long rows, long long 
   return FM_OK;
 }
 
+// ---------------------------------------------------------------- heads
+// One per-head problem: `total` blocks of head side d and long side n.
+struct HeadsPlan {
+  long long d, n, total;
+  int dp;        // d padded to the kernels' size
+  bool direct;   // TMA reads G in place
+  int kblocks, split, kbps;
+  size_t gram, q, inv, pack, bytes;  // workspace offsets and size
+  long long pack_ld;                 // row stride of the copy
+};
+
+// Splits of the long side per head in the Gram kernel: enough units for one
+// per SM of a 148-SM B200, but at least four k-blocks (256 elements) each — a
+// split costs the iterate kernel one more d x d partial to read.
+HeadsPlan plan_heads(long long batch, long long rows, long long cols, long long heads, int dim,
+                     bool direct) {
+  HeadsPlan P{};
+  P.d = (dim == 0 ? rows : cols) / heads;
+  P.n = dim == 0 ? cols : rows;
+  P.total = batch * heads;
+  P.dp = P.d <= 64 ? 64 : 128;
+  P.direct = direct;
+  P.kblocks = int((P.n + kHeadsK - 1) / kHeadsK);
+  long long s = std::max<long long>(1, 148 / P.total);
+  s = std::min<long long>(s, std::max(1, P.kblocks / 4));
+  P.kbps = int((P.kblocks + s - 1) / s);
+  P.split = (P.kblocks + P.kbps - 1) / P.kbps;
+  auto a256 = [](size_t b) { return (b + 255) & ~size_t(255); };
+  const size_t mat = size_t(P.dp) * P.dp;
+  size_t off = 0;
+  P.gram = off; off += a256(size_t(P.total) * P.split * mat * 4);
+  P.q = off; off += a256(size_t(P.total) * 2 * mat * 2);
+  P.inv = off; off += a256(size_t(P.total) * 4);
+  P.pack = off;
+  P.pack_ld = round_up(dim == 0 ? P.n : P.d, 8);
+  if (!direct) off += a256(size_t(P.total) * (dim == 0 ? P.d : P.n) * P.pack_ld * 2);
+  P.bytes = off;
+  return P;
+}
+
+// Whether TMA can address the heads of G in place: 16-bit elements whose rows,
+// heads and matrices start on 16-byte boundaries.
+bool heads_direct(const void* G, int dtype, long long ldg, long long bs_g, long long batch,
+                  long long d, int dim) {
+  if (dtype != FM_DT_BF16 && dtype != FM_DT_F16) return false;
+  return (reinterpret_cast<uintptr_t>(G) & 15) == 0 && ldg % 8 == 0 &&
+         (batch == 1 || bs_g % 8 == 0) && (dim == 0 || d % 8 == 0);
+}
+
+// 16-bit 4-D map (inner, outer, head, matrix) with element strides of the
+// outer three; a dimension of one element gets any valid stride.
+int heads_map(CUtensorMap* map, const void* base, long long inner, long long outer, long long heads,
+              long long mats, long long ld, long long head_stride, long long mat_stride,
+              int box_inner, int box_outer) {
+  if (heads == 1) head_stride = round_up(ld, 8);
+  if (mats == 1) mat_stride = round_up(ld, 8);
+  if (outer == 1) ld = round_up(inner, 8);
+  cuuint64_t dims[4] = {cuuint64_t(inner), cuuint64_t(outer), cuuint64_t(heads), cuuint64_t(mats)};
+  cuuint64_t strides[3] = {cuuint64_t(ld * 2), cuuint64_t(head_stride * 2),
+                           cuuint64_t(mat_stride * 2)};
+  cuuint32_t box[4] = {cuuint32_t(box_inner), cuuint32_t(box_outer), 1, 1};
+  cuuint32_t estr[4] = {1, 1, 1, 1};
+  const CUresult r = g_encode(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, const_cast<void*>(base),
+                              dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                              CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) return fail(FM_E_CUDA, "cuTensorMapEncodeTiled failed (%d)", int(r));
+  return FM_OK;
+}
+
+template <int DP, bool COLS, bool HALF>
+int heads_launch(const DeviceState& ds, const HeadsPlan& P, const CUtensorMap& gram_map,
+                 const CUtensorMap& g_map, const CUtensorMap& q_map, const CUtensorMap& o_map,
+                 const HeadsArgs& a, cudaStream_t st) {
+  const long long tm = timer_begin(4, st);
+  FM_CUDA(launch_pdl(heads_gram_kernel<DP, COLS, HALF>, dim3(unsigned(P.total * P.split)),
+                     dim3(kGramThreads), GramCfg<DP>::kSmem, st, false, gram_map, a));
+  FM_CUDA(launch_pdl(heads_iterate_kernel<DP, HALF>, dim3(unsigned(P.total)), dim3(kIterThreads),
+                     IterCfg<DP>::kSmem, st, false, a));
+  const long long units = P.total * a.chunks;
+  FM_CUDA(launch_pdl(heads_apply_kernel<DP, COLS, HALF>,
+                     dim3(unsigned(std::min<long long>(units, ds.sm_count))), dim3(kApplyThreads),
+                     ApplyCfg<DP>::kSmem, st, false, g_map, q_map, o_map, a));
+  timer_end(tm, st);
+  return FM_OK;
+}
+
+int heads_check(long long batch, long long rows, long long cols, long long heads, int dim) {
+  if (batch < 1 || rows < 1 || cols < 1 || heads < 1)
+    return fail(FM_E_INVALID, "batch, rows, cols and heads must be positive");
+  if (dim != 0 && dim != 1) return fail(FM_E_INVALID, "dim must be 0 or 1, got %d", dim);
+  const long long side = dim == 0 ? rows : cols;
+  if (side % heads != 0)
+    return fail(FM_E_INVALID, "%lld %s do not divide into %lld heads", side,
+                dim == 0 ? "rows" : "columns", heads);
+  if (side / heads > kHeadsMaxDim)
+    return fail(FM_E_INVALID, "heads of %lld %s are wider than %d", side / heads,
+                dim == 0 ? "rows" : "columns", kHeadsMaxDim);
+  if (batch > 65535 || heads > 65535 || batch * heads > 65535)
+    return fail(FM_E_INVALID, "at most 65535 heads in one call, got %lld x %lld", batch, heads);
+  if (std::max(rows, cols) > (1ll << 30)) return fail(FM_E_INVALID, "matrix %lld x %lld too large", rows, cols);
+  return FM_OK;
+}
+
+int heads_run(const void* G, int dtype, long long batch, long long rows, long long cols,
+              long long ldg, long long bs_g, long long heads, int dim, void* out, int steps,
+              void* workspace, uint64_t workspace_bytes, cudaStream_t st) {
+  if (!G || !out || !workspace) return fail(FM_E_INVALID, "null pointer argument");
+  if (dtype < FM_DT_BF16 || dtype > FM_DT_F64) return fail(FM_E_INVALID, "unknown dtype %d", dtype);
+  if (steps < 0 || steps > kHeadsMaxSteps)
+    return fail(FM_E_INVALID, "steps must be in [0, %d], got %d", kHeadsMaxSteps, steps);
+  if (int rc = heads_check(batch, rows, cols, heads, dim)) return rc;
+  if (ldg < cols) return fail(FM_E_INVALID, "ldg %lld < cols %lld", ldg, cols);
+  if (batch > 1 && bs_g < (rows - 1) * ldg + cols)
+    return fail(FM_E_INVALID, "batch strides must not overlap matrices");
+  if ((reinterpret_cast<uintptr_t>(workspace) & 255) != 0)
+    return fail(FM_E_INVALID, "workspace must be 256-byte aligned");
+  const long long d = (dim == 0 ? rows : cols) / heads;
+  const HeadsPlan P = plan_heads(batch, rows, cols, heads, dim,
+                                 heads_direct(G, dtype, ldg, bs_g, batch, d, dim));
+  if (workspace_bytes < P.bytes)
+    return fail(FM_E_WORKSPACE, "workspace too small: need %zu bytes, got %llu", P.bytes,
+                (unsigned long long)workspace_bytes);
+  DeviceState* ds;
+  if (int rc = device_state(&ds)) return rc;
+  char* ws = static_cast<char*>(workspace);
+  const bool cols_form = dim == 1, half = dtype == FM_DT_F16;
+
+  HeadsArgs a{};
+  a.d = int(P.d);
+  a.n = int(P.n);
+  a.heads = int(heads);
+  a.total = int(P.total);
+  a.kblocks = P.kblocks;
+  a.split = P.split;
+  a.kbps = P.kbps;
+  a.steps = steps;
+  a.gram = reinterpret_cast<float*>(ws + P.gram);
+  a.q = ws + P.q;
+  a.inv = reinterpret_cast<float*>(ws + P.inv);
+  a.out = static_cast<__nv_bfloat16*>(out);
+  a.out_ld = cols;
+  a.out_head = cols_form ? P.d : P.d * cols;
+  a.out_mat = rows * cols;
+  a.chunks = int((P.n + kApplyN - 1) / kApplyN);
+  a.err = ds->err_word;
+
+  // strides of the G that the kernels read
+  const void* src = G;
+  long long ld = ldg, hs = cols_form ? P.d : P.d * ldg, ms = bs_g;
+  if (!P.direct) {
+    const long long outer = cols_form ? P.n : P.d;
+    const int inner = int(cols_form ? P.d : P.n);
+    const long long blocks = std::min<long long>(outer, std::max<long long>(1, ds->sm_count * 8ll / P.total));
+    const dim3 grid(unsigned(blocks), unsigned(P.total));
+    if (half) {
+      FM_CUDA(launch_pdl(heads_pack_kernel<__half>, grid, dim3(256), 0, st, false, G, dtype, ldg,
+                         bs_g, int(heads), hs, outer, inner, reinterpret_cast<__half*>(ws + P.pack),
+                         P.pack_ld));
+    } else {
+      FM_CUDA(launch_pdl(heads_pack_kernel<__nv_bfloat16>, grid, dim3(256), 0, st, false, G, dtype,
+                         ldg, bs_g, int(heads), hs, outer, inner,
+                         reinterpret_cast<__nv_bfloat16*>(ws + P.pack), P.pack_ld));
+    }
+    src = ws + P.pack;
+    ld = P.pack_ld;
+    hs = outer * ld;
+    ms = hs * heads;
+  }
+  const long long inner = cols_form ? P.d : P.n, outer = cols_form ? P.n : P.d;
+  CUtensorMap gram_map, g_map, q_map, o_map;
+  int rc;
+  if ((rc = heads_map(&gram_map, src, inner, outer, heads, batch, ld, hs, ms, 64,
+                      cols_form ? kHeadsK : P.dp)))
+    return rc;
+  if ((rc = heads_map(&g_map, src, inner, outer, heads, batch, ld, hs, ms, 64,
+                      cols_form ? kApplyN : P.dp)))
+    return rc;
+  // both terms of a head as 2·DP rows
+  if ((rc = make_map(&q_map, a.q, P.total, 2 * P.dp, P.dp, P.dp, 2ll * P.dp * P.dp, 64, P.dp)))
+    return rc;
+  a.tma_out = (reinterpret_cast<uintptr_t>(out) & 15) == 0 && cols % 8 == 0 &&
+              (!cols_form || P.d % 8 == 0);
+  if (a.tma_out) {
+    if ((rc = heads_map(&o_map, out, inner, outer, heads, batch, cols, a.out_head, a.out_mat, 64, 32)))
+      return rc;
+  } else {
+    o_map = g_map;  // unused
+  }
+#define FM_HEADS(DP, C, H) heads_launch<DP, C, H>(*ds, P, gram_map, g_map, q_map, o_map, a, st)
+  if (P.dp == 64) {
+    if (cols_form) return half ? FM_HEADS(64, true, true) : FM_HEADS(64, true, false);
+    return half ? FM_HEADS(64, false, true) : FM_HEADS(64, false, false);
+  }
+  if (cols_form) return half ? FM_HEADS(128, true, true) : FM_HEADS(128, true, false);
+  return half ? FM_HEADS(128, false, true) : FM_HEADS(128, false, false);
+#undef FM_HEADS
+}
+
 template <typename T, typename M, int CAP>
 int adamw_launch(const fm_adamw_tensor* ts, int64_t count, float decay, float w1, float w2,
                  float eps, cudaStream_t st) {
@@ -985,6 +1208,21 @@ int fm_muon_apply(void* param, int dtype, const void* update, int64_t n, float d
   FM_CUDA(cudaGetLastError());
   note_launch();
   return FM_OK;
+}
+
+int fm_heads_workspace_size(int64_t batch, int64_t rows, int64_t cols, int64_t heads, int dim,
+                            uint64_t* bytes) {
+  if (!bytes) return fail(FM_E_INVALID, "bytes is null");
+  if (int rc = heads_check(batch, rows, cols, heads, dim)) return rc;
+  *bytes = plan_heads(batch, rows, cols, heads, dim, false).bytes;
+  return FM_OK;
+}
+
+int fm_newton_schulz_heads(const void* G, int dtype, int64_t batch, int64_t rows, int64_t cols,
+                           int64_t ldg, int64_t batch_stride_g, int64_t heads, int dim, void* out,
+                           int steps, void* workspace, uint64_t workspace_bytes, void* stream) {
+  return heads_run(G, dtype, batch, rows, cols, ldg, batch_stride_g, heads, dim, out, steps,
+                   workspace, workspace_bytes, static_cast<cudaStream_t>(stream));
 }
 
 int fm_adamw(const fm_adamw_tensor* tensors, int64_t count, int dtype, int moment_dtype,

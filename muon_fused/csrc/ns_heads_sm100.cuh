@@ -1,0 +1,725 @@
+// Per-head Newton-Schulz in Gram form.
+//
+// A head is a block of d <= 128 rows (or columns) of a projection, n long, and
+// is orthogonalised by itself.  With X0 = G/(‖G‖+1e-7) and A0 = X0·X0ᵀ (d x d),
+// every iterate is a polynomial of A0 times X0, X_k = Q_k·X0, so the iteration
+// runs on d x d matrices alone:
+//
+//   B = a·I + b·A + c·A²      Q ← B·Q      A ← B·A·B      (Q_0 = I)
+//
+// G is read for A0 and once more for Q·G; the whole-matrix path reads and
+// writes X in each of its 15 products and pads every d-row block to a
+// 256-row tile.  Three kernels:
+//
+//   heads_gram     partial G·Gᵀ over a range of n            (HBM bound)
+//   heads_iterate  sum of the partials, norm, all iterations  (latency bound)
+//   heads_apply    out = Q·G/(‖G‖+1e-7)                       (HBM bound)
+//
+// Precision.  A0 is an fp32 sum of exact products.  Products of the 16-bit
+// factors alone would not do: an error e in A0 grows by a² = 11.9 per step
+// relative to a small eigenvalue, and single fp16 (bf16) factors leave 6-33 %
+// (more) error in the result on ill-conditioned heads.  So A, B, C = B·A and Q
+// are kept as fp16 pairs hi + lo (22 bits) and each product is three tensor-core
+// products hi·hi + hi·lo + lo·hi in one fp32 accumulator; A is held scaled by
+// DP so that its average diagonal is 1 and lo stays clear of fp16's subnormals.
+// Q enters the last product as two terms of G's type.  The result is then within
+// its bf16 rounding of the exact one for Gaussian, ill-conditioned (1e5) and
+// rank-deficient heads.  fp16's range bounds Q, at most a^steps = 3.4445^steps:
+// steps <= 8.
+//
+// d is padded to DP = 64 or 128 by TMA's zero fill; padded rows and columns of A
+// stay zero and change nothing.  tcgen05.mma always runs M = 128 here: with DP =
+// 64 its upper 64 rows read whatever follows in shared memory and land in
+// accumulator rows nobody reads.
+#pragma once
+#include <cuda.h>
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cstdint>
+
+#include "fm_ptx.cuh"
+#include "muon_elementwise.cuh"
+#include "ns_gemm_sm100.cuh"
+#include "ns_prep.cuh"
+
+namespace fm {
+
+// 4-D tile load: (inner, outer, head, matrix).
+__device__ __forceinline__ void tma_load_4d(void* smem_dst, const CUtensorMap* map, uint64_t* bar,
+                                            int c0, int c1, int c2, int c3) {
+  asm volatile(
+      "cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes"
+      " [%0], [%1, {%3, %4, %5, %6}], [%2];" ::"r"(smem_u32(smem_dst)),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(smem_u32(bar)), "r"(c0), "r"(c1), "r"(c2), "r"(c3)
+      : "memory");
+}
+__device__ __forceinline__ void tma_store_4d(const CUtensorMap* map, const void* smem_src, int c0,
+                                             int c1, int c2, int c3) {
+  asm volatile(
+      "cp.async.bulk.tensor.4d.global.shared::cta.tile.bulk_group [%0, {%2, %3, %4, %5}], [%1];" ::
+          "l"(reinterpret_cast<uint64_t>(map)),
+      "r"(smem_u32(smem_src)), "r"(c0), "r"(c1), "r"(c2), "r"(c3)
+      : "memory");
+}
+
+// Instruction descriptor of kind::f16 with both operands fp16 (`half`) or bf16.
+__host__ __device__ constexpr uint32_t make_idesc_16(bool half, int M, int N, int a_mn, int b_mn) {
+  return half ? make_idesc_bf16(M, N, a_mn, b_mn) & ~((7u << 7) | (7u << 10))
+              : make_idesc_bf16(M, N, a_mn, b_mn);
+}
+
+constexpr int kHeadsMaxDim = 128;
+constexpr int kHeadsMaxSteps = 8;
+constexpr int kHeadsK = 64;        // reduction columns per gram stage (one swizzle row)
+constexpr int kGramStages = 6;
+constexpr int kGramThreads = 192;  // producer, MMA, 4 epilogue warps
+constexpr int kIterThreads = 288;  // 8 epilogue warps, MMA
+constexpr int kApplyN = 128;       // long-side elements per apply unit
+constexpr int kApplyStages = 3;
+constexpr int kApplyThreads = 320; // 8 epilogue warps, producer, MMA
+
+// Index of element (row 32q + lane, col) in a stored DP x DP fp32 partial: a
+// warp's access to one column is 128 contiguous bytes.
+template <int DP>
+__device__ __forceinline__ int gram_index(int q, int col, int lane) {
+  return (q * DP + col) * 32 + lane;
+}
+
+struct HeadsArgs {
+  int d, n;          // head side, long side
+  int heads;         // per matrix
+  int total;         // heads x matrices
+  int kblocks;       // ceil(n / kHeadsK)
+  int split, kbps;   // gram: splits per head, k-blocks per split
+  int steps;
+  float* gram;       // total x split x DP x DP
+  void* q;           // total x 2 x DP x DP of G's type
+  float* inv;        // total: 1/(‖G‖+1e-7)
+  __nv_bfloat16* out;
+  long long out_ld, out_head, out_mat;  // strides of out: row, head, matrix (elements)
+  int chunks;        // apply: ceil(n / kApplyN)
+  int tma_out;
+  unsigned* err;
+};
+
+// ------------------------------------------------------------------- gram
+template <int DP>
+struct GramCfg {
+  static constexpr int kStage = DP * kHeadsK * 2;
+  // MMAs of M = 128 on DP = 64 read one stage past the last
+  static constexpr int kSmem = (kGramStages + (DP == 64 ? 1 : 0)) * kStage + 1024 + 256;
+};
+
+// COLS: heads are column blocks (the head side is contiguous in memory), so the
+// operands are MN-major: a stage holds 64 long-side rows of DP columns.
+template <int DP, bool COLS, bool HALF>
+__global__ void __launch_bounds__(kGramThreads)
+    heads_gram_kernel(const __grid_constant__ CUtensorMap tm, const HeadsArgs g) {
+  extern __shared__ __align__(1024) uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
+                                             ~static_cast<uintptr_t>(1023));
+  constexpr int kStage = GramCfg<DP>::kStage;
+  uint64_t* full = reinterpret_cast<uint64_t*>(smem + (kGramStages + (DP == 64 ? 1 : 0)) * kStage);
+  uint64_t* empty = full + kGramStages;
+  uint64_t* acc_bar = empty + kGramStages;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(acc_bar + 1);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < kGramStages; ++s) {
+      mbar_init(&full[s], 1);
+      mbar_init(&empty[s], 1);
+    }
+    mbar_init(acc_bar, 1);
+    *abort_flag = 0;
+    fence_barrier_init();
+    tma_prefetch_desc(&tm);
+  }
+  if (warp == 1) {
+    tmem_alloc(tmem_slot, DP);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+  pdl_wait();
+
+  const int unit = blockIdx.x;
+  const int head = unit / g.split, sp = unit - head * g.split;
+  const int kb0 = sp * g.kbps, kb1 = min(g.kblocks, kb0 + g.kbps);
+  const int h = head % g.heads, mat = head / g.heads;
+  if (warp == 0) {
+    if (lane == 0) {
+      for (int kb = kb0; kb < kb1; ++kb) {
+        const int i = kb - kb0, s = i % kGramStages;
+        if (!mbar_wait(&empty[s], ((i / kGramStages) & 1) ^ 1, abort_flag, g.err, kErrWaitEmpty))
+          break;
+        mbar_arrive_expect_tx(&full[s], kStage);
+        uint8_t* dst = smem + s * kStage;
+        if constexpr (COLS) {
+#pragma unroll
+          for (int c = 0; c < DP / 64; ++c)
+            tma_load_4d(dst + c * (kHeadsK * 128), &tm, &full[s], c * 64, kb * kHeadsK, h, mat);
+        } else {
+          tma_load_4d(dst, &tm, &full[s], kb * kHeadsK, 0, h, mat);
+        }
+      }
+      pdl_trigger();
+    }
+  } else if (warp == 1) {
+    if (lane == 0) {
+      constexpr uint32_t idesc = make_idesc_16(HALF, 128, DP, COLS ? 1 : 0, COLS ? 1 : 0);
+      bool ok = true;
+      for (int kb = kb0; kb < kb1; ++kb) {
+        const int i = kb - kb0, s = i % kGramStages;
+        if (!mbar_wait(&full[s], (i / kGramStages) & 1, abort_flag, g.err, kErrWaitFull)) {
+          ok = false;
+          break;
+        }
+        tc_fence_after();
+        const uint32_t base = smem_u32(smem + s * kStage);
+#pragma unroll
+        for (int k = 0; k < kHeadsK / 16; ++k) {
+          // MN-major: 16 long-side rows are 2048 bytes, 64-column chunks 8 KB apart
+          const uint64_t desc = COLS ? make_sdesc_sw128(base + k * 2048, kHeadsK * 128, 1024)
+                                     : make_sdesc_sw128(base + k * 32, 16, 1024);
+          tc_mma_bf16(tmem, desc, desc, idesc, (i | k) != 0 ? 1u : 0u);
+        }
+        tc_commit(&empty[s]);
+      }
+      if (ok) tc_commit(acc_bar);
+    }
+  } else {
+    const int q = warp & 3;
+    if (q * 32 < DP && mbar_wait(acc_bar, 0, abort_flag, g.err, kErrWaitAccFull)) {
+      tc_fence_after();
+      float* dst = g.gram + static_cast<long long>(unit) * (DP * DP);
+#pragma unroll 1
+      for (int c = 0; c < DP / 32; ++c) {
+        float v[32];
+        tmem_ld_32x32b_x32(tmem + c * 32 + (static_cast<uint32_t>(q * 32) << 16), v);
+#pragma unroll
+        for (int k = 0; k < 32; ++k) __stcg(dst + gram_index<DP>(q, c * 32 + k, lane), v[k]);
+      }
+      tc_fence_before();
+    }
+    __syncwarp();
+  }
+  __syncthreads();
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc(tmem, DP);
+  }
+}
+
+// ---------------------------------------------------------------- iterate
+template <int DP>
+struct IterCfg {
+  static constexpr int kMat = DP * DP * 2;  // one 16-bit matrix: DP/64 k-blocks of DP rows
+  static constexpr int kPer = DP / 2;       // accumulator columns per epilogue thread
+  static constexpr int kWarps = 2 * (DP / 32);  // epilogue warps with rows to hold
+  static constexpr int kTmem = DP == 128 ? 512 : 256;
+  // A, B, Q as hi and lo; MMAs of M = 128 on DP = 64 read one matrix past the end
+  static constexpr int kSmem = 6 * kMat + (DP == 64 ? kMat : 0) + 1024 + 256;
+};
+
+// Sixteen bits hi, sixteen bits lo of 8 consecutive values into the swizzled
+// K-major operand: row r, columns 8·chunk.. of k-block kb.
+template <int DP>
+__device__ __forceinline__ void put_split8(uint8_t* hi, int r, int kb, int chunk, const float* v) {
+  const int off = kb * (DP * 128) + r * 128 + ((chunk ^ (r & 7)) << 4);
+  uint4 h, l;
+  __half2* hp = reinterpret_cast<__half2*>(&h);
+  __half2* lp = reinterpret_cast<__half2*>(&l);
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    hp[k] = __floats2half2_rn(v[2 * k], v[2 * k + 1]);
+    const float2 f = __half22float2(hp[k]);
+    lp[k] = __floats2half2_rn(v[2 * k] - f.x, v[2 * k + 1] - f.y);
+  }
+  *reinterpret_cast<uint4*>(hi + off) = h;
+  *reinterpret_cast<uint4*>(hi + IterCfg<DP>::kMat + off) = l;
+}
+
+template <int DP, bool HALF>
+__global__ void __launch_bounds__(kIterThreads, 1) heads_iterate_kernel(const HeadsArgs g) {
+  using Cfg = IterCfg<DP>;
+  extern __shared__ __align__(1024) uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
+                                             ~static_cast<uintptr_t>(1023));
+  uint8_t* sA = smem;                  // hi, lo
+  uint8_t* sB = smem + 2 * Cfg::kMat;
+  uint8_t* sQ = smem + 4 * Cfg::kMat;
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + Cfg::kSmem - 1024 - 256);
+  uint64_t* op_a = bars;       // operand A (or C in its place) written
+  uint64_t* op_b = bars + 1;
+  uint64_t* op_c = bars + 2;
+  uint64_t* acc_sq = bars + 3;  // A² ready
+  uint64_t* acc_c = bars + 4;   // B·A
+  uint64_t* acc_q = bars + 5;   // B·Q
+  uint64_t* acc_a = bars + 6;   // B·C
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 7);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+  float* s_tr = reinterpret_cast<float*>(tmem_slot + 2);  // one per epilogue warp
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int head = blockIdx.x;
+
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < 3; ++i) mbar_init(&bars[i], Cfg::kWarps);
+    for (int i = 3; i < 7; ++i) mbar_init(&bars[i], 1);
+    *abort_flag = 0;
+    fence_barrier_init();
+  }
+  if (warp == 8) {
+    tmem_alloc(tmem_slot, Cfg::kTmem);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+  const uint32_t d0 = tmem, d1 = tmem + DP, d2 = tmem + 2 * DP;
+  pdl_wait();
+  pdl_trigger();
+
+  // Epilogue warp: accumulator rows 32q.., columns col0 .. col0 + kPer - 1.
+  const int q = warp & 3, half = (warp >> 2) & 1;
+  const int row = q * 32 + lane, col0 = half * Cfg::kPer;
+  const bool worker = warp < 8 && q * 32 < DP;
+  constexpr float kScale = static_cast<float>(DP);  // A is held as DP·A
+  float a[Cfg::kPer];
+  if (worker) {
+    const float* src = g.gram + static_cast<long long>(head) * g.split * (DP * DP);
+#pragma unroll
+    for (int k = 0; k < Cfg::kPer; ++k) a[k] = __ldcg(src + gram_index<DP>(q, col0 + k, lane));
+    for (int s = 1; s < g.split; ++s) {
+      const float* ps = src + static_cast<long long>(s) * (DP * DP);
+#pragma unroll
+      for (int k = 0; k < Cfg::kPer; ++k) a[k] += __ldcg(ps + gram_index<DP>(q, col0 + k, lane));
+    }
+    float tr = 0.f;
+#pragma unroll
+    for (int k = 0; k < Cfg::kPer; ++k) tr += col0 + k == row ? a[k] : 0.f;
+    tr = warp_sum(tr);
+    if (lane == 0) s_tr[warp] = tr;
+  }
+  __syncthreads();
+
+  if (worker) {
+    float tr = 0.f;
+#pragma unroll
+    for (int w = 0; w < 8; ++w) tr += (w & 3) * 32 < DP ? s_tr[w] : 0.f;
+    const float inv = 1.f / (sqrtf(tr) + 1e-7f);
+    if (threadIdx.x == 0) g.inv[head] = inv;
+    // inv twice: inv² alone may leave fp32's range where A does not
+#pragma unroll
+    for (int k = 0; k < Cfg::kPer; ++k) a[k] = a[k] * inv * (inv * kScale);
+
+    const uint32_t lane_off = static_cast<uint32_t>(q * 32) << 16;
+    constexpr int kChunks = Cfg::kPer / 8;
+    const int kb = col0 / 64, chunk0 = (col0 % 64) / 8;
+    auto put = [&](uint8_t* dst, const float* v) {
+#pragma unroll
+      for (int c = 0; c < kChunks; ++c) put_split8<DP>(dst, row, kb, chunk0 + c, v + 8 * c);
+    };
+    auto ready = [&](uint64_t* bar) {
+      tc_fence_before();
+      fence_proxy_async_shared();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(bar);
+    };
+    float v[Cfg::kPer];
+    auto get = [&](uint32_t d) {
+      tc_fence_after();
+#pragma unroll
+      for (int c = 0; c < Cfg::kPer / 32; ++c) {
+        float t[32];
+        tmem_ld_32x32b_x32(d + col0 + c * 32 + lane_off, t);
+#pragma unroll
+        for (int k = 0; k < 32; ++k) v[32 * c + k] = t[k];
+      }
+    };
+    bool ok = true;
+    if (g.steps == 0) {
+#pragma unroll
+      for (int k = 0; k < Cfg::kPer; ++k) v[k] = col0 + k == row ? 1.f : 0.f;
+    } else {
+      put(sA, a);
+      ready(op_a);
+    }
+#pragma unroll 1
+    for (int it = 0; it < g.steps && ok; ++it) {
+      const bool last = it == g.steps - 1;
+      const uint32_t ph = it & 1;
+      if (!(ok = mbar_wait(acc_sq, ph, abort_flag, g.err, kErrWaitAccFull))) break;
+      get(d0);
+#pragma unroll
+      for (int k = 0; k < Cfg::kPer; ++k) {
+        v[k] = fmaf(kNsC / (kScale * kScale), v[k], (kNsB / kScale) * a[k]);
+        if (col0 + k == row) v[k] += kNsA;
+      }
+      if (it == 0 && last) break;  // Q = B
+      put(sB, v);
+      if (it == 0) put(sQ, v);
+      ready(op_b);
+      if (!last) {
+        if (!(ok = mbar_wait(acc_c, ph, abort_flag, g.err, kErrWaitAccFull))) break;
+        get(d1);
+        put(sA, v);
+        ready(op_c);
+      }
+      if (it > 0) {
+        if (!(ok = mbar_wait(acc_q, ph ^ 1, abort_flag, g.err, kErrWaitAccFull))) break;
+        get(d2);
+        if (last) break;  // Q is complete
+        put(sQ, v);
+      }
+      if (!(ok = mbar_wait(acc_a, ph, abort_flag, g.err, kErrWaitAccFull))) break;
+      get(d0);
+#pragma unroll
+      for (int k = 0; k < Cfg::kPer; ++k) a[k] = v[k];
+      put(sA, a);
+      ready(op_a);
+    }
+    if (ok) {
+      // Q as two terms of G's type, row-major.
+      uint16_t* dst = static_cast<uint16_t*>(g.q) +
+                      static_cast<long long>(head) * (2 * DP * DP) + row * DP + col0;
+#pragma unroll
+      for (int c = 0; c < kChunks; ++c) {
+        uint16_t h[8], l[8];
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+          const float x = v[8 * c + k];
+          if constexpr (HALF) {
+            const __half t = __float2half_rn(x);
+            h[k] = __half_as_ushort(t);
+            l[k] = __half_as_ushort(__float2half_rn(x - __half2float(t)));
+          } else {
+            const __nv_bfloat16 t = __float2bfloat16_rn(x);
+            h[k] = __bfloat16_as_ushort(t);
+            l[k] = __bfloat16_as_ushort(__float2bfloat16_rn(x - __bfloat162float(t)));
+          }
+        }
+        uint4 hv, lv;
+        uint32_t* hw = reinterpret_cast<uint32_t*>(&hv);
+        uint32_t* lw = reinterpret_cast<uint32_t*>(&lv);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          hw[k] = h[2 * k] | (static_cast<uint32_t>(h[2 * k + 1]) << 16);
+          lw[k] = l[2 * k] | (static_cast<uint32_t>(l[2 * k + 1]) << 16);
+        }
+        reinterpret_cast<uint4*>(dst)[c] = hv;
+        reinterpret_cast<uint4*>(dst + DP * DP)[c] = lv;
+      }
+    }
+    tc_fence_before();
+  } else if (warp == 8 && lane == 0) {
+    constexpr uint32_t idesc = make_idesc_16(true, 128, DP, 0, 0);
+    // D = X·Y (Y symmetric): hi·hi + hi·lo + lo·hi
+    auto product = [&](uint32_t d, const uint8_t* x, const uint8_t* y) {
+      const uint32_t xb = smem_u32(x), yb = smem_u32(y);
+#pragma unroll
+      for (int t = 0; t < 3; ++t) {
+        const uint32_t xo = xb + (t == 2 ? Cfg::kMat : 0), yo = yb + (t == 1 ? Cfg::kMat : 0);
+#pragma unroll
+        for (int k = 0; k < DP / 16; ++k) {
+          const uint32_t off = (k / 4) * (DP * 128) + (k % 4) * 32;
+          tc_mma_bf16(d, make_sdesc_sw128(xo + off, 16, 1024), make_sdesc_sw128(yo + off, 16, 1024),
+                      idesc, (t | k) != 0 ? 1u : 0u);
+        }
+      }
+    };
+    for (int it = 0; it < g.steps; ++it) {
+      const bool last = it == g.steps - 1;
+      const uint32_t ph = it & 1;
+      if (!mbar_wait(op_a, ph, abort_flag, g.err, kErrWaitFull)) break;
+      tc_fence_after();
+      product(d0, sA, sA);
+      tc_commit(acc_sq);
+      if (it == 0 && last) break;
+      if (!mbar_wait(op_b, ph, abort_flag, g.err, kErrWaitFull)) break;
+      tc_fence_after();
+      if (!last) {
+        product(d1, sB, sA);
+        tc_commit(acc_c);
+      }
+      if (it > 0) {
+        product(d2, sB, sQ);
+        tc_commit(acc_q);
+      }
+      if (!last) {
+        if (!mbar_wait(op_c, ph, abort_flag, g.err, kErrWaitFull)) break;
+        tc_fence_after();
+        product(d0, sB, sA);
+        tc_commit(acc_a);
+      }
+    }
+  }
+  __syncthreads();
+  if (warp == 8) {
+    tc_fence_after();
+    tmem_dealloc(tmem, Cfg::kTmem);
+  }
+}
+
+// ------------------------------------------------------------------ apply
+template <int DP>
+struct ApplyCfg {
+  static constexpr int kStage = DP * kApplyN * 2;
+  static constexpr int kQ = 2 * DP * DP * 2;          // both terms of one head
+  static constexpr int kStaging = 8 * 32 * 64 * 2 * 2;  // per epilogue warp: two 32 x 64 blocks
+  static constexpr int kSmem = kApplyStages * kStage + kQ + (DP == 64 ? DP * 128 : 0) + kStaging +
+                               1024 + 256;
+};
+
+// Stores one staged 32 x 64 bf16 block (128-byte rows, 16-byte chunks XORed
+// with row & 7) element by element, a row per instruction.
+__device__ __forceinline__ void store_block_plain(const uint8_t* blk, __nv_bfloat16* dst,
+                                                  long long ld, int rows, int cols, int lane) {
+  for (int r = 0; r < rows; ++r) {
+#pragma unroll
+    for (int p = 0; p < 2; ++p) {
+      const int c = p * 32 + lane;
+      if (c < cols)
+        dst[r * ld + c] = *reinterpret_cast<const __nv_bfloat16*>(
+            blk + r * 128 + (((c >> 3) ^ (r & 7)) << 4) + (c & 7) * 2);
+    }
+  }
+}
+
+// Units are (head, chunk of 128 long-side elements), walked by contiguous
+// ranges so that a block loads a head's Q once or twice.  Row heads: D = Q·G
+// (rows of the head x 128 columns).  Column heads: D = G·Q (128 rows x columns
+// of the head), Q being symmetric.
+template <int DP, bool COLS, bool HALF>
+__global__ void __launch_bounds__(kApplyThreads, 1)
+    heads_apply_kernel(const __grid_constant__ CUtensorMap tmG,
+                       const __grid_constant__ CUtensorMap tmQ,
+                       const __grid_constant__ CUtensorMap tmO, const HeadsArgs g) {
+  using Cfg = ApplyCfg<DP>;
+  extern __shared__ __align__(1024) uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
+                                             ~static_cast<uintptr_t>(1023));
+  uint8_t* sG = smem;
+  uint8_t* sQ = smem + kApplyStages * Cfg::kStage;
+  uint8_t* staging = sQ + Cfg::kQ + (DP == 64 ? DP * 128 : 0);
+  uint64_t* full = reinterpret_cast<uint64_t*>(staging + Cfg::kStaging);
+  uint64_t* empty = full + kApplyStages;
+  uint64_t* q_full = empty + kApplyStages;
+  uint64_t* q_empty = q_full + 1;
+  uint64_t* accf = q_empty + 1;  // [2]
+  uint64_t* acce = accf + 2;     // [2]
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(acce + 2);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  constexpr int kAccWarps = COLS ? 8 : 2 * (DP / 32);  // epilogue warps that drain an accumulator
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < kApplyStages; ++s) {
+      mbar_init(&full[s], 1);
+      mbar_init(&empty[s], 1);
+    }
+    mbar_init(q_full, 1);
+    mbar_init(q_empty, 1);
+    for (int s = 0; s < 2; ++s) {
+      mbar_init(&accf[s], 1);
+      mbar_init(&acce[s], kAccWarps);
+    }
+    *abort_flag = 0;
+    fence_barrier_init();
+    tma_prefetch_desc(&tmG);
+    tma_prefetch_desc(&tmQ);
+  }
+  if (warp == 9) {
+    tmem_alloc(tmem_slot, 256);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+
+  const long long units = static_cast<long long>(g.total) * g.chunks;
+  const long long u0 = units * blockIdx.x / gridDim.x, u1 = units * (blockIdx.x + 1) / gridDim.x;
+
+  if (warp == 8) {
+    // producer
+    if (lane == 0) {
+      int head_in = -1;
+      uint32_t q_phase = 0;
+      int i = 0;
+      pdl_wait();
+      for (long long u = u0; u < u1; ++u, ++i) {
+        const int head = static_cast<int>(u / g.chunks), chunk = static_cast<int>(u % g.chunks);
+        const int h = head % g.heads, mat = head / g.heads;
+        if (head != head_in) {
+          if (!mbar_wait(q_empty, q_phase ^ 1, abort_flag, g.err, kErrWaitEmpty)) break;
+          mbar_arrive_expect_tx(q_full, Cfg::kQ);
+#pragma unroll
+          for (int t = 0; t < 2; ++t)
+#pragma unroll
+            for (int kb = 0; kb < DP / 64; ++kb)
+              tma_load_3d(sQ + (t * (DP / 64) + kb) * (DP * 128), &tmQ, q_full, kb * 64, t * DP,
+                          head);
+          q_phase ^= 1;
+          head_in = head;
+        }
+        const int s = i % kApplyStages;
+        if (!mbar_wait(&empty[s], ((i / kApplyStages) & 1) ^ 1, abort_flag, g.err, kErrWaitEmpty))
+          break;
+        mbar_arrive_expect_tx(&full[s], Cfg::kStage);
+        uint8_t* dst = sG + s * Cfg::kStage;
+        if constexpr (COLS) {
+#pragma unroll
+          for (int c = 0; c < DP / 64; ++c)
+            tma_load_4d(dst + c * (kApplyN * 128), &tmG, &full[s], c * 64, chunk * kApplyN, h, mat);
+        } else {
+#pragma unroll
+          for (int c = 0; c < kApplyN / 64; ++c)
+            tma_load_4d(dst + c * (DP * 128), &tmG, &full[s], chunk * kApplyN + c * 64, 0, h, mat);
+        }
+      }
+    }
+  } else if (warp == 9) {
+    // MMA issuer
+    if (lane == 0) {
+      constexpr uint32_t idesc = COLS ? make_idesc_16(HALF, 128, DP, 0, 0)
+                                      : make_idesc_16(HALF, 128, kApplyN, 0, 1);
+      int head_in = -1;
+      uint32_t q_phase = 0;
+      int i = 0;
+      for (long long u = u0; u < u1; ++u, ++i) {
+        const int head = static_cast<int>(u / g.chunks);
+        if (head != head_in) {
+          // the previous head's MMAs have read its Q once they complete
+          if (head_in >= 0) tc_commit(q_empty);
+          if (!mbar_wait(q_full, q_phase, abort_flag, g.err, kErrWaitFull)) break;
+          q_phase ^= 1;
+          head_in = head;
+        }
+        const int acc = i & 1, s = i % kApplyStages;
+        if (!mbar_wait(&acce[acc], ((i >> 1) & 1) ^ 1, abort_flag, g.err, kErrWaitAccEmpty)) break;
+        if (!mbar_wait(&full[s], (i / kApplyStages) & 1, abort_flag, g.err, kErrWaitFull)) break;
+        tc_fence_after();
+        const uint32_t gb = smem_u32(sG + s * Cfg::kStage), qb = smem_u32(sQ);
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+#pragma unroll
+          for (int k = 0; k < DP / 16; ++k) {
+            const uint64_t qd = make_sdesc_sw128(
+                qb + t * (DP * DP * 2) + (k / 4) * (DP * 128) + (k % 4) * 32, 16, 1024);
+            const uint32_t first = (t | k) != 0 ? 1u : 0u;
+            if constexpr (COLS) {
+              const uint64_t gd =
+                  make_sdesc_sw128(gb + (k / 4) * (kApplyN * 128) + (k % 4) * 32, 16, 1024);
+              tc_mma_bf16(tmem + acc * 128, gd, qd, idesc, first);
+            } else {
+              // MN-major: 16 head rows are 2048 bytes, 64-column chunks DP rows apart
+              const uint64_t gd = make_sdesc_sw128(gb + k * 2048, DP * 128, 1024);
+              tc_mma_bf16(tmem + acc * 128, qd, gd, idesc, first);
+            }
+          }
+        }
+        tc_commit(&empty[s]);
+        tc_commit(&accf[acc]);
+      }
+    }
+  } else {
+    // epilogue: rows 32q.. of the accumulator, columns 64·(warp / 4)..
+    const int q = warp & 3, half = warp >> 2;
+    const bool worker = COLS ? half * 64 < DP : q * 32 < DP;
+    pdl_wait();
+    if (worker || COLS) {
+      uint8_t* buf = staging + warp * (32 * 64 * 2 * 2);
+      int i = 0;
+      for (long long u = u0; u < u1; ++u, ++i) {
+        const int head = static_cast<int>(u / g.chunks), chunk = static_cast<int>(u % g.chunks);
+        const int h = head % g.heads, mat = head / g.heads;
+        const int acc = i & 1;
+        // the block's place in the output: rows r0.., columns c0.. of the head
+        const int r0 = COLS ? chunk * kApplyN + q * 32 : q * 32;
+        const int c0 = COLS ? half * 64 : chunk * kApplyN + half * 64;
+        const int rows = min(32, (COLS ? g.n : g.d) - r0), cols = min(64, (COLS ? g.d : g.n) - c0);
+        const float inv = __ldcg(g.inv + head);
+        if (!mbar_wait(&accf[acc], (i >> 1) & 1, abort_flag, g.err, kErrWaitAccFull)) break;
+        tc_fence_after();
+        const bool any = worker && rows > 0 && cols > 0;
+        uint8_t* blk = buf + (i & 1) * (32 * 64 * 2);
+        if (any) {
+          float v[2][32];
+#pragma unroll
+          for (int c = 0; c < 2; ++c)
+            tmem_ld_32x32b_x32(
+                tmem + acc * 128 + half * 64 + c * 32 + (static_cast<uint32_t>(q * 32) << 16), v[c]);
+          if (g.tma_out) {
+            if (lane == 0) bulk_wait_read<1>();  // the block of two units ago has been read
+            __syncwarp();
+          }
+#pragma unroll
+          for (int c = 0; c < 8; ++c) {
+            float t[8];
+#pragma unroll
+            for (int k = 0; k < 8; ++k) t[k] = v[c / 4][(c % 4) * 8 + k] * inv;
+            *reinterpret_cast<uint4*>(blk + lane * 128 + ((c ^ (lane & 7)) << 4)) = pack8_bf16(t);
+          }
+        }
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&acce[acc]);
+        if (any) {
+          if (g.tma_out) {
+            fence_proxy_async_shared();
+            __syncwarp();
+            if (lane == 0) {
+              tma_store_4d(&tmO, blk, c0, r0, h, mat);
+              bulk_commit();
+            }
+          } else {
+            store_block_plain(blk,
+                              g.out + mat * g.out_mat + h * g.out_head + r0 * g.out_ld + c0,
+                              g.out_ld, rows, cols, lane);
+            __syncwarp();
+          }
+        }
+      }
+      if (lane == 0) bulk_wait_all();
+      __syncwarp();
+    }
+  }
+  __syncthreads();
+  if (warp == 9) {
+    tc_fence_after();
+    tmem_dealloc(tmem, 256);
+  }
+}
+
+// ------------------------------------------------------------------- pack
+// Copy of G that TMA can address, for inputs it cannot (other types, unaligned
+// rows or heads): outer x inner blocks per head with a row stride of ld
+// elements, values rounded to T.  Padding columns are never read.
+template <typename T>
+__global__ void __launch_bounds__(256)
+    heads_pack_kernel(const void* __restrict__ G, int dtype, long long ldg, long long mat_stride,
+                      int heads, long long head_stride, long long outer, int inner, T* dst,
+                      long long ld) {
+  pdl_wait();
+  const int head = blockIdx.y;
+  const long long base = (head / heads) * mat_stride + (head % heads) * head_stride;
+  T* out = dst + head * outer * ld;
+  for (long long r = blockIdx.x; r < outer; r += gridDim.x) {
+    for (int c = threadIdx.x; c < inner; c += blockDim.x) {
+      const long long i = base + r * ldg + c;
+      float x;
+      if (dtype == 0) x = __bfloat162float(static_cast<const __nv_bfloat16*>(G)[i]);
+      else if (dtype == 1) x = __half2float(static_cast<const __half*>(G)[i]);
+      else if (dtype == 2) x = static_cast<const float*>(G)[i];
+      else x = __bfloat162float(__double2bfloat16(static_cast<const double*>(G)[i]));
+      out[r * ld + c] = from_f<T>(x);
+    }
+  }
+}
+
+}  // namespace fm

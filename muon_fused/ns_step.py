@@ -46,3 +46,83 @@ def fused_newton_schulz(
         raise RuntimeError(
             "fused_newton_schulz needs a CUDA tensor; this build has no CPU fallback")
     return _C.fused_newton_schulz(G, steps, workspace)
+
+
+def _check_heads(shape, heads: int, dim: int) -> int:
+    """Width of a head; raises where the projection does not divide into heads."""
+    if dim not in (0, 1):
+        raise RuntimeError(f"dim must be 0 (heads are rows) or 1 (columns), got {dim}")
+    side = int(shape[-2 + dim])
+    if heads < 1 or side % heads:
+        raise RuntimeError(f"{side} {'columns' if dim else 'rows'} do not divide into {heads} heads")
+    return side // heads
+
+
+def _heads_gram_form(d: int, steps: int) -> bool:
+    """Whether the per-head kernels take a head of width d: they hold d x d
+    matrices of at most 128 on chip, with fp16's range for 3.4445^steps."""
+    return d <= 128 and steps <= 8
+
+
+def workspace_size_heads(shape, heads: int, *, dim: int = 0, steps: int = 5) -> int:
+    """Bytes of device workspace ``fused_newton_schulz_heads`` needs for a
+    (rows, cols) or (batch, rows, cols) projection."""
+    d = _check_heads(shape, heads, dim)
+    batch = int(shape[0]) if len(shape) == 3 else 1
+    rows, cols = int(shape[-2]), int(shape[-1])
+    if _heads_gram_form(d, steps):
+        return _C.workspace_size_heads(batch, rows, cols, heads, dim)
+    return _C.workspace_size_batched(batch * heads, d, cols if dim == 0 else rows)
+
+
+def fused_newton_schulz_heads(
+    G: torch.Tensor,
+    heads: int,
+    steps: int = 5,
+    workspace: torch.Tensor | None = None,
+    *,
+    dim: int = 0,
+    out: torch.Tensor | None = None,
+) -> torch.Tensor:
+    """Newton-Schulz of every attention head of a projection by itself.
+
+    A head is a block of ``rows / heads`` rows (``dim=0``: query, key and value
+    projections, one matrix or fused) or of ``cols / heads`` columns (``dim=1``:
+    output projection); each is normalised by its own Frobenius norm and
+    orthogonalised as ``fused_newton_schulz`` does a matrix.  Returns bf16 with
+    ``G``'s shape.
+
+    Heads up to 128 wide (and up to 8 steps) iterate on head x head matrices
+    in split fp16: the result is the exact one up to its bf16 rounding, on
+    ill-conditioned heads too.  Wider heads run as a batch of matrices on the
+    bf16 path of ``fused_newton_schulz``.
+
+    Args:
+        G: CUDA tensor (rows, cols), or (batch, rows, cols) for same-shape
+            projections, of any floating dtype.  fp32 and fp64 are rounded to
+            bf16 first, as in ``fused_newton_schulz``; bf16 and, for heads up
+            to 128, fp16 are taken as they are.
+        heads: heads per projection.
+        steps: number of iterations (default 5).
+        workspace: optional pre-allocated CUDA buffer of at least
+            ``workspace_size_heads(G.shape, heads, dim=dim, steps=steps)`` bytes.
+        dim: 0 where heads are blocks of rows, 1 where of columns.
+        out: optional contiguous bf16 tensor of ``G``'s shape for the result;
+            must not share memory with ``G``.
+    """
+    assert G.ndim in (2, 3), f"Expected a 2-D or 3-D tensor, got {G.ndim}-D"
+    if not G.is_cuda:
+        raise RuntimeError(
+            "fused_newton_schulz_heads needs a CUDA tensor; this build has no CPU fallback")
+    d = _check_heads(G.shape, heads, dim)
+    if _heads_gram_form(d, steps):
+        return _C.newton_schulz_heads(G, heads, steps, dim, workspace, out)
+    blocks = G.unflatten(G.ndim - 2 + dim, (heads, d))
+    if dim == 1:
+        blocks = blocks.movedim(-2, -3)  # heads before rows
+    res = _C.fused_newton_schulz_batched(blocks.reshape(-1, *blocks.shape[-2:]), steps, workspace)
+    res = res.view(blocks.shape)
+    if dim == 1:
+        res = res.movedim(-3, -2)
+    res = res.reshape(G.shape)
+    return res if out is None else out.copy_(res)

@@ -1,0 +1,264 @@
+"""fused_newton_schulz_heads on the GPU against its definition in 64 bits.
+
+Tolerances.  The output's own rounding is half a bf16 step, 2^-8 of each value,
+so at most 2^-8 in the Frobenius norm.  Before it: A and Q carry 22 bits, and an
+error of A relative to a small eigenvalue grows by 3.4445² a step, 2^-22·11.9^4 =
+5e-3 at worst in directions that start at 1e-4 of the largest, which hold a
+small part of the norm; Q enters the last product with 17 bits, 2^-17·3.4445^5 =
+4e-3 of such a direction again.  Together under 1e-3 of the whole norm: gate
+2^-8 + 1e-3.  Single elements: their rounding, and 4e-3 of the largest value.
+"""
+
+import math
+
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+DEV = "cuda"
+A, B, C = 3.4445, -4.7750, 2.0315
+FRO = 2.0 ** -8 + 1e-3
+
+
+def ref64(G, heads, steps, dim):
+    g = (G if G.dim() == 3 else G[None]).double()
+    x = torch.stack(g.chunk(heads, 1 + dim), 1)
+    x = x / (x.flatten(2).norm(dim=2)[..., None, None] + 1e-7)
+    for _ in range(steps):
+        a = x @ x.mT if dim == 0 else x.mT @ x
+        p = B * a + C * (a @ a)
+        x = A * x + (p @ x if dim == 0 else x @ p)
+    return torch.cat(x.unbind(1), 1 + dim).reshape(G.shape)
+
+
+def check(out, G, heads, steps, dim, fro=FRO):
+    assert out.dtype == torch.bfloat16 and out.shape == G.shape
+    ref = ref64(G, heads, steps, dim)
+    diff = out.double() - ref
+    blocks = torch.stack((diff if diff.dim() == 3 else diff[None]).chunk(heads, 1 + dim), 1)
+    rblocks = torch.stack((ref if ref.dim() == 3 else ref[None]).chunk(heads, 1 + dim), 1)
+    rel = blocks.flatten(2).norm(dim=2) / rblocks.flatten(2).norm(dim=2).clamp_min(1e-30)
+    assert float(rel.max()) <= fro, (float(rel.max()), int(rel.argmax()))
+    big = float(ref.abs().max())
+    assert bool((diff.abs() <= 2.0 ** -8 * ref.abs() + 4e-3 * big).all()), float(diff.abs().max()) / big
+
+
+def rand(shape, seed, dtype=torch.bfloat16):
+    return torch.randn(shape, generator=torch.Generator().manual_seed(seed)).to(dtype).to(DEV)
+
+
+@pytest.mark.parametrize("d,n", [(128, 512), (64, 512), (128, 4096), (64, 64), (96, 200), (16, 72),
+                                 (8, 1024), (128, 8), (72, 1000), (32, 2304), (112, 65)])
+@pytest.mark.parametrize("dim", [0, 1])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_aligned(cuda_lib, d, n, dim, dtype):
+    from muon_fused import fused_newton_schulz_heads
+
+    heads = 5
+    shape = (heads * d, n) if dim == 0 else (n, heads * d)
+    G = rand(shape, d + n, dtype)
+    check(fused_newton_schulz_heads(G, heads, dim=dim), G, heads, 5, dim)
+
+
+@pytest.mark.parametrize("d,n", [(1, 1), (1, 130), (3, 1), (37, 129), (65, 333), (127, 1001), (100, 7)])
+@pytest.mark.parametrize("dim", [0, 1])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_odd_sizes(cuda_lib, d, n, dim, dtype):
+    """Rows, heads and outputs off 16-byte boundaries (copied input, plain stores)."""
+    from muon_fused import fused_newton_schulz_heads
+
+    heads = 3
+    shape = (2, heads * d, n) if dim == 0 else (2, n, heads * d)
+    G = rand(shape, d * n, dtype)
+    check(fused_newton_schulz_heads(G, heads, dim=dim), G, heads, 5, dim)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float64])
+@pytest.mark.parametrize("dim", [0, 1])
+def test_wide_types_are_rounded_to_bf16_first(cuda_lib, dtype, dim):
+    from muon_fused import fused_newton_schulz_heads
+
+    G = rand((256, 192), 3, dtype)
+    out = fused_newton_schulz_heads(G, 2, dim=dim)
+    assert torch.equal(out, fused_newton_schulz_heads(G.bfloat16(), 2, dim=dim))
+
+
+@pytest.mark.parametrize("steps", [0, 1, 2, 3, 8])
+@pytest.mark.parametrize("d", [48, 128])
+def test_steps(cuda_lib, steps, d):
+    from muon_fused import fused_newton_schulz_heads
+
+    for dim in (0, 1):
+        G = rand((4 * d, 1024) if dim == 0 else (1024, 4 * d), steps)
+        check(fused_newton_schulz_heads(G, 4, steps, dim=dim), G, 4, steps, dim)
+
+
+@pytest.mark.parametrize("dim", [0, 1])
+@pytest.mark.parametrize("kind", ["cond1e2", "cond1e5", "rank8", "momentum"])
+def test_ill_conditioned_heads(cuda_lib, kind, dim):
+    """Where the bf16 iteration is off by 5 to 50 %."""
+    from muon_fused import fused_newton_schulz_heads
+
+    heads, d, n = 4, 128, 1024
+    gen = torch.Generator().manual_seed(1)
+    blocks = []
+    for _ in range(heads):
+        if kind.startswith("cond"):
+            u = torch.linalg.qr(torch.randn(d, d, generator=gen))[0]
+            v = torch.linalg.qr(torch.randn(n, d, generator=gen))[0]
+            x = (u * torch.logspace(0, -math.log10(float(kind[4:])), d)) @ v.T
+        elif kind == "rank8":
+            x = torch.randn(d, 8, generator=gen) @ torch.randn(8, n, generator=gen)
+        else:
+            s = 4.0 / torch.arange(1, 17)
+            x = 1e-3 * (torch.randn(d, n, generator=gen)
+                        + (torch.randn(d, 16, generator=gen) * s) @ torch.randn(16, n, generator=gen))
+        blocks.append(x)
+    G = torch.cat(blocks).bfloat16().to(DEV)
+    G = G if dim == 0 else G.T.contiguous()
+    check(fused_newton_schulz_heads(G, heads, dim=dim), G, heads, 5, dim)
+
+
+@pytest.mark.parametrize("dim", [0, 1])
+def test_scales_of_the_input(cuda_lib, dim):
+    """Gradients from 1e-10 to 1e4, a head of zeros among them."""
+    from muon_fused import fused_newton_schulz_heads
+
+    scale = torch.tensor([1e-10, 1e-5, 0.0, 1.0, 1e4], device=DEV).repeat_interleave(64)
+    G = rand((320, 512), 2, torch.float32) * scale[:, None]
+    G = (G if dim == 0 else G.T.contiguous()).bfloat16()
+    out = fused_newton_schulz_heads(G, 5, dim=dim)
+    check(out, G, 5, 5, dim)
+    assert not out.narrow(dim, 128, 64).any()
+
+
+@pytest.mark.parametrize("dim", [0, 1])
+@pytest.mark.parametrize("bad", [math.nan, math.inf])
+def test_nonfinite_stays_in_its_head(cuda_lib, dim, bad):
+    from muon_fused import fused_newton_schulz_heads
+
+    G = rand((3 * 80, 256), 5) if dim == 0 else rand((256, 3 * 80), 5)
+    clean = fused_newton_schulz_heads(G, 3, dim=dim)
+    G2 = G.clone()
+    G2.narrow(dim, 80, 80)[3, 5] = bad
+    out = fused_newton_schulz_heads(G2, 3, dim=dim)
+    for h in range(3):
+        got = out.narrow(dim, 80 * h, 80)
+        if h == 1:
+            assert bool(got.isnan().all())
+        else:
+            assert torch.equal(got, clean.narrow(dim, 80 * h, 80))
+
+
+@pytest.mark.parametrize("dim", [0, 1])
+def test_strides_batches_and_views(cuda_lib, dim):
+    """Row strides beyond the columns, batch strides, transposed inputs and
+    unaligned bases give what a contiguous copy gives."""
+    from muon_fused import fused_newton_schulz_heads
+
+    base = rand((3, 300, 400), 7)
+    views = [base[:, :256, :384], base[:, 4:260, 8:392], base[::2, :256, 3:387],
+             base.transpose(1, 2)[:, :384, :256].transpose(1, 2)[:, :256, :384], base[1, :256, :384]]
+    for v in views:
+        want = fused_newton_schulz_heads(v.contiguous(), 4, dim=dim)
+        assert torch.equal(fused_newton_schulz_heads(v, 4, dim=dim), want)
+        check(want, v, 4, 5, dim)
+
+
+def test_batch_equals_single_calls_bit_for_bit_without_splits(cuda_lib):
+    """200 heads fill the GPU without splitting the long side, as does one head
+    of 256 columns: same order of sums, same bits; and runs repeat."""
+    from muon_fused import fused_newton_schulz_heads
+
+    G = rand((50, 4 * 64, 256), 8)
+    out = fused_newton_schulz_heads(G, 4)
+    assert torch.equal(out, fused_newton_schulz_heads(G, 4))
+    for b in (0, 17, 49):
+        assert torch.equal(out[b], fused_newton_schulz_heads(G[b], 4))
+
+
+def test_many_heads_across_waves(cuda_lib):
+    from muon_fused import fused_newton_schulz_heads
+
+    for dim in (0, 1):
+        G = rand((6, 64 * 32, 192) if dim == 0 else (6, 192, 64 * 32), 9)
+        check(fused_newton_schulz_heads(G, 64, dim=dim), G, 64, 5, dim)
+
+
+@pytest.mark.parametrize("dim", [0, 1])
+def test_wide_heads_run_as_a_batch(cuda_lib, dim):
+    """Heads of 256: the bf16 path's accuracy (1e-2, as its own tests)."""
+    from muon_fused import fused_newton_schulz_heads
+
+    G = rand((512, 1024) if dim == 0 else (1024, 512), 10)
+    out = fused_newton_schulz_heads(G, 2, dim=dim)
+    ref = ref64(G, 2, 5, dim)
+    assert float((out.double() - ref).norm() / ref.norm()) <= 1e-2
+    buf = torch.empty_like(G)
+    assert fused_newton_schulz_heads(G, 2, dim=dim, out=buf) is buf and torch.equal(buf, out)
+
+
+def test_past_32_bit_offsets(cuda_lib):
+    """Five projections of 128 x 2^22 (2.7e9 elements): the last one's values."""
+    from muon_fused import fused_newton_schulz_heads
+
+    n = 1 << 22
+    G = torch.zeros(5, 128, n, dtype=torch.bfloat16, device=DEV)
+    G[4, :, -128:] = rand((128, 128), 11)
+    out = fused_newton_schulz_heads(G, 1)
+    assert not out[:4].any() and not out[4, :, :-128].any()
+    check(out[4, :, -128:].contiguous(), G[4, :, -128:].contiguous(), 1, 5, 0)
+
+
+def test_workspace_out_stream_and_refusals(cuda_lib):
+    from muon_fused import fused_newton_schulz_heads, workspace_size_heads
+
+    G = rand((256, 512), 12)
+    want = fused_newton_schulz_heads(G, 4)
+    ws = torch.empty(workspace_size_heads(G.shape, 4), dtype=torch.uint8, device=DEV)
+    out = torch.full((256, 512), 7.0, dtype=torch.bfloat16, device=DEV)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        got = fused_newton_schulz_heads(G, 4, workspace=ws, out=out)
+    torch.cuda.current_stream().wait_stream(side)
+    assert got is out and torch.equal(out, want)
+    small = torch.empty(16, dtype=torch.uint8, device=DEV)
+    assert torch.equal(fused_newton_schulz_heads(G, 4, workspace=small), want)
+    with pytest.raises(RuntimeError, match="share memory"):
+        fused_newton_schulz_heads(G, 4, out=G)
+    with pytest.raises(RuntimeError, match="out must be"):
+        fused_newton_schulz_heads(G, 4, out=out.float())
+    with pytest.raises(RuntimeError, match="divide"):
+        fused_newton_schulz_heads(G, 3)
+    with pytest.raises(RuntimeError, match="dim must be"):
+        fused_newton_schulz_heads(G, 4, dim=2)
+    with pytest.raises(RuntimeError, match="steps"):
+        fused_newton_schulz_heads(G, 4, -1)
+    with pytest.raises(RuntimeError, match="dtype"):
+        fused_newton_schulz_heads(G.int(), 4)
+    assert fused_newton_schulz_heads(G[:, :0], 4).shape == (256, 0)
+
+
+def test_no_device_error(cuda_lib):
+    from muon_fused import _lib
+
+    assert _lib.device_error() == 0
+
+
+@pytest.mark.parametrize("dim", [0, 1])
+def test_graph_replay(cuda_lib, dim):
+    from muon_fused import fused_newton_schulz_heads
+
+    G = rand((256, 320), 13)
+    fused_newton_schulz_heads(G, 4, dim=dim)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = fused_newton_schulz_heads(G, 4, dim=dim)
+    for seed in (14, 15):
+        G.copy_(rand((256, 320), seed))
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, fused_newton_schulz_heads(G.clone(), 4, dim=dim))
