@@ -197,8 +197,8 @@ int fm_newton_schulz_heads(const void* G, int dtype, int64_t batch, int64_t rows
  * FM_DT_F32 beside 16-bit parameters.  With equal types every op rounds to that
  * type as the reference's torch ops do (bit-identical results); 16-bit
  * parameters with fp32 moments are computed in fp32 and rounded once.  The
- * list is read during the call (host memory); tensors with n = 0 are skipped
- * and the tensors must not overlap.
+ * list is read during the call (host memory); tensors with n = 0 are skipped.
+ * What the call writes must not overlap any other of its tensors.
  * Replaces: muon_fused/optimizer.py:165-200 (nine torch ops per tensor).
  */
 typedef struct {
@@ -222,7 +222,7 @@ int fm_adamw(const fm_adamw_tensor* tensors, int64_t count, int dtype, int momen
  * type dtype (FM_DT_F32 / BF16 / F16) and, like update, rows x cols contiguous
  * elements; row_moment holds rows floats.  workspace: at least
  * fm_normed_workspace_size() bytes, 256-byte aligned.  The list is read during
- * the call; the matrices must not overlap.
+ * the call; what it writes must not overlap any other of its memory.
  * Replaces: nothing; it stands beside fm_muon_apply.
  */
 typedef struct {

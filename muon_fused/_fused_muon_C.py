@@ -8,6 +8,8 @@ All calls run on torch's current CUDA stream and never synchronise the host.
 
 from __future__ import annotations
 
+import contextlib
+
 import torch
 
 from muon_fused import _lib
@@ -22,6 +24,14 @@ _DTYPE_CODE = {
 
 def _stream(t: torch.Tensor) -> int:
     return torch.cuda.current_stream(t.device).cuda_stream
+
+
+_HERE = contextlib.nullcontext()
+
+
+def _on_device(t: torch.Tensor):
+    """Context in which t's device is current (nothing to do where it is)."""
+    return _HERE if t.device.index == torch.cuda.current_device() else torch.cuda.device(t.device)
 
 
 def _check_cuda(t: torch.Tensor, name: str) -> None:
@@ -154,7 +164,7 @@ def newton_schulz_heads(G: torch.Tensor, heads: int, steps: int = 5, dim: int = 
             raise RuntimeError("workspace must be on the same device as the input")
         if workspace.nbytes < need:
             workspace = torch.empty(need, dtype=torch.uint8, device=G.device)
-    with torch.cuda.device(G.device):
+    with _on_device(G):
         _lib.check(
             _lib.load().fm_newton_schulz_heads(
                 G.data_ptr(), _DTYPE_CODE[G.dtype], batch, rows, cols, ld, bs, int(heads), int(dim),

@@ -15,6 +15,7 @@
 #include <cstdint>
 
 #include "fm_ptx.cuh"
+#include "adamw_list.cuh"
 #include "muon_elementwise.cuh"
 #include "ns_prep.cuh"
 
@@ -22,7 +23,9 @@ namespace fm {
 
 constexpr int kNormedThreads = 256;
 constexpr int kNormedList = 64;        // matrices per launch
-constexpr int kNormedMaxBlocks = 1184; // row blocks per matrix = F² partials per matrix
+constexpr int kNormedMaxBlocks = 592;  // row blocks per matrix = F² partials per matrix
+constexpr int kNormedUnits = 2;        // apply: 4-element units per thread
+constexpr int kNormedChunk = kNormedThreads * 4 * kNormedUnits;  // elements per apply block
 
 struct NormedEntry {
   void* p;
@@ -59,15 +62,16 @@ __device__ __forceinline__ float row_sumsq(const __nv_bfloat16* row, long long c
   const long long vecs = (cols - head) / 8;
   const uint4* q = reinterpret_cast<const uint4*>(row + head);
   float acc[4] = {0.f, 0.f, 0.f, 0.f};
-  long long i = t;
-  for (; i + 3ll * width < vecs; i += 4ll * width) {
-    uint4 a[4];
+  for (long long i = t; i < vecs; i += 8ll * width) {
+    uint4 a[8];
 #pragma unroll
-    for (int k = 0; k < 4; ++k) a[k] = __ldg(q + i + static_cast<long long>(k) * width);
+    for (int k = 0; k < 8; ++k) {
+      const long long j = i + static_cast<long long>(k) * width;
+      a[k] = j < vecs ? __ldg(q + j) : make_uint4(0u, 0u, 0u, 0u);
+    }
 #pragma unroll
-    for (int k = 0; k < 4; ++k) acc[k] = bf16x8_sumsq(a[k], acc[k]);
+    for (int k = 0; k < 8; ++k) acc[k & 3] = bf16x8_sumsq(a[k], acc[k & 3]);
   }
-  for (; i < vecs; i += width) acc[0] = bf16x8_sumsq(__ldg(q + i), acc[0]);
   if (t < head) {
     const float x = __bfloat162float(row[t]);
     acc[1] = fmaf(x, x, acc[1]);
@@ -96,6 +100,7 @@ __global__ void __launch_bounds__(kNormedThreads)
        r0 += static_cast<long long>(gridDim.x) * kPer) {
     const long long r = r0 + sub;
     const bool ok = r < a.rows;
+    const float v_old = ok && t == 0 ? e.v[r] : 0.f;  // fetched beside the row
     float s = ok ? row_sumsq(e.u + r * a.cols, a.cols, t, TPR) : 0.f;
     s = warp_sum(s);
     if constexpr (TPR > 32) {
@@ -107,7 +112,7 @@ __global__ void __launch_bounds__(kNormedThreads)
       for (int w = 0; w < TPR / 32; ++w) s += s_part[w];
     }
     if (ok && t == 0) {
-      const float v = fmaf(a.beta2, e.v[r], (1.f - a.beta2) * (s / static_cast<float>(a.cols)));
+      const float v = fmaf(a.beta2, v_old, (1.f - a.beta2) * (s / static_cast<float>(a.cols)));
       e.v[r] = v;
       const float ri = 1.f / (sqrtf(v) + a.eps);
       rinv[r] = ri;
@@ -126,15 +131,60 @@ __global__ void __launch_bounds__(kNormedThreads)
   }
 }
 
-template <typename T>
+// One block per chunk of 2048 consecutive elements, the last chunk first.
+// Row r of element i costs a division; a unit of four elements needs one where
+// cols divides by 4 (ROW4), else its elements may lie in two or more rows.
+template <typename T, bool ROW4>
 __global__ void __launch_bounds__(kNormedThreads)
     normed_apply_kernel(const __grid_constant__ NormedArgs a) {
   __shared__ float s_part[kNormedThreads / 32];
   pdl_wait();
   const NormedEntry e = a.e[blockIdx.y];
-  T* p = static_cast<T*>(e.p);
   const float* rinv = a.rinv + a.rows * blockIdx.y;
   const float* part = a.partials + static_cast<long long>(blockIdx.y) * kNormedMaxBlocks;
+  const long long n = a.rows * a.cols;
+  const long long e0 = static_cast<long long>(gridDim.x - 1 - blockIdx.x) * kNormedChunk;
+  T* p = static_cast<T*>(e.p) + e0;
+  const __nv_bfloat16* u = e.u + e0;
+  // 32-bit division where it is enough: the 64-bit one costs more than the chunk's arithmetic
+  const long long r0 = n <= 0xffffffffll
+                           ? static_cast<unsigned>(e0) / static_cast<unsigned>(a.cols)
+                           : e0 / a.cols;
+  const long long c0 = e0 - r0 * a.cols;
+  const int cnt = static_cast<int>(min(static_cast<long long>(kNormedChunk), n - e0));
+  const bool full = cnt == kNormedChunk && aligned16(p) && aligned16(u);
+  float pv[kNormedUnits][4], uv[kNormedUnits][4], rv[kNormedUnits][4];
+
+#pragma unroll
+  for (int w = 0; w < kNormedUnits; ++w) {
+    const int i = (w * kNormedThreads + threadIdx.x) * 4;
+    if (full) {
+      load4(p + i, pv[w]);
+      load4(u + i, uv[w]);
+    } else {
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        pv[w][k] = i + k < cnt ? to_f(p[i + k]) : 0.f;
+        uv[w][k] = i + k < cnt ? __bfloat162float(u[i + k]) : 0.f;
+      }
+    }
+    // row offset and column of the unit's first element; o < cols + 2048
+    const long long o = c0 + i;
+    if constexpr (ROW4) {
+      const unsigned q = o < a.cols ? 0u : static_cast<unsigned>(o) / static_cast<unsigned>(a.cols);
+      rv[w][0] = i < cnt ? rinv[r0 + q] : 0.f;
+#pragma unroll
+      for (int k = 1; k < 4; ++k) rv[w][k] = rv[w][0];
+    } else {
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const long long ok = o + k;
+        const unsigned q = ok < a.cols ? 0u : static_cast<unsigned>(ok) / static_cast<unsigned>(a.cols);
+        rv[w][k] = i + k < cnt ? rinv[r0 + q] : 0.f;
+      }
+    }
+  }
+
   float f2 = 0.f;
   for (int i = threadIdx.x; i < a.row_blocks; i += kNormedThreads) f2 += part[i];
   f2 = warp_sum(f2);
@@ -145,48 +195,18 @@ __global__ void __launch_bounds__(kNormedThreads)
   for (int w = 0; w < kNormedThreads / 32; ++w) f2 += s_part[w];
   const float eta = -a.step / (sqrtf(f2) + 1e-7f);
 
-  const long long n = a.rows * a.cols;
-  const long long chunks = (n + 7) / 8;
-  const bool vec = aligned16(p) && aligned16(e.u);
-  for (long long b = blockIdx.x; b * kNormedThreads < chunks; b += gridDim.x) {
-    const long long c = chunks - 1 - (b * kNormedThreads + threadIdx.x);
-    if (c < 0) continue;
-    const long long i0 = c * 8;
-    const int cnt = static_cast<int>(min(8ll, n - i0));
-    // 32-bit division where it is enough: the 64-bit one costs more than the chunk's arithmetic
-    long long row = n <= 0xffffffffll ? static_cast<unsigned>(i0) / static_cast<unsigned>(a.cols)
-                                      : i0 / a.cols;
-    long long left = (row + 1) * a.cols - i0;  // elements of the chunk's first row from i0 on
-    float x[8], u[8];
-    const bool full = vec && cnt == 8;
+#pragma unroll
+  for (int w = 0; w < kNormedUnits; ++w) {
+    const int i = (w * kNormedThreads + threadIdx.x) * 4;
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+      pv[w][k] = fmaf(eta * rv[w][k], uv[w][k], __fmul_rn(pv[w][k], a.decay));
     if (full) {
-      load8(p + i0, true, x);
-      load8(e.u + i0, true, u);
+      store4(p + i, pv[w]);
     } else {
 #pragma unroll
-      for (int k = 0; k < 8; ++k) {
-        x[k] = k < cnt ? to_f(p[i0 + k]) : 0.f;
-        u[k] = k < cnt ? __bfloat162float(e.u[i0 + k]) : 0.f;
-      }
-    }
-    float f = eta * rinv[row];
-#pragma unroll
-    for (int k = 0; k < 8; ++k) {
-      if (k < cnt) {
-        if (left == 0) {
-          left = a.cols;
-          f = eta * rinv[++row];
-        }
-        --left;
-        x[k] = fmaf(f, u[k], __fmul_rn(x[k], a.decay));
-      }
-    }
-    if (full) {
-      store8(p + i0, true, x);
-    } else {
-#pragma unroll
-      for (int k = 0; k < 8; ++k)
-        if (k < cnt) p[i0 + k] = from_f<T>(x[k]);
+      for (int k = 0; k < 4; ++k)
+        if (i + k < cnt) p[i + k] = from_f<T>(pv[w][k]);
     }
   }
 }

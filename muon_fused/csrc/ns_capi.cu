@@ -14,6 +14,7 @@
 #include <cstdarg>
 #include <cstdio>
 #include <cstring>
+#include <exception>
 #include <mutex>
 #include <utility>
 #include <vector>
@@ -946,6 +947,32 @@ int heads_run(const void* G, int dtype, long long batch, long long rows, long lo
 #undef FM_HEADS
 }
 
+// Whether a span that a call writes shares memory with another of its spans.
+// Spans are added as (first byte, bytes, written); `overlap` sorts them.
+struct SpanCheck {
+  struct Span {
+    uintptr_t lo, hi;
+    bool written;
+  };
+  std::vector<Span> spans;
+  void add(const void* p, long long bytes, bool written) {
+    const uintptr_t lo = reinterpret_cast<uintptr_t>(p);
+    if (bytes > 0) spans.push_back({lo, lo + uintptr_t(bytes), written});
+  }
+  bool overlap() {
+    auto less = [](const Span& a, const Span& b) { return a.lo < b.lo; };
+    if (!std::is_sorted(spans.begin(), spans.end(), less))
+      std::sort(spans.begin(), spans.end(), less);
+    uintptr_t end = 0, written_end = 0;  // furthest end so far, of all and of the written ones
+    for (const Span& s : spans) {
+      if (s.lo < written_end || (s.written && s.lo < end)) return true;
+      end = std::max(end, s.hi);
+      if (s.written) written_end = std::max(written_end, s.hi);
+    }
+    return false;
+  }
+};
+
 template <typename T, typename M, int CAP>
 int adamw_launch(const fm_adamw_tensor* ts, int64_t count, float decay, float w1, float w2,
                  float eps, cudaStream_t st) {
@@ -999,7 +1026,7 @@ int adamw_any(const fm_adamw_tensor* ts, int64_t count, float decay, float w1, f
 }
 
 template <typename T>
-int normed_launch(const DeviceState& ds, const fm_normed_matrix* mats, int64_t count,
+int normed_launch(const fm_normed_matrix* mats, int64_t count,
                   long long rows, long long cols, float decay, float step, float beta2, float eps,
                   float* ws, cudaStream_t st) {
   // Matrices per pair of launches: few enough that their updates stay in L2
@@ -1010,7 +1037,8 @@ int normed_launch(const DeviceState& ds, const fm_normed_matrix* mats, int64_t c
   // A warp per row up to 4096 columns (16 loads of 16 bytes a lane), a block per longer row.
   const bool wide = cols > 4096;
   const long long per = wide ? 1 : kNormedThreads / 32;
-  const long long chunks = (rows * cols + 7) / 8;
+  const long long chunks = (rows * cols + kNormedChunk - 1) / kNormedChunk;
+  if (chunks > 0x7fffffffll) return fail(FM_E_INVALID, "matrix %lld x %lld too large", rows, cols);
   for (int64_t i = 0; i < count; i += group) {
     const int k = int(std::min<long long>(group, count - i));
     NormedArgs a;
@@ -1029,12 +1057,13 @@ int normed_launch(const DeviceState& ds, const fm_normed_matrix* mats, int64_t c
     a.beta2 = beta2;
     a.eps = eps;
     const dim3 g1(unsigned(a.row_blocks), unsigned(k));
-    const long long want = (chunks + kNormedThreads - 1) / kNormedThreads;
-    const dim3 g2(unsigned(std::min<long long>(want, ds.sm_count * 8ll)), unsigned(k));
+    const dim3 g2{unsigned(chunks), unsigned(k), 1};
     FM_CUDA(wide ? launch_pdl(normed_rows_kernel<kNormedThreads>, g1, dim3(kNormedThreads), 0, st,
                               false, a)
                  : launch_pdl(normed_rows_kernel<32>, g1, dim3(kNormedThreads), 0, st, false, a));
-    FM_CUDA(launch_pdl(normed_apply_kernel<T>, g2, dim3(kNormedThreads), 0, st, false, a));
+    void (*apply)(NormedArgs) =
+        cols % 4 == 0 ? normed_apply_kernel<T, true> : normed_apply_kernel<T, false>;
+    FM_CUDA(launch_pdl(apply, g2, dim3(kNormedThreads), 0, st, false, a));
   }
   return FM_OK;
 }
@@ -1241,6 +1270,21 @@ int fm_adamw(const fm_adamw_tensor* tensors, int64_t count, int dtype, int momen
     if (t.n > 0 && (!t.param || !t.grad || !t.moment1 || !t.moment2))
       return fail(FM_E_INVALID, "fm_adamw: tensor %lld has a null pointer", (long long)i);
   }
+  try {  // no exception leaves a C entry
+    SpanCheck check;
+    check.spans.reserve(size_t(count) * 4);
+    const long long pe = dtype == FM_DT_F32 ? 4 : 2, me = moment_dtype == FM_DT_F32 ? 4 : 2;
+    for (int64_t i = 0; i < count; ++i) {
+      const fm_adamw_tensor& t = tensors[i];
+      check.add(t.param, t.n * pe, true);
+      check.add(t.grad, t.n * pe, false);
+      check.add(t.moment1, t.n * me, true);
+      check.add(t.moment2, t.n * me, true);
+    }
+    if (check.overlap()) return fail(FM_E_INVALID, "fm_adamw: tensors overlap in memory");
+  } catch (const std::exception& e) {
+    return fail(FM_E_INVALID, "fm_adamw: %s", e.what());
+  }
   DeviceState* ds;
   if (int rc = device_state(&ds)) return rc;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
@@ -1285,18 +1329,32 @@ int fm_muon_apply_normed(const fm_normed_matrix* mats, int64_t count, int64_t ro
   for (int64_t i = 0; i < count; ++i)
     if (!mats[i].param || !mats[i].update || !mats[i].row_moment)
       return fail(FM_E_INVALID, "fm_muon_apply_normed: matrix %lld has a null pointer", (long long)i);
+  try {
+    SpanCheck check;
+    check.spans.reserve(size_t(count) * 3 + 1);
+    const long long n = rows * cols;
+    for (int64_t i = 0; i < count; ++i) {
+      check.add(mats[i].param, n * (dtype == FM_DT_F32 ? 4 : 2), true);
+      check.add(mats[i].update, n * 2, false);
+      check.add(mats[i].row_moment, rows * 4, true);
+    }
+    check.add(workspace, (long long)need, true);
+    if (check.overlap()) return fail(FM_E_INVALID, "fm_muon_apply_normed: memory overlaps");
+  } catch (const std::exception& e) {
+    return fail(FM_E_INVALID, "fm_muon_apply_normed: %s", e.what());
+  }
   DeviceState* ds;
   if (int rc = device_state(&ds)) return rc;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   float* ws = static_cast<float*>(workspace);
   switch (dtype) {
     case FM_DT_F32:
-      return normed_launch<float>(*ds, mats, count, rows, cols, decay, step, beta2, eps, ws, st);
+      return normed_launch<float>(mats, count, rows, cols, decay, step, beta2, eps, ws, st);
     case FM_DT_BF16:
-      return normed_launch<__nv_bfloat16>(*ds, mats, count, rows, cols, decay, step, beta2, eps, ws,
+      return normed_launch<__nv_bfloat16>(mats, count, rows, cols, decay, step, beta2, eps, ws,
                                           st);
     default:
-      return normed_launch<__half>(*ds, mats, count, rows, cols, decay, step, beta2, eps, ws, st);
+      return normed_launch<__half>(mats, count, rows, cols, decay, step, beta2, eps, ws, st);
   }
 }
 

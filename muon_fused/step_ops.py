@@ -21,7 +21,7 @@ import torch
 from torch.autograd.graph import increment_version
 
 from muon_fused import _lib
-from muon_fused._fused_muon_C import _check_cuda, _stream
+from muon_fused._fused_muon_C import _check_cuda, _on_device, _stream
 
 STEP_DTYPES = {torch.float32: _lib.FM_DT_F32, torch.bfloat16: _lib.FM_DT_BF16,
                torch.float16: _lib.FM_DT_F16}
@@ -37,24 +37,16 @@ def _check_list(tensors, name: str, count: int | None = None) -> list[torch.Tens
     return tensors
 
 
-def _check_disjoint(*lists) -> None:
-    """No memory twice in one call: its elements would be updated in no order."""
-    spans = sorted((t.data_ptr(), t.data_ptr() + t.nbytes) for ts in lists for t in ts if t.numel())
-    for (_, end), (start, _) in zip(spans, spans[1:]):
-        if start < end:
-            raise RuntimeError("the tensors of one call must not overlap in memory")
-
-
 def adamw_launch(params, grads, moments1, moments2, alphas, lr: float, wd: float, betas,
                  eps: float) -> None:
-    """The unchecked call: tensors of one device, one parameter type and one
-    moment type, all contiguous; ``alphas`` holds each tensor's -lr/scale."""
-    pack = _lib.ADAMW_TENSOR.pack
-    table = b"".join([
-        pack(p.data_ptr(), g.data_ptr(), m.data_ptr(), v.data_ptr(), p.numel(), a)
-        for p, g, m, v, a in zip(params, grads, moments1, moments2, alphas)])
+    """The call after the checks: tensors of one device, one parameter type and
+    one moment type, all contiguous; ``alphas`` holds each tensor's -lr/scale."""
+    ptr = torch.Tensor.data_ptr
+    table = b"".join(map(_lib.ADAMW_TENSOR.pack, map(ptr, params), map(ptr, grads),
+                         map(ptr, moments1), map(ptr, moments2),
+                         map(torch.Tensor.numel, params), alphas))
     p0 = params[0]
-    with torch.cuda.device(p0.device):
+    with _on_device(p0):
         _lib.check(_lib.load().fm_adamw(
             table, len(params), STEP_DTYPES[p0.dtype], STEP_DTYPES[moments1[0].dtype],
             1 - lr * wd, 1 - betas[0], 1 - betas[1], eps, _stream(p0)), "fm_adamw")
@@ -91,47 +83,52 @@ def fused_adamw(
             for all.
         lr, wd, betas, eps: as in :class:`FusedMuon`.
 
-    A list may mix types and sizes; tensors of zero elements are skipped.  No
-    two tensors may share memory.
+    A list may mix types and sizes; tensors of zero elements are skipped.  What
+    a call writes must not share memory with another of its tensors.
     """
     params = _check_list(params, "params")
     n = len(params)
     grads = _check_list(grads, "grads", n)
     moments1 = _check_list(moments1, "moments1", n)
     moments2 = _check_list(moments2, "moments2", n)
-    steps = [steps] * n if isinstance(steps, int) else [int(s) for s in steps]
-    if len(steps) != n:
-        raise RuntimeError(f"steps must be an int or one per parameter, got {len(steps)} for {n}")
-    if any(s < 1 for s in steps):
-        raise RuntimeError("steps must be >= 1")
     if not all(0.0 <= b < 1.0 for b in betas):
         raise RuntimeError(f"betas must be in [0, 1), got {betas}")
+    if isinstance(steps, int):
+        if steps < 1:
+            raise RuntimeError("steps must be >= 1")
+        alphas = [adamw_alpha(lr, betas, steps)] * n
+    else:
+        steps = [int(t) for t in steps]
+        if len(steps) != n:
+            raise RuntimeError(f"steps must be an int or one per parameter, got {len(steps)} for {n}")
+        if any(t < 1 for t in steps):
+            raise RuntimeError("steps must be >= 1")
+        alphas = [adamw_alpha(lr, betas, t) for t in steps]
     if n == 0:
         return
-    device = params[0].device
-    groups: dict[tuple, list[int]] = {}
-    for i, (p, g, m, v) in enumerate(zip(params, grads, moments1, moments2)):
-        if not (p.device == g.device == m.device == v.device == device):
-            raise RuntimeError("fused_adamw needs all tensors on one device")
-        _check_cuda(p, "params")
-        if p.dtype not in STEP_DTYPES or g.dtype != p.dtype:
+    _check_cuda(params[0], "params")
+    lists = (params, grads, moments1, moments2)
+    # bulk checks: a long list of small tensors is bound by this loop, not the kernel
+    if len(set().union(*(map(torch.Tensor.get_device, ts) for ts in lists))) != 1:
+        raise RuntimeError("fused_adamw needs all tensors on one device")
+    if not all(all(map(torch.Tensor.is_contiguous, ts)) for ts in lists):
+        raise RuntimeError("fused_adamw needs contiguous tensors")
+    if not all(all(map(torch.Tensor.is_same_size, params, ts)) for ts in lists[1:]):
+        raise RuntimeError("params, grads and moments must have the same shapes")
+    types = [(p.dtype, g.dtype, m.dtype, v.dtype) for p, g, m, v in zip(*lists)]
+    for pt, gt, mt, vt in set(types):
+        if pt not in STEP_DTYPES or gt != pt:
             raise RuntimeError(f"params and grads must be fp32, bf16 or fp16 of one type, got "
-                               f"{p.dtype} and {g.dtype}")
-        if m.dtype != v.dtype or m.dtype not in (p.dtype, torch.float32):
-            raise RuntimeError(f"moments must have the parameter's type or fp32, got {m.dtype} "
-                               f"and {v.dtype}")
-        if not (p.shape == g.shape == m.shape == v.shape):
-            raise RuntimeError("params, grads and moments must have the same shapes")
-        if not (p.is_contiguous() and g.is_contiguous() and m.is_contiguous()
-                and v.is_contiguous()):
-            raise RuntimeError("fused_adamw needs contiguous tensors")
-        if p.numel():
-            groups.setdefault((p.dtype, m.dtype), []).append(i)
-    _check_disjoint(params, grads, moments1, moments2)
-    for idx in groups.values():
-        adamw_launch([params[i] for i in idx], [grads[i] for i in idx],
-                     [moments1[i] for i in idx], [moments2[i] for i in idx],
-                     [adamw_alpha(lr, betas, steps[i]) for i in idx], lr, wd, betas, eps)
+                               f"{pt} and {gt}")
+        if mt != vt or mt not in (pt, torch.float32):
+            raise RuntimeError(f"moments must have the parameter's type or fp32, got {mt} and {vt}")
+    for kind in dict.fromkeys(types):
+        if types.count(kind) == n:
+            adamw_launch(*lists, alphas, lr, wd, betas, eps)
+        else:
+            idx = [i for i in range(n) if types[i] == kind]
+            adamw_launch(*([ts[i] for i in idx] for ts in lists), [alphas[i] for i in idx], lr, wd,
+                         betas, eps)
     increment_version(params + moments1 + moments2)
 
 
@@ -191,20 +188,20 @@ def fused_normed_update(
         raise RuntimeError(f"params must be fp32, bf16 or fp16, got {p0.dtype}")
     rows = p0.size(0)
     cols = p0.numel() // rows if rows else 0
+    if len(set().union(*(map(torch.Tensor.get_device, ts)
+                         for ts in (params, updates, row_moments)))) != 1:
+        raise RuntimeError("fused_normed_update needs all tensors on one device")
     for p, u, v in zip(params, updates, row_moments):
-        if not (p.device == u.device == v.device == p0.device):
-            raise RuntimeError("fused_normed_update needs all tensors on one device")
-        if p.dtype != p0.dtype or p.shape != p0.shape:
+        if p.dtype != p0.dtype or not p.is_same_size(p0):
             raise RuntimeError("the params of one call must have one shape and type")
         if u.dtype != torch.bfloat16 or u.numel() != p.numel() or (u.dim() and u.size(0) != rows):
             raise RuntimeError("updates must be bf16 and shaped like the parameters")
-        if v.dtype != torch.float32 or v.shape != (rows,):
+        if v.dtype != torch.float32 or v.dim() != 1 or v.numel() != rows:
             raise RuntimeError("row_moments must be fp32 vectors of one element per row")
         if not (p.is_contiguous() and u.is_contiguous() and v.is_contiguous()):
             raise RuntimeError("fused_normed_update needs contiguous tensors")
     if p0.numel() == 0:
         return
-    _check_disjoint(params, updates, row_moments)
     need = normed_workspace_size(n, rows)
     if workspace is None:
         workspace = torch.empty(need, dtype=torch.uint8, device=p0.device)
@@ -214,10 +211,10 @@ def fused_normed_update(
             raise RuntimeError("workspace must be on the same device as the input")
         if workspace.nbytes < need:  # as everywhere: too small is replaced
             workspace = torch.empty(need, dtype=torch.uint8, device=p0.device)
-    pack = _lib.NORMED_MATRIX.pack
-    table = b"".join([pack(p.data_ptr(), u.data_ptr(), v.data_ptr())
-                      for p, u, v in zip(params, updates, row_moments)])
-    with torch.cuda.device(p0.device):
+    ptr = torch.Tensor.data_ptr
+    table = b"".join(map(_lib.NORMED_MATRIX.pack, map(ptr, params), map(ptr, updates),
+                         map(ptr, row_moments)))
+    with _on_device(p0):
         _lib.check(_lib.load().fm_muon_apply_normed(
             table, n, rows, cols, STEP_DTYPES[p0.dtype], 1 - lr * wd,
             lr * 0.2 * math.sqrt(rows * cols), beta2, eps, workspace.data_ptr(), workspace.nbytes,

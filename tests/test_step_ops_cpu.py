@@ -67,6 +67,28 @@ def test_c_entries_refuse_before_device_work():
                                     None) == _lib.FM_E_INVALID
 
 
+def test_c_entries_refuse_overlapping_memory():
+    lib = _lib.load()
+
+    def adam(*rows):
+        return lib.fm_adamw(b"".join(_lib.ADAMW_TENSOR.pack(*r) for r in rows), len(rows),
+                            _lib.FM_DT_F32, _lib.FM_DT_F32, 1, 0.1, 0.1, 1e-8, None)
+
+    ok = (0x1000, 0x2000, 0x3000, 0x4000, 8, -0.1)
+    for bad in [(0x1000, 0x2000, 0x3000, 0x4000, 8, -0.1),  # the same tensor twice
+                (0x5000, 0x6000, 0x401C, 0x7000, 8, -0.1),  # starts in the last element
+                (0x5000, 0x3010, 0x6000, 0x7000, 8, -0.1),  # a gradient inside a moment
+                (0x5000, 0x6000, 0x6004, 0x7000, 8, -0.1)]:
+        assert adam(ok, bad) == _lib.FM_E_INVALID and b"overlap" in lib.fm_last_error()
+    # inside a longer span that neither neighbour in the order touches
+    assert adam((0x1000, 0x9000, 0xA000, 0xB000, 1000, 0.0), (0x1100, 0x9FFC, 0xAFFC, 0xBFFC, 1, 0.0),
+                ) == _lib.FM_E_INVALID
+    m = [_lib.NORMED_MATRIX.pack(0x1000, 0x2000, 0x3000), _lib.NORMED_MATRIX.pack(0x4000, 0x2000, 0x3008)]
+    args = (4, 8, _lib.FM_DT_F32, 1, 0.1, 0.95, 1e-8, 0x100000, 1 << 20, None)
+    assert lib.fm_muon_apply_normed(b"".join(m), 2, *args) == _lib.FM_E_INVALID
+    assert b"overlap" in lib.fm_last_error()
+
+
 @pytest.mark.parametrize("count,rows", [(1, 1), (3, 4096), (70, 41)])
 def test_normed_workspace_size(count, rows):
     from muon_fused.step_ops import normed_workspace_size

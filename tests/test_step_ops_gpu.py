@@ -170,8 +170,8 @@ NORMED_SHAPES = [(1, 1), (1, 40), (40, 1), (3, 5), (64, 64), (100, 77), (33, 409
 @pytest.mark.parametrize("shape", NORMED_SHAPES)
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
 def test_normed_against_64_bits(cuda_lib, shape, dtype):
-    """v: a row's sum of c squares is added in chains of at most c/256 + 40
-    terms (8 per load of a lane, then 5 + 8 in the warp and block): that many
+    """v: a row's sum of c squares is added in chains of at most c/128 + 60 terms
+    (c/1024 past 4096 columns; a lane's chains, then 2 + 5 + 8): that many
     roundings, and 6 for the mean and the mix.  The update: v's error halves in
     the root, F's is no larger, and 12 roundings of their own; p adds 2 and its
     type's half step (fp16 subnormals: 2^-25)."""
@@ -191,7 +191,7 @@ def test_normed_against_64_bits(cuda_lib, shape, dtype):
     half = torch.finfo(dtype).eps / 2
     for i, (rp, rv, rd) in enumerate(refs):
         assert ((vs[i].double() - rv).abs() <= rv_tol * rv).all()
-        fp32 = (2 * rv_tol + 12 * U32 + (rows / 1184 + 40) * U32) * rd.abs() + 2 * U32 * p0[i].abs()
+        fp32 = (2 * rv_tol + 12 * U32 + (rows / 592 + 60) * U32) * rd.abs() + 2 * U32 * p0[i].abs()
         tol = fp32 + half * (rp.abs() + fp32) + (2.0 ** -25 if dtype == torch.float16 else 0.0)
         assert ((ps[i].double() - rp).abs() <= tol).all(), i
 
@@ -204,6 +204,44 @@ def test_normed_zero_update_only_decays(cuda_lib):
     v = [torch.zeros(32, device=DEV)]
     fused_normed_update(p, torch.zeros(1, 32, 48, dtype=torch.bfloat16, device=DEV), v, lr=LR, wd=WD)
     assert torch.equal(p[0], want) and not v[0].any()
+
+
+def test_normed_shared_update_and_refusals(cuda_lib):
+    """Two parameters may read one update; nothing written may be given twice."""
+    from muon_fused import fused_adamw, fused_normed_update
+
+    u = _rand((8, 16), 3, 0.1, torch.bfloat16)
+    a, b = _rand((8, 16), 4), _rand((8, 16), 4)
+    va, vb = torch.zeros(8, device=DEV), torch.zeros(8, device=DEV)
+    fused_normed_update([a, b], [u, u], [va, vb], lr=LR)
+    assert torch.equal(a, b) and torch.equal(va, vb)
+    bad = [([a, a], [u, u], [va, vb]), ([a, b], [u, u], [va, va]),
+           ([a], [a.view(-1)[:64].view(torch.bfloat16).view(8, 16)], [va])]
+    for args in bad:
+        with pytest.raises(RuntimeError, match="overlap"):
+            fused_normed_update(*args, lr=LR)
+    with pytest.raises(RuntimeError, match="one shape and type"):
+        fused_normed_update([a, b[:4]], [u, u], [va, vb], lr=LR)
+    with pytest.raises(RuntimeError, match="contiguous"):
+        fused_normed_update([a.T], [u.view(16, 8)], [torch.zeros(16, device=DEV)], lr=LR)
+    with pytest.raises(RuntimeError, match="bf16"):
+        fused_normed_update([a], [u.float()], [va], lr=LR)
+    with pytest.raises(RuntimeError, match="row_moments"):
+        fused_normed_update([a], [u], [va.bfloat16()], lr=LR)
+    with pytest.raises(RuntimeError, match="one device"):
+        fused_normed_update([a], [u.cpu()], [va], lr=LR)
+    z = [torch.zeros(4, device=DEV) for _ in range(4)]
+    with pytest.raises(RuntimeError, match="overlap"):
+        fused_adamw([z[0], z[0]], z[:2], z[1:3], z[2:], 1, lr=LR)
+    with pytest.raises(RuntimeError, match="shapes"):
+        fused_adamw([z[0]], [z[1].view(2, 2)], [z[2]], [z[3]], 1, lr=LR)
+    with pytest.raises(RuntimeError, match="one type"):
+        fused_adamw([z[0]], [z[1].double()], [z[2]], [z[3]], 1, lr=LR)
+    with pytest.raises(RuntimeError, match="moments"):
+        fused_adamw([z[0]], [z[1]], [z[2].half()], [z[3].half()], 1, lr=LR)
+    with pytest.raises(RuntimeError, match="contiguous"):
+        w = [torch.zeros(4, 2, device=DEV).T for _ in range(4)]
+        fused_adamw(*[[x] for x in w], 1, lr=LR)
 
 
 def test_normed_long_list_views_and_repeatability(cuda_lib):
