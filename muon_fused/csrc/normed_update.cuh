@@ -7,8 +7,12 @@
 //
 // F needs only the row sums, so two passes over u and one over p suffice:
 //   normed_rows   one row per warp (or block): Σ u², v, r and the block's share of F²
+//   normed_scale  F from the shares; r_i becomes the row's whole factor of u
 //   normed_apply  p, walking the matrix backwards so that the rows of u read
 //                 last by normed_rows are still in L2
+// normed_scale is a launch of its own (2 µs) because apply cannot afford it: with
+// every apply block adding up the shares, that chain of loads and not HBM set the
+// pace (107 against 53 µs on a bf16 4096 x 14336 matrix).
 // HBM bounds both.  All statistics are fp32; p is rounded once.  Sums run in a
 // fixed order (no atomics), so results repeat bit for bit.
 #pragma once
@@ -24,7 +28,7 @@ namespace fm {
 constexpr int kNormedThreads = 256;
 constexpr int kNormedList = 64;        // matrices per launch
 constexpr int kNormedMaxBlocks = 592;  // row blocks per matrix = F² partials per matrix
-constexpr int kNormedUnits = 2;        // apply: 4-element units per thread
+constexpr int kNormedUnits = 4;        // apply: 4-element units per thread
 constexpr int kNormedChunk = kNormedThreads * 4 * kNormedUnits;  // elements per apply block
 
 struct NormedEntry {
@@ -62,15 +66,23 @@ __device__ __forceinline__ float row_sumsq(const __nv_bfloat16* row, long long c
   const long long vecs = (cols - head) / 8;
   const uint4* q = reinterpret_cast<const uint4*>(row + head);
   float acc[4] = {0.f, 0.f, 0.f, 0.f};
-  for (long long i = t; i < vecs; i += 8ll * width) {
+  long long i = t;
+  for (; i + 7ll * width < vecs; i += 8ll * width) {
     uint4 a[8];
 #pragma unroll
-    for (int k = 0; k < 8; ++k) {
+    for (int k = 0; k < 8; ++k) a[k] = __ldg(q + i + static_cast<long long>(k) * width);
+#pragma unroll
+    for (int k = 0; k < 8; ++k) acc[k & 3] = bf16x8_sumsq(a[k], acc[k & 3]);
+  }
+  {  // up to seven more, fetched together
+    uint4 a[7];
+#pragma unroll
+    for (int k = 0; k < 7; ++k) {
       const long long j = i + static_cast<long long>(k) * width;
       a[k] = j < vecs ? __ldg(q + j) : make_uint4(0u, 0u, 0u, 0u);
     }
 #pragma unroll
-    for (int k = 0; k < 8; ++k) acc[k & 3] = bf16x8_sumsq(a[k], acc[k & 3]);
+    for (int k = 0; k < 7; ++k) acc[k & 3] = bf16x8_sumsq(a[k], acc[k & 3]);
   }
   if (t < head) {
     const float x = __bfloat162float(row[t]);
@@ -131,62 +143,20 @@ __global__ void __launch_bounds__(kNormedThreads)
   }
 }
 
-// One block per chunk of 2048 consecutive elements, the last chunk first.
-// Row r of element i costs a division; a unit of four elements needs one where
-// cols divides by 4 (ROW4), else its elements may lie in two or more rows.
-template <typename T, bool ROW4>
+// Turns r into -step/(F + 1e-7) · r, every block adding up the shares in the
+// same order.
 __global__ void __launch_bounds__(kNormedThreads)
-    normed_apply_kernel(const __grid_constant__ NormedArgs a) {
+    normed_scale_kernel(const __grid_constant__ NormedArgs a) {
   __shared__ float s_part[kNormedThreads / 32];
   pdl_wait();
-  const NormedEntry e = a.e[blockIdx.y];
-  const float* rinv = a.rinv + a.rows * blockIdx.y;
   const float* part = a.partials + static_cast<long long>(blockIdx.y) * kNormedMaxBlocks;
-  const long long n = a.rows * a.cols;
-  const long long e0 = static_cast<long long>(gridDim.x - 1 - blockIdx.x) * kNormedChunk;
-  T* p = static_cast<T*>(e.p) + e0;
-  const __nv_bfloat16* u = e.u + e0;
-  // 32-bit division where it is enough: the 64-bit one costs more than the chunk's arithmetic
-  const long long r0 = n <= 0xffffffffll
-                           ? static_cast<unsigned>(e0) / static_cast<unsigned>(a.cols)
-                           : e0 / a.cols;
-  const long long c0 = e0 - r0 * a.cols;
-  const int cnt = static_cast<int>(min(static_cast<long long>(kNormedChunk), n - e0));
-  const bool full = cnt == kNormedChunk && aligned16(p) && aligned16(u);
-  float pv[kNormedUnits][4], uv[kNormedUnits][4], rv[kNormedUnits][4];
-
-#pragma unroll
-  for (int w = 0; w < kNormedUnits; ++w) {
-    const int i = (w * kNormedThreads + threadIdx.x) * 4;
-    if (full) {
-      load4(p + i, pv[w]);
-      load4(u + i, uv[w]);
-    } else {
-#pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        pv[w][k] = i + k < cnt ? to_f(p[i + k]) : 0.f;
-        uv[w][k] = i + k < cnt ? __bfloat162float(u[i + k]) : 0.f;
-      }
-    }
-    // row offset and column of the unit's first element; o < cols + 2048
-    const long long o = c0 + i;
-    if constexpr (ROW4) {
-      const unsigned q = o < a.cols ? 0u : static_cast<unsigned>(o) / static_cast<unsigned>(a.cols);
-      rv[w][0] = i < cnt ? rinv[r0 + q] : 0.f;
-#pragma unroll
-      for (int k = 1; k < 4; ++k) rv[w][k] = rv[w][0];
-    } else {
-#pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        const long long ok = o + k;
-        const unsigned q = ok < a.cols ? 0u : static_cast<unsigned>(ok) / static_cast<unsigned>(a.cols);
-        rv[w][k] = i + k < cnt ? rinv[r0 + q] : 0.f;
-      }
-    }
-  }
-
+  float* rinv = a.rinv + a.rows * blockIdx.y;
   float f2 = 0.f;
-  for (int i = threadIdx.x; i < a.row_blocks; i += kNormedThreads) f2 += part[i];
+#pragma unroll
+  for (int k = 0; k < (kNormedMaxBlocks + kNormedThreads - 1) / kNormedThreads; ++k) {
+    const int i = k * kNormedThreads + threadIdx.x;
+    f2 += i < a.row_blocks ? part[i] : 0.f;
+  }
   f2 = warp_sum(f2);
   if ((threadIdx.x & 31) == 0) s_part[threadIdx.x >> 5] = f2;
   __syncthreads();
@@ -194,19 +164,76 @@ __global__ void __launch_bounds__(kNormedThreads)
 #pragma unroll
   for (int w = 0; w < kNormedThreads / 32; ++w) f2 += s_part[w];
   const float eta = -a.step / (sqrtf(f2) + 1e-7f);
+  for (long long r = static_cast<long long>(blockIdx.x) * kNormedThreads + threadIdx.x; r < a.rows;
+       r += static_cast<long long>(gridDim.x) * kNormedThreads)
+    rinv[r] *= eta;
+}
 
+// Four elements from offset o of the block's first row: p = p·decay + f·u, where
+// f is the factor of each element's row.  A unit of four lies in one row where
+// cols divides by 4 (ROW4); else the rows of its elements are found singly.
+template <bool ROW4>
+__device__ __forceinline__ void normed4(float (&p)[4], const float (&u)[4], const float* r,
+                                        long long o, long long cols, float decay, int cnt) {
+  float f[4];
+  if constexpr (ROW4) {
+    const unsigned q = o < cols ? 0u : static_cast<unsigned>(o) / static_cast<unsigned>(cols);
+    f[0] = r[q];
+    f[1] = f[2] = f[3] = f[0];
+  } else {
 #pragma unroll
-  for (int w = 0; w < kNormedUnits; ++w) {
-    const int i = (w * kNormedThreads + threadIdx.x) * 4;
+    for (int k = 0; k < 4; ++k) {
+      const unsigned q =
+          o + k < cols ? 0u : static_cast<unsigned>(o + k) / static_cast<unsigned>(cols);
+      f[k] = k < cnt ? r[q] : 0.f;
+    }
+  }
 #pragma unroll
-    for (int k = 0; k < 4; ++k)
-      pv[w][k] = fmaf(eta * rv[w][k], uv[w][k], __fmul_rn(pv[w][k], a.decay));
-    if (full) {
+  for (int k = 0; k < 4; ++k) p[k] = fmaf(f[k], u[k], __fmul_rn(p[k], decay));
+}
+
+// One block per chunk of 4096 consecutive elements, the last chunk first.
+template <typename T, bool ROW4>
+__global__ void __launch_bounds__(kNormedThreads)
+    normed_apply_kernel(const __grid_constant__ NormedArgs a) {
+  pdl_wait();
+  const NormedEntry e = a.e[blockIdx.y];
+  const long long n = a.rows * a.cols;
+  const long long e0 = static_cast<long long>(gridDim.x - 1 - blockIdx.x) * kNormedChunk;
+  T* p = static_cast<T*>(e.p) + e0;
+  const __nv_bfloat16* u = e.u + e0;
+  // 32-bit division where it is enough: the 64-bit one costs as much as the chunk's arithmetic
+  const long long r0 = n <= 0xffffffffll
+                           ? static_cast<unsigned>(e0) / static_cast<unsigned>(a.cols)
+                           : e0 / a.cols;
+  const long long c0 = e0 - r0 * a.cols;  // offsets from it stay below cols + 4096
+  const float* r = a.rinv + a.rows * blockIdx.y + r0;
+  if (e0 + kNormedChunk <= n && aligned16(p) && aligned16(u)) {
+    float pv[kNormedUnits][4], uv[kNormedUnits][4];
+#pragma unroll
+    for (int w = 0; w < kNormedUnits; ++w) {
+      load4(p + (w * kNormedThreads + threadIdx.x) * 4, pv[w]);
+      load4(u + (w * kNormedThreads + threadIdx.x) * 4, uv[w]);
+    }
+#pragma unroll
+    for (int w = 0; w < kNormedUnits; ++w) {
+      const int i = (w * kNormedThreads + threadIdx.x) * 4;
+      normed4<ROW4>(pv[w], uv[w], r, c0 + i, a.cols, a.decay, 4);
       store4(p + i, pv[w]);
-    } else {
+    }
+  } else {
+    const int cnt = static_cast<int>(min(static_cast<long long>(kNormedChunk), n - e0));
+    for (int i = threadIdx.x * 4; i < cnt; i += kNormedThreads * 4) {
+      float pv[4], uv[4];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        pv[k] = i + k < cnt ? to_f(p[i + k]) : 0.f;
+        uv[k] = i + k < cnt ? __bfloat162float(u[i + k]) : 0.f;
+      }
+      normed4<ROW4>(pv, uv, r, c0 + i, a.cols, a.decay, cnt - i);
 #pragma unroll
       for (int k = 0; k < 4; ++k)
-        if (i + k < cnt) p[i + k] = from_f<T>(pv[w][k]);
+        if (i + k < cnt) p[i + k] = from_f<T>(pv[k]);
     }
   }
 }

@@ -1034,8 +1034,9 @@ int normed_launch(const fm_normed_matrix* mats, int64_t count,
   constexpr long long kL2Keep = 64ll << 20;
   const long long group = std::max<long long>(
       1, std::min<long long>(kNormedList, kL2Keep / std::max<long long>(1, 2 * rows * cols)));
-  // A warp per row up to 4096 columns (16 loads of 16 bytes a lane), a block per longer row.
-  const bool wide = cols > 4096;
+  // A warp per row where the launch has rows for 16 warps an SM (or rows are
+  // short), a block per row where it has fewer and longer ones.
+  const bool wide = cols > 1024 && rows * std::min<long long>(group, count) < 148 * 16;
   const long long per = wide ? 1 : kNormedThreads / 32;
   const long long chunks = (rows * cols + kNormedChunk - 1) / kNormedChunk;
   if (chunks > 0x7fffffffll) return fail(FM_E_INVALID, "matrix %lld x %lld too large", rows, cols);
@@ -1061,6 +1062,9 @@ int normed_launch(const fm_normed_matrix* mats, int64_t count,
     FM_CUDA(wide ? launch_pdl(normed_rows_kernel<kNormedThreads>, g1, dim3(kNormedThreads), 0, st,
                               false, a)
                  : launch_pdl(normed_rows_kernel<32>, g1, dim3(kNormedThreads), 0, st, false, a));
+    const dim3 gs{unsigned(std::min<long long>(64, (rows + kNormedThreads - 1) / kNormedThreads)),
+                  unsigned(k), 1};
+    FM_CUDA(launch_pdl(normed_scale_kernel, gs, dim3(kNormedThreads), 0, st, false, a));
     void (*apply)(NormedArgs) =
         cols % 4 == 0 ? normed_apply_kernel<T, true> : normed_apply_kernel<T, false>;
     FM_CUDA(launch_pdl(apply, g2, dim3(kNormedThreads), 0, st, false, a));
