@@ -820,8 +820,7 @@ int heads_map(CUtensorMap* map, const void* base, long long inner, long long out
 
 template <int DP, bool COLS, bool HALF>
 int heads_launch(const DeviceState& ds, const HeadsPlan& P, const CUtensorMap& gram_map,
-                 const CUtensorMap& g_map, const CUtensorMap& q_map, const CUtensorMap& o_map,
-                 const HeadsArgs& a, cudaStream_t st) {
+                 const CUtensorMap& g_map, const CUtensorMap& o_map, const HeadsArgs& a, cudaStream_t st) {
   const long long tm = timer_begin(4, st);
   FM_CUDA(launch_pdl(heads_gram_kernel<DP, COLS, HALF>, dim3(unsigned(P.total * P.split)),
                      dim3(kGramThreads), GramCfg<DP>::kSmem, st, false, gram_map, a));
@@ -830,7 +829,7 @@ int heads_launch(const DeviceState& ds, const HeadsPlan& P, const CUtensorMap& g
   const long long units = P.total * a.chunks;
   FM_CUDA(launch_pdl(heads_apply_kernel<DP, COLS, HALF>,
                      dim3(unsigned(std::min<long long>(units, ds.sm_count))), dim3(kApplyThreads),
-                     ApplyCfg<DP>::kSmem, st, false, g_map, q_map, o_map, a));
+                     ApplyCfg<DP>::kSmem, st, false, g_map, o_map, a));
   timer_end(tm, st);
   return FM_OK;
 }
@@ -918,16 +917,13 @@ int heads_run(const void* G, int dtype, long long batch, long long rows, long lo
     ms = hs * heads;
   }
   const long long inner = cols_form ? P.d : P.n, outer = cols_form ? P.n : P.d;
-  CUtensorMap gram_map, g_map, q_map, o_map;
+  CUtensorMap gram_map, g_map, o_map;
   int rc;
   if ((rc = heads_map(&gram_map, src, inner, outer, heads, batch, ld, hs, ms, 64,
                       cols_form ? kHeadsK : P.dp)))
     return rc;
   if ((rc = heads_map(&g_map, src, inner, outer, heads, batch, ld, hs, ms, 64,
                       cols_form ? kApplyN : P.dp)))
-    return rc;
-  // both terms of a head as 2·DP rows
-  if ((rc = make_map(&q_map, a.q, P.total, 2 * P.dp, P.dp, P.dp, 2ll * P.dp * P.dp, 64, P.dp)))
     return rc;
   a.tma_out = (reinterpret_cast<uintptr_t>(out) & 15) == 0 && cols % 8 == 0 &&
               (!cols_form || P.d % 8 == 0);
@@ -937,7 +933,7 @@ int heads_run(const void* G, int dtype, long long batch, long long rows, long lo
   } else {
     o_map = g_map;  // unused
   }
-#define FM_HEADS(DP, C, H) heads_launch<DP, C, H>(*ds, P, gram_map, g_map, q_map, o_map, a, st)
+#define FM_HEADS(DP, C, H) heads_launch<DP, C, H>(*ds, P, gram_map, g_map, o_map, a, st)
   if (P.dp == 64) {
     if (cols_form) return half ? FM_HEADS(64, true, true) : FM_HEADS(64, true, false);
     return half ? FM_HEADS(64, false, true) : FM_HEADS(64, false, false);

@@ -73,7 +73,6 @@ constexpr int kHeadsMaxSteps = 8;
 constexpr int kHeadsK = 64;        // reduction columns per gram stage (one swizzle row)
 constexpr int kGramStages = 6;
 constexpr int kGramThreads = 192;  // producer, MMA, 4 epilogue warps
-constexpr int kIterThreads = 288;  // 8 epilogue warps, MMA
 constexpr int kApplyN = 128;       // long-side elements per apply unit
 constexpr int kApplyStages = 3;
 constexpr int kApplyThreads = 320; // 8 epilogue warps, producer, MMA
@@ -93,7 +92,7 @@ struct HeadsArgs {
   int split, kbps;   // gram: splits per head, k-blocks per split
   int steps;
   float* gram;       // total x split x DP x DP
-  void* q;           // total x 2 x DP x DP of G's type
+  void* q;           // per head two terms of G's type, in the MMAs' swizzled layout
   float* inv;        // total: 1/(‖G‖+1e-7)
   __nv_bfloat16* out;
   long long out_ld, out_head, out_mat;  // strides of out: row, head, matrix (elements)
@@ -215,54 +214,166 @@ __global__ void __launch_bounds__(kGramThreads)
 }
 
 // ---------------------------------------------------------------- iterate
+// One CTA per head.  With P = b·A + c·A² (the diagonal a·I stays in fp32):
+//
+//   A² → P      C = a·A + P·A      Q ← a·Q + P·Q      A ← a·C + P·C
+//
+// P is the MMAs' first factor in TMEM, A (then C in its place) and Q the second in
+// shared memory, all as hi and lo.  The fp32 terms a·X and b·A are where the
+// accumulators start: the epilogue that holds X writes them to TMEM before the
+// product's MMAs, which all accumulate.  The tensor pipe sets the pace: 24 MMAs a product, 4 products an iteration.  Q's product hides the
+// two epilogues between the others: its first half runs under C's, its second
+// under A's; P's epilogue alone is exposed.
+//
+// Tried: a CTA pair per head with cta_group::2 M = 128 (64 rows a CTA, two heads an
+// SM): its MMAs took as long as M = 128 on one CTA, and arrivals at the peer's
+// barrier cost more than the halved epilogue saved (330 against 326 µs on 384
+// heads of 128 x 4096).
+constexpr int kIterWarps = 16;                        // epilogue warps
+constexpr int kIterThreads = 32 * (kIterWarps + 1);   // and the MMA issuer
+
 template <int DP>
 struct IterCfg {
   static constexpr int kMat = DP * DP * 2;  // one 16-bit matrix: DP/64 k-blocks of DP rows
-  static constexpr int kPer = DP / 2;       // accumulator columns per epilogue thread
-  static constexpr int kWarps = 2 * (DP / 32);  // epilogue warps with rows to hold
-  static constexpr int kTmem = DP == 128 ? 512 : 256;
-  // A, B, Q as hi and lo; MMAs of M = 128 on DP = 64 read one matrix past the end
-  static constexpr int kSmem = 6 * kMat + (DP == 64 ? kMat : 0) + 1024 + 256;
+  static constexpr int kPer = DP / 4;       // columns per epilogue thread
+  static constexpr int kWarps = 4 * (DP / 32);  // epilogue warps with rows to hold
+  static constexpr int kTmem = DP == 128 ? 512 : 256;  // 3 accumulators, P hi and lo
+  static constexpr int kSmem = 4 * kMat + 1024 + 256;  // A and Q as hi and lo
 };
 
-// Sixteen bits hi, sixteen bits lo of 8 consecutive values into the swizzled
-// K-major operand: row r, columns 8·chunk.. of k-block kb.
-template <int DP>
+// Two floats as packed 16-bit hi (returned) and the rest as packed lo.
+template <bool HALF>
+__device__ __forceinline__ uint32_t split2(float x, float y, uint32_t& lo) {
+  if constexpr (HALF) {
+    const __half2 h = __floats2half2_rn(x, y);
+    const float2 f = __half22float2(h);
+    const __half2 l = __floats2half2_rn(x - f.x, y - f.y);
+    lo = *reinterpret_cast<const uint32_t*>(&l);
+    return *reinterpret_cast<const uint32_t*>(&h);
+  } else {
+    const __nv_bfloat162 h = __floats2bfloat162_rn(x, y);
+    const float2 f = __bfloat1622float2(h);
+    const __nv_bfloat162 l = __floats2bfloat162_rn(x - f.x, y - f.y);
+    lo = *reinterpret_cast<const uint32_t*>(&l);
+    return *reinterpret_cast<const uint32_t*>(&h);
+  }
+}
+
+// Hi and lo of 8 consecutive values into the swizzled K-major operand: row r,
+// columns 8·chunk.. of k-block kb.
+template <int DP, bool HALF = true>
 __device__ __forceinline__ void put_split8(uint8_t* hi, int r, int kb, int chunk, const float* v) {
   const int off = kb * (DP * 128) + r * 128 + ((chunk ^ (r & 7)) << 4);
   uint4 h, l;
-  __half2* hp = reinterpret_cast<__half2*>(&h);
-  __half2* lp = reinterpret_cast<__half2*>(&l);
-#pragma unroll
-  for (int k = 0; k < 4; ++k) {
-    hp[k] = __floats2half2_rn(v[2 * k], v[2 * k + 1]);
-    const float2 f = __half22float2(hp[k]);
-    lp[k] = __floats2half2_rn(v[2 * k] - f.x, v[2 * k + 1] - f.y);
-  }
+  h.x = split2<HALF>(v[0], v[1], l.x);
+  h.y = split2<HALF>(v[2], v[3], l.y);
+  h.z = split2<HALF>(v[4], v[5], l.z);
+  h.w = split2<HALF>(v[6], v[7], l.w);
   *reinterpret_cast<uint4*>(hi + off) = h;
   *reinterpret_cast<uint4*>(hi + IterCfg<DP>::kMat + off) = l;
+}
+
+// 32 lanes x N consecutive 32-bit columns, N = 32 or 16.
+template <int N>
+__device__ __forceinline__ void tmem_ld_cols(uint32_t taddr, float (&v)[N]) {
+  static_assert(N == 32 || N == 16);
+  if constexpr (N == 32) {
+    tmem_ld_32x32b_x32(taddr, v);
+  } else {
+    uint32_t r[16];
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
+        "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]),
+          "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]),
+          "=r"(r[14]), "=r"(r[15])
+        : "r"(taddr)
+        : "memory");
+    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+#pragma unroll
+    for (int i = 0; i < 16; ++i) v[i] = __uint_as_float(r[i]);
+  }
+}
+template <int N>
+__device__ __forceinline__ void tmem_st_cols(uint32_t taddr, const uint32_t (&r)[N]) {
+  static_assert(N == 32 || N == 16 || N == 8);
+  if constexpr (N == 32) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], "
+        "{%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,"
+        "%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32};" ::"r"(taddr),
+        "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]),
+        "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]),
+        "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]),
+        "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]),
+        "r"(r[29]), "r"(r[30]), "r"(r[31])
+        : "memory");
+  } else if constexpr (N == 16) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], "
+        "{%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(taddr),
+        "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]),
+        "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]),
+        "r"(r[15])
+        : "memory");
+  } else {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"r"(taddr),
+        "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
+        : "memory");
+  }
+}
+__device__ __forceinline__ void tmem_wait_st() {
+  asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+}
+
+// D[tmem] (+)= A[tmem] * B[smem]^T: lane = row of A, two 16-bit K elements a column.
+__device__ __forceinline__ void tc_mma_16_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_t bdesc,
+                                             uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d_tmem),
+      "r"(a_tmem), "l"(bdesc), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+
+// Untiled bulk copies (both addresses and the size multiples of 16 bytes).
+__device__ __forceinline__ void bulk_store(void* dst, const void* smem_src, uint32_t bytes) {
+  asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;" ::"l"(dst),
+               "r"(smem_u32(smem_src)), "r"(bytes)
+               : "memory");
+}
+__device__ __forceinline__ void bulk_load(void* smem_dst, const void* src, uint32_t bytes,
+                                          uint64_t* bar) {
+  asm volatile(
+      "cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(
+          smem_u32(smem_dst)),
+      "l"(src), "r"(bytes), "r"(smem_u32(bar))
+      : "memory");
 }
 
 template <int DP, bool HALF>
 __global__ void __launch_bounds__(kIterThreads, 1) heads_iterate_kernel(const HeadsArgs g) {
   using Cfg = IterCfg<DP>;
+  constexpr int kPer = Cfg::kPer;
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
                                              ~static_cast<uintptr_t>(1023));
-  uint8_t* sA = smem;                  // hi, lo
-  uint8_t* sB = smem + 2 * Cfg::kMat;
-  uint8_t* sQ = smem + 4 * Cfg::kMat;
-  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + Cfg::kSmem - 1024 - 256);
-  uint64_t* op_a = bars;       // operand A (or C in its place) written
-  uint64_t* op_b = bars + 1;
+  uint8_t* sA = smem;  // hi, lo
+  uint8_t* sQ = smem + 2 * Cfg::kMat;
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + 4 * Cfg::kMat);
+  uint64_t* op_a = bars;        // operand A (or C in its place) written
+  uint64_t* op_p = bars + 1;    // P (and Q) written
   uint64_t* op_c = bars + 2;
   uint64_t* acc_sq = bars + 3;  // A² ready
-  uint64_t* acc_c = bars + 4;   // B·A
-  uint64_t* acc_q = bars + 5;   // B·Q
-  uint64_t* acc_a = bars + 6;   // B·C
+  uint64_t* acc_c = bars + 4;   // P·A
+  uint64_t* acc_q = bars + 5;   // P·Q
+  uint64_t* acc_a = bars + 6;   // P·C
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 7);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
-  float* s_tr = reinterpret_cast<float*>(tmem_slot + 2);  // one per epilogue warp
+  int* s_done = reinterpret_cast<int*>(tmem_slot + 2);    // Q staged by every epilogue warp
+  float* s_tr = reinterpret_cast<float*>(tmem_slot + 4);  // trace, one part per epilogue warp
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int head = blockIdx.x;
 
@@ -270,9 +381,10 @@ __global__ void __launch_bounds__(kIterThreads, 1) heads_iterate_kernel(const He
     for (int i = 0; i < 3; ++i) mbar_init(&bars[i], Cfg::kWarps);
     for (int i = 3; i < 7; ++i) mbar_init(&bars[i], 1);
     *abort_flag = 0;
+    *s_done = 0;
     fence_barrier_init();
   }
-  if (warp == 8) {
+  if (warp == kIterWarps) {
     tmem_alloc(tmem_slot, Cfg::kTmem);
     tmem_relinquish();
   }
@@ -281,27 +393,30 @@ __global__ void __launch_bounds__(kIterThreads, 1) heads_iterate_kernel(const He
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
   const uint32_t d0 = tmem, d1 = tmem + DP, d2 = tmem + 2 * DP;
+  const uint32_t p_hi = tmem + 3 * DP, p_lo = p_hi + DP / 2;
   pdl_wait();
   pdl_trigger();
 
   // Epilogue warp: accumulator rows 32q.., columns col0 .. col0 + kPer - 1.
-  const int q = warp & 3, half = (warp >> 2) & 1;
-  const int row = q * 32 + lane, col0 = half * Cfg::kPer;
-  const bool worker = warp < 8 && q * 32 < DP;
-  constexpr float kScale = static_cast<float>(DP);  // A is held as DP·A
-  float a[Cfg::kPer];
+  const int q = warp & 3, sub = (warp >> 2) & 3;
+  const int row = q * 32 + lane, col0 = sub * kPer;
+  const bool worker = warp < kIterWarps && q * 32 < DP;
+  // A is held as A' = DP·A, so P = c/DP² · (b·DP/c · A' + A'²)
+  constexpr float kScale = static_cast<float>(DP);
+  constexpr float kP = kNsC / (kScale * kScale), kPA = kNsB * kScale / kNsC;
+  float v[kPer];  // this thread's part of the matrix at hand
   if (worker) {
     const float* src = g.gram + static_cast<long long>(head) * g.split * (DP * DP);
 #pragma unroll
-    for (int k = 0; k < Cfg::kPer; ++k) a[k] = __ldcg(src + gram_index<DP>(q, col0 + k, lane));
+    for (int k = 0; k < kPer; ++k) v[k] = __ldcg(src + gram_index<DP>(q, col0 + k, lane));
     for (int s = 1; s < g.split; ++s) {
       const float* ps = src + static_cast<long long>(s) * (DP * DP);
 #pragma unroll
-      for (int k = 0; k < Cfg::kPer; ++k) a[k] += __ldcg(ps + gram_index<DP>(q, col0 + k, lane));
+      for (int k = 0; k < kPer; ++k) v[k] += __ldcg(ps + gram_index<DP>(q, col0 + k, lane));
     }
     float tr = 0.f;
 #pragma unroll
-    for (int k = 0; k < Cfg::kPer; ++k) tr += col0 + k == row ? a[k] : 0.f;
+    for (int k = 0; k < kPer; ++k) tr += col0 + k == row ? v[k] : 0.f;
     tr = warp_sum(tr);
     if (lane == 0) s_tr[warp] = tr;
   }
@@ -310,126 +425,143 @@ __global__ void __launch_bounds__(kIterThreads, 1) heads_iterate_kernel(const He
   if (worker) {
     float tr = 0.f;
 #pragma unroll
-    for (int w = 0; w < 8; ++w) tr += (w & 3) * 32 < DP ? s_tr[w] : 0.f;
+    for (int w = 0; w < kIterWarps; ++w) tr += (w & 3) * 32 < DP ? s_tr[w] : 0.f;
     const float inv = 1.f / (sqrtf(tr) + 1e-7f);
     if (threadIdx.x == 0) g.inv[head] = inv;
-    // inv twice: inv² alone may leave fp32's range where A does not
-#pragma unroll
-    for (int k = 0; k < Cfg::kPer; ++k) a[k] = a[k] * inv * (inv * kScale);
 
-    const uint32_t lane_off = static_cast<uint32_t>(q * 32) << 16;
-    constexpr int kChunks = Cfg::kPer / 8;
+    const uint32_t mine = col0 + (static_cast<uint32_t>(q * 32) << 16);
     const int kb = col0 / 64, chunk0 = (col0 % 64) / 8;
-    auto put = [&](uint8_t* dst, const float* v) {
+    auto put = [&](uint8_t* dst) {  // v into an operand
 #pragma unroll
-      for (int c = 0; c < kChunks; ++c) put_split8<DP>(dst, row, kb, chunk0 + c, v + 8 * c);
+      for (int c = 0; c < kPer / 8; ++c) put_split8<DP>(dst, row, kb, chunk0 + c, v + 8 * c);
+    };
+    auto get = [&](uint32_t d) {  // v from an accumulator
+      tc_fence_after();
+      tmem_ld_cols<kPer>(d + mine, v);
+    };
+    auto start = [&](uint32_t d, float f) {  // f·v where an accumulator starts
+      uint32_t r[kPer];
+#pragma unroll
+      for (int k = 0; k < kPer; ++k) r[k] = __float_as_uint(f * v[k]);
+      tmem_st_cols<kPer>(d + mine, r);
     };
     auto ready = [&](uint64_t* bar) {
+      tmem_wait_st();
       tc_fence_before();
       fence_proxy_async_shared();
       __syncwarp();
       if (lane == 0) mbar_arrive(bar);
     };
-    float v[Cfg::kPer];
-    auto get = [&](uint32_t d) {
-      tc_fence_after();
+    auto add_diag = [&](float f) {
 #pragma unroll
-      for (int c = 0; c < Cfg::kPer / 32; ++c) {
-        float t[32];
-        tmem_ld_32x32b_x32(d + col0 + c * 32 + lane_off, t);
-#pragma unroll
-        for (int k = 0; k < 32; ++k) v[32 * c + k] = t[k];
-      }
+      for (int k = 0; k < kPer; ++k)
+        if (col0 + k == row) v[k] += f;
     };
     bool ok = true;
-    if (g.steps == 0) {
+    if (g.steps == 0) {  // Q = I
 #pragma unroll
-      for (int k = 0; k < Cfg::kPer; ++k) v[k] = col0 + k == row ? 1.f : 0.f;
+      for (int k = 0; k < kPer; ++k) v[k] = 0.f;
+      add_diag(1.f);
     } else {
-      put(sA, a);
+      // inv twice: inv² alone may leave fp32's range where A does not
+#pragma unroll
+      for (int k = 0; k < kPer; ++k) v[k] = v[k] * inv * (inv * kScale);
+      put(sA);
+      start(d0, kPA);
+      start(d1, kNsA);
       ready(op_a);
     }
 #pragma unroll 1
-    for (int it = 0; it < g.steps && ok; ++it) {
+    for (int it = 0; it < g.steps; ++it) {
       const bool last = it == g.steps - 1;
       const uint32_t ph = it & 1;
       if (!(ok = mbar_wait(acc_sq, ph, abort_flag, g.err, kErrWaitAccFull))) break;
       get(d0);
 #pragma unroll
-      for (int k = 0; k < Cfg::kPer; ++k) {
-        v[k] = fmaf(kNsC / (kScale * kScale), v[k], (kNsB / kScale) * a[k]);
-        if (col0 + k == row) v[k] += kNsA;
+      for (int k = 0; k < kPer; ++k) v[k] *= kP;
+      {
+        uint32_t h[kPer / 2], l[kPer / 2];
+#pragma unroll
+        for (int k = 0; k < kPer / 2; ++k) h[k] = split2<true>(v[2 * k], v[2 * k + 1], l[k]);
+        const uint32_t at = col0 / 2 + (static_cast<uint32_t>(q * 32) << 16);
+        tmem_st_cols<kPer / 2>(p_hi + at, h);
+        tmem_st_cols<kPer / 2>(p_lo + at, l);
       }
-      if (it == 0 && last) break;  // Q = B
-      put(sB, v);
-      if (it == 0) put(sQ, v);
-      ready(op_b);
+      if (it > 0) {
+        ready(op_p);
+      } else {  // Q = a·I + P
+        if (!last) ready(op_p);
+        add_diag(kNsA);
+        if (last) break;
+        put(sQ);
+        start(d2, kNsA);
+      }
       if (!last) {
         if (!(ok = mbar_wait(acc_c, ph, abort_flag, g.err, kErrWaitAccFull))) break;
         get(d1);
-        put(sA, v);
+        put(sA);
+        start(d0, kNsA);
         ready(op_c);
+        if (!(ok = mbar_wait(acc_a, ph, abort_flag, g.err, kErrWaitAccFull))) break;
+        get(d0);
+        put(sA);
+        start(d0, kPA);
+        start(d1, kNsA);
+        ready(op_a);
       }
       if (it > 0) {
         if (!(ok = mbar_wait(acc_q, ph ^ 1, abort_flag, g.err, kErrWaitAccFull))) break;
         get(d2);
-        if (last) break;  // Q is complete
-        put(sQ, v);
+        if (!last) {
+          put(sQ);
+          start(d2, kNsA);
+        }
       }
-      if (!(ok = mbar_wait(acc_a, ph, abort_flag, g.err, kErrWaitAccFull))) break;
-      get(d0);
-#pragma unroll
-      for (int k = 0; k < Cfg::kPer; ++k) a[k] = v[k];
-      put(sA, a);
-      ready(op_a);
     }
     if (ok) {
-      // Q as two terms of G's type, row-major.
-      uint16_t* dst = static_cast<uint16_t*>(g.q) +
-                      static_cast<long long>(head) * (2 * DP * DP) + row * DP + col0;
+      // Q as two terms of G's type, staged in the layout that heads_apply's MMAs
+      // read and copied out as it is.  Every product is complete.
 #pragma unroll
-      for (int c = 0; c < kChunks; ++c) {
-        uint16_t h[8], l[8];
-#pragma unroll
-        for (int k = 0; k < 8; ++k) {
-          const float x = v[8 * c + k];
-          if constexpr (HALF) {
-            const __half t = __float2half_rn(x);
-            h[k] = __half_as_ushort(t);
-            l[k] = __half_as_ushort(__float2half_rn(x - __half2float(t)));
-          } else {
-            const __nv_bfloat16 t = __float2bfloat16_rn(x);
-            h[k] = __bfloat16_as_ushort(t);
-            l[k] = __bfloat16_as_ushort(__float2bfloat16_rn(x - __bfloat162float(t)));
-          }
+      for (int c = 0; c < kPer / 8; ++c)
+        put_split8<DP, HALF>(sQ, row, kb, chunk0 + c, v + 8 * c);
+      fence_proxy_async_shared();
+      __syncwarp();
+      if (lane == 0) {
+        __threadfence_block();
+        if (atomicAdd(s_done, 1) == Cfg::kWarps - 1) {
+          __threadfence_block();
+          fence_proxy_async_shared();
+          bulk_store(static_cast<uint8_t*>(g.q) + static_cast<long long>(head) * (2 * Cfg::kMat), sQ,
+                     2 * Cfg::kMat);
+          bulk_commit();
+          bulk_wait_all();
         }
-        uint4 hv, lv;
-        uint32_t* hw = reinterpret_cast<uint32_t*>(&hv);
-        uint32_t* lw = reinterpret_cast<uint32_t*>(&lv);
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          hw[k] = h[2 * k] | (static_cast<uint32_t>(h[2 * k + 1]) << 16);
-          lw[k] = l[2 * k] | (static_cast<uint32_t>(l[2 * k + 1]) << 16);
-        }
-        reinterpret_cast<uint4*>(dst)[c] = hv;
-        reinterpret_cast<uint4*>(dst + DP * DP)[c] = lv;
       }
+      __syncwarp();
     }
     tc_fence_before();
-  } else if (warp == 8 && lane == 0) {
-    constexpr uint32_t idesc = make_idesc_16(true, 128, DP, 0, 0);
-    // D = X·Y (Y symmetric): hi·hi + hi·lo + lo·hi
-    auto product = [&](uint32_t d, const uint8_t* x, const uint8_t* y) {
-      const uint32_t xb = smem_u32(x), yb = smem_u32(y);
+  } else if (warp == kIterWarps && lane == 0) {
+    // The second factor is read MN-major, so that a product is X·Y and not X·Yᵀ:
+    // beside the untransposed a·X terms, transposed ones would turn the antisymmetric
+    // part of A's rounding error round in sign and let it grow by (2a - 1) a step.
+    constexpr uint32_t idesc = make_idesc_16(true, 128, DP, 0, 1);
+    constexpr int kSteps = DP / 16;  // K steps of a product
+    auto first = [](uint32_t base, int k) {  // rows, 16 columns from 16·k
+      return make_sdesc_sw128(base + (k / 4) * (DP * 128) + (k % 4) * 32, 16, 1024);
+    };
+    auto second = [](uint32_t base, int k) {  // 16 rows from 16·k, all columns
+      return make_sdesc_sw128(base + k * 2048, DP * 128, 1024);
+    };
+    // D += P·Y, terms hi·hi + hi·lo + lo·hi, K steps [k0, k1).
+    auto times_p = [&](uint32_t d, const uint8_t* y, int k0, int k1) {
+      const uint32_t yb = smem_u32(y);
 #pragma unroll
-      for (int t = 0; t < 3; ++t) {
-        const uint32_t xo = xb + (t == 2 ? Cfg::kMat : 0), yo = yb + (t == 1 ? Cfg::kMat : 0);
-#pragma unroll
-        for (int k = 0; k < DP / 16; ++k) {
-          const uint32_t off = (k / 4) * (DP * 128) + (k % 4) * 32;
-          tc_mma_bf16(d, make_sdesc_sw128(xo + off, 16, 1024), make_sdesc_sw128(yo + off, 16, 1024),
-                      idesc, (t | k) != 0 ? 1u : 0u);
-        }
+      for (int k = 0; k < kSteps; ++k) {
+        if (k < k0 || k >= k1) continue;
+        const uint64_t yh = second(yb, k), yl = second(yb + Cfg::kMat, k);
+        tc_mma_16_ts(d, p_hi + k * 8, yh, idesc, 1u);
+        tc_mma_16_ts(d, p_hi + k * 8, yl, idesc, 1u);
+        tc_mma_16_ts(d, p_lo + k * 8, yh, idesc, 1u);
       }
     };
     for (int it = 0; it < g.steps; ++it) {
@@ -437,29 +569,40 @@ __global__ void __launch_bounds__(kIterThreads, 1) heads_iterate_kernel(const He
       const uint32_t ph = it & 1;
       if (!mbar_wait(op_a, ph, abort_flag, g.err, kErrWaitFull)) break;
       tc_fence_after();
-      product(d0, sA, sA);
+      {
+        const uint32_t ab = smem_u32(sA);
+#pragma unroll
+        for (int k = 0; k < kSteps; ++k) {
+          const uint64_t xh = first(ab, k), yh = second(ab, k);
+          tc_mma_bf16(d0, xh, yh, idesc, 1u);
+          tc_mma_bf16(d0, xh, second(ab + Cfg::kMat, k), idesc, 1u);
+          tc_mma_bf16(d0, first(ab + Cfg::kMat, k), yh, idesc, 1u);
+        }
+      }
       tc_commit(acc_sq);
       if (it == 0 && last) break;
-      if (!mbar_wait(op_b, ph, abort_flag, g.err, kErrWaitFull)) break;
+      if (!mbar_wait(op_p, ph, abort_flag, g.err, kErrWaitFull)) break;
       tc_fence_after();
       if (!last) {
-        product(d1, sB, sA);
+        times_p(d1, sA, 0, kSteps);
         tc_commit(acc_c);
-      }
-      if (it > 0) {
-        product(d2, sB, sQ);
-        tc_commit(acc_q);
-      }
-      if (!last) {
+        if (it > 0) times_p(d2, sQ, 0, kSteps / 2);
         if (!mbar_wait(op_c, ph, abort_flag, g.err, kErrWaitFull)) break;
         tc_fence_after();
-        product(d0, sB, sA);
+        times_p(d0, sA, 0, kSteps);
         tc_commit(acc_a);
+        if (it > 0) {
+          times_p(d2, sQ, kSteps / 2, kSteps);
+          tc_commit(acc_q);
+        }
+      } else {
+        times_p(d2, sQ, 0, kSteps);
+        tc_commit(acc_q);
       }
     }
   }
   __syncthreads();
-  if (warp == 8) {
+  if (warp == kIterWarps) {
     tc_fence_after();
     tmem_dealloc(tmem, Cfg::kTmem);
   }
@@ -497,7 +640,6 @@ __device__ __forceinline__ void store_block_plain(const uint8_t* blk, __nv_bfloa
 template <int DP, bool COLS, bool HALF>
 __global__ void __launch_bounds__(kApplyThreads, 1)
     heads_apply_kernel(const __grid_constant__ CUtensorMap tmG,
-                       const __grid_constant__ CUtensorMap tmQ,
                        const __grid_constant__ CUtensorMap tmO, const HeadsArgs g) {
   using Cfg = ApplyCfg<DP>;
   extern __shared__ __align__(1024) uint8_t smem_raw[];
@@ -531,7 +673,6 @@ __global__ void __launch_bounds__(kApplyThreads, 1)
     *abort_flag = 0;
     fence_barrier_init();
     tma_prefetch_desc(&tmG);
-    tma_prefetch_desc(&tmQ);
   }
   if (warp == 9) {
     tmem_alloc(tmem_slot, 256);
@@ -558,12 +699,8 @@ __global__ void __launch_bounds__(kApplyThreads, 1)
         if (head != head_in) {
           if (!mbar_wait(q_empty, q_phase ^ 1, abort_flag, g.err, kErrWaitEmpty)) break;
           mbar_arrive_expect_tx(q_full, Cfg::kQ);
-#pragma unroll
-          for (int t = 0; t < 2; ++t)
-#pragma unroll
-            for (int kb = 0; kb < DP / 64; ++kb)
-              tma_load_3d(sQ + (t * (DP / 64) + kb) * (DP * 128), &tmQ, q_full, kb * 64, t * DP,
-                          head);
+          bulk_load(sQ, static_cast<const uint8_t*>(g.q) + static_cast<long long>(head) * Cfg::kQ,
+                    Cfg::kQ, q_full);
           q_phase ^= 1;
           head_in = head;
         }
