@@ -338,10 +338,10 @@ Workspace layout(long long batch, long long m, long long n, void* base) {
 
 // Launch with programmatic stream serialization (PDL): the kernel may begin
 // while the previous kernel on the stream drains; it waits (griddepcontrol)
-// before touching global memory.  cluster2 adds a 2-CTA cluster dimension.
+// before touching global memory.  `cluster` > 1 adds a cluster dimension.
 template <typename... KArgs, typename... Args>
-cudaError_t launch_pdl(void (*kernel)(KArgs...), dim3 grid, dim3 block, size_t smem,
-                       cudaStream_t st, bool cluster2, Args&&... args) {
+cudaError_t launch_pdl_cluster(void (*kernel)(KArgs...), dim3 grid, dim3 block, size_t smem,
+                               cudaStream_t st, int cluster, Args&&... args) {
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = grid;
   cfg.blockDim = block;
@@ -351,9 +351,9 @@ cudaError_t launch_pdl(void (*kernel)(KArgs...), dim3 grid, dim3 block, size_t s
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   int n = 1;
-  if (cluster2) {
+  if (cluster > 1) {
     attr[1].id = cudaLaunchAttributeClusterDimension;
-    attr[1].val.clusterDim.x = 2;
+    attr[1].val.clusterDim.x = unsigned(cluster);
     attr[1].val.clusterDim.y = 1;
     attr[1].val.clusterDim.z = 1;
     n = 2;
@@ -363,6 +363,13 @@ cudaError_t launch_pdl(void (*kernel)(KArgs...), dim3 grid, dim3 block, size_t s
   const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, std::forward<Args>(args)...);
   if (e == cudaSuccess) note_launch();
   return e;
+}
+
+template <typename... KArgs, typename... Args>
+cudaError_t launch_pdl(void (*kernel)(KArgs...), dim3 grid, dim3 block, size_t smem,
+                       cudaStream_t st, bool cluster2, Args&&... args) {
+  return launch_pdl_cluster(kernel, grid, block, smem, st, cluster2 ? 2 : 1,
+                            std::forward<Args>(args)...);
 }
 
 template <int MODE>
@@ -759,9 +766,11 @@ struct HeadsPlan {
   long long pack_ld;                 // row stride of the copy
 };
 
-// Splits of the long side per head in the Gram kernel: enough units for one
-// per SM of a 148-SM B200, but at least four k-blocks (256 elements) each — a
-// split costs the iterate kernel one more d x d partial to read.
+// Splits of the long side per head in the Gram kernel (the cluster size): about one
+// unit for each SM of a 148-SM B200, with at least four k-blocks (256 elements)
+// each.  Two units an SM stream no faster, and adding up more partials through the
+// cluster costs more than they save (8 splits of 32 heads of 128 x 4096: 11.6 µs,
+// 4: 9.7; 2 splits of 384 heads: 88 µs, none: 78).
 HeadsPlan plan_heads(long long batch, long long rows, long long cols, long long heads, int dim,
                      bool direct) {
   HeadsPlan P{};
@@ -771,14 +780,14 @@ HeadsPlan plan_heads(long long batch, long long rows, long long cols, long long 
   P.dp = P.d <= 64 ? 64 : 128;
   P.direct = direct;
   P.kblocks = int((P.n + kHeadsK - 1) / kHeadsK);
-  long long s = std::max<long long>(1, 148 / P.total);
+  long long s = std::max<long long>(1, std::min<long long>(kGramMaxSplit, 148 / P.total));
   s = std::min<long long>(s, std::max(1, P.kblocks / 4));
   P.kbps = int((P.kblocks + s - 1) / s);
   P.split = (P.kblocks + P.kbps - 1) / P.kbps;
   auto a256 = [](size_t b) { return (b + 255) & ~size_t(255); };
   const size_t mat = size_t(P.dp) * P.dp;
   size_t off = 0;
-  P.gram = off; off += a256(size_t(P.total) * P.split * mat * 4);
+  P.gram = off; off += a256(size_t(P.total) * mat * 4);
   P.q = off; off += a256(size_t(P.total) * 2 * mat * 2);
   P.inv = off; off += a256(size_t(P.total) * 4);
   P.pack = off;
@@ -822,8 +831,8 @@ template <int DP, bool COLS, bool HALF>
 int heads_launch(const DeviceState& ds, const HeadsPlan& P, const CUtensorMap& gram_map,
                  const CUtensorMap& g_map, const CUtensorMap& o_map, const HeadsArgs& a, cudaStream_t st) {
   const long long tm = timer_begin(4, st);
-  FM_CUDA(launch_pdl(heads_gram_kernel<DP, COLS, HALF>, dim3(unsigned(P.total * P.split)),
-                     dim3(kGramThreads), GramCfg<DP>::kSmem, st, false, gram_map, a));
+  FM_CUDA(launch_pdl_cluster(heads_gram_kernel<DP, COLS, HALF>, dim3(unsigned(P.total * P.split)),
+                             dim3(kGramThreads), GramCfg<DP>::kSmem, st, P.split, gram_map, a));
   FM_CUDA(launch_pdl(heads_iterate_kernel<DP, HALF>, dim3(unsigned(P.total)), dim3(kIterThreads),
                      IterCfg<DP>::kSmem, st, false, a));
   const long long units = P.total * a.chunks;

@@ -11,8 +11,8 @@
 // writes X in each of its 15 products and pads every d-row block to a
 // 256-row tile.  Three kernels:
 //
-//   heads_gram     partial G·Gᵀ over a range of n            (HBM bound)
-//   heads_iterate  sum of the partials, norm, all iterations  (latency bound)
+//   heads_gram     G·Gᵀ, n split over a cluster               (HBM bound)
+//   heads_iterate  norm and all iterations, a CTA per head    (latency bound)
 //   heads_apply    out = Q·G/(‖G‖+1e-7)                       (HBM bound)
 //
 // Precision.  A0 is an fp32 sum of exact products.  Products of the 16-bit
@@ -72,6 +72,7 @@ constexpr int kHeadsMaxDim = 128;
 constexpr int kHeadsMaxSteps = 8;
 constexpr int kHeadsK = 64;        // reduction columns per gram stage (one swizzle row)
 constexpr int kGramStages = 6;
+constexpr int kGramMaxSplit = 8;   // portable cluster size
 constexpr int kGramThreads = 192;  // producer, MMA, 4 epilogue warps
 constexpr int kApplyN = 128;       // long-side elements per apply unit
 constexpr int kApplyStages = 3;
@@ -84,6 +85,16 @@ __device__ __forceinline__ int gram_index(int q, int col, int lane) {
   return (q * DP + col) * 32 + lane;
 }
 
+// 16 bytes of another cluster CTA's shared memory.
+__device__ __forceinline__ float4 ld_cluster_f4(uint32_t cluster_addr) {
+  float4 v;
+  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
+               : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
+               : "r"(cluster_addr)
+               : "memory");
+  return v;
+}
+
 struct HeadsArgs {
   int d, n;          // head side, long side
   int heads;         // per matrix
@@ -91,7 +102,7 @@ struct HeadsArgs {
   int kblocks;       // ceil(n / kHeadsK)
   int split, kbps;   // gram: splits per head, k-blocks per split
   int steps;
-  float* gram;       // total x split x DP x DP
+  float* gram;       // total x DP x DP
   void* q;           // per head two terms of G's type, in the MMAs' swizzled layout
   float* inv;        // total: 1/(‖G‖+1e-7)
   __nv_bfloat16* out;
@@ -107,8 +118,13 @@ struct GramCfg {
   static constexpr int kStage = DP * kHeadsK * 2;
   // MMAs of M = 128 on DP = 64 read one stage past the last
   static constexpr int kSmem = (kGramStages + (DP == 64 ? 1 : 0)) * kStage + 1024 + 256;
+  static_assert(DP * DP * 4 <= kGramStages * kStage, "the fp32 partial reuses the stages");
 };
 
+// A cluster of g.split CTAs per head, each with a range of n; its CTAs then add
+// one share of the matrix each, in the order of the splits, from all CTAs' shared
+// memory.  (Partials through global memory cost the iterate kernel, one CTA a
+// head, 4 µs of reading at four splits.)
 // COLS: heads are column blocks (the head side is contiguous in memory), so the
 // operands are MN-major: a stage holds 64 long-side rows of DP columns.
 template <int DP, bool COLS, bool HALF>
@@ -194,13 +210,15 @@ __global__ void __launch_bounds__(kGramThreads)
     const int q = warp & 3;
     if (q * 32 < DP && mbar_wait(acc_bar, 0, abort_flag, g.err, kErrWaitAccFull)) {
       tc_fence_after();
-      float* dst = g.gram + static_cast<long long>(unit) * (DP * DP);
+      // the stages are free: every load has been consumed by a completed MMA
+      float* dst = g.split == 1 ? g.gram + static_cast<long long>(head) * (DP * DP)
+                                : reinterpret_cast<float*>(smem);
 #pragma unroll 1
       for (int c = 0; c < DP / 32; ++c) {
         float v[32];
         tmem_ld_32x32b_x32(tmem + c * 32 + (static_cast<uint32_t>(q * 32) << 16), v);
 #pragma unroll
-        for (int k = 0; k < 32; ++k) __stcg(dst + gram_index<DP>(q, c * 32 + k, lane), v[k]);
+        for (int k = 0; k < 32; ++k) dst[gram_index<DP>(q, c * 32 + k, lane)] = v[k];
       }
       tc_fence_before();
     }
@@ -210,6 +228,28 @@ __global__ void __launch_bounds__(kGramThreads)
   if (warp == 1) {
     tc_fence_after();
     tmem_dealloc(tmem, DP);
+  }
+  if (g.split > 1) {
+    cluster_sync();  // every CTA's partial is in its shared memory
+    const uint32_t base = smem_u32(smem);
+    float4* dst = reinterpret_cast<float4*>(g.gram + static_cast<long long>(head) * (DP * DP));
+    for (int i = sp * kGramThreads + threadIdx.x; i < DP * DP / 4; i += g.split * kGramThreads) {
+      float4 x[kGramMaxSplit];  // all fetched before the first is added
+#pragma unroll
+      for (int s = 0; s < kGramMaxSplit; ++s)
+        if (s < g.split) x[s] = ld_cluster_f4(mapa_shared(base + i * 16, s));
+#pragma unroll
+      for (int s = 1; s < kGramMaxSplit; ++s) {
+        if (s < g.split) {
+          x[0].x += x[s].x;
+          x[0].y += x[s].y;
+          x[0].z += x[s].z;
+          x[0].w += x[s].w;
+        }
+      }
+      __stcg(dst + i, x[0]);
+    }
+    cluster_sync();  // nobody leaves while its partial is read
   }
 }
 
@@ -221,11 +261,17 @@ __global__ void __launch_bounds__(kGramThreads)
 // P is the MMAs' first factor in TMEM, A (then C in its place) and Q the second in
 // shared memory, all as hi and lo.  The fp32 terms a·X and b·A are where the
 // accumulators start: the epilogue that holds X writes them to TMEM before the
-// product's MMAs, which all accumulate.  The tensor pipe sets the pace: 24 MMAs a product, 4 products an iteration.  Q's product hides the
-// two epilogues between the others: its first half runs under C's, its second
-// under A's; P's epilogue alone is exposed.
+// product's MMAs, which all accumulate.  The tensor pipe sets the pace (24 MMAs of
+// 64 clocks a product, 4 products an iteration); Q's product runs under C's
+// epilogue and Q's epilogue under A², P's epilogue gives its columns in two halves
+// so that C's MMAs start under the second, and A's is exposed.
 //
-// Tried: a CTA pair per head with cta_group::2 M = 128 (64 rows a CTA, two heads an
+// Measured at 128 x 128: 49-54k clocks for five iterations, 26k of them MMAs; the
+// rest are P's epilogue (1k an iteration), hand-overs between the roles (0.4k each)
+// and shared memory shared by MMAs and epilogues.
+//
+// Tried: hi alone for A² and P in the last iteration: 1 % faster, but the cut-off hi
+// doubles the error of the result (3.2e-3 against 1.66e-3).  A CTA pair per head with cta_group::2 M = 128 (64 rows a CTA, two heads an
 // SM): its MMAs took as long as M = 128 on one CTA, and arrivals at the peer's
 // barrier cost more than the halved epilogue saved (330 against 326 µs on 384
 // heads of 128 x 4096).
@@ -235,19 +281,40 @@ constexpr int kIterThreads = 32 * (kIterWarps + 1);   // and the MMA issuer
 template <int DP>
 struct IterCfg {
   static constexpr int kMat = DP * DP * 2;  // one 16-bit matrix: DP/64 k-blocks of DP rows
-  static constexpr int kPer = DP / 4;       // columns per epilogue thread
+  static constexpr int kPer = DP / 8;       // columns per epilogue thread in each half
   static constexpr int kWarps = 4 * (DP / 32);  // epilogue warps with rows to hold
   static constexpr int kTmem = DP == 128 ? 512 : 256;  // 3 accumulators, P hi and lo
   static constexpr int kSmem = 4 * kMat + 1024 + 256;  // A and Q as hi and lo
 };
 
-// Two floats as packed 16-bit hi (returned) and the rest as packed lo.
+// Packed fp32 pairs: one instruction for two lanes of an epilogue that the issue
+// rate bounds.
+__device__ __forceinline__ void mul2(float& x, float& y, float f) {
+  asm("{\n\t.reg .b64 a, b;\n\t"
+      "mov.b64 a, {%0, %1};\n\tmov.b64 b, {%2, %2};\n\t"
+      "mul.rn.f32x2 a, a, b;\n\tmov.b64 {%0, %1}, a;\n\t}"
+      : "+f"(x), "+f"(y)
+      : "f"(f));
+}
+__device__ __forceinline__ void sub2(float& x, float& y, float u, float w) {
+  asm("{\n\t.reg .b64 a, b, m;\n\t"
+      "mov.b64 a, {%0, %1};\n\tmov.b64 b, {%2, %3};\n\tmov.b64 m, {%4, %4};\n\t"
+      "fma.rn.f32x2 a, b, m, a;\n\tmov.b64 {%0, %1}, a;\n\t}"
+      : "+f"(x), "+f"(y)
+      : "f"(u), "f"(w), "f"(-1.f));
+}
+
+// Two floats as packed 16-bit hi (returned) and the rest as packed lo.  fp16's hi
+// is cut off in the float's bits (11 of them, so hi + lo has 22): converting it
+// back from fp16 to subtract took as long as the rest of an epilogue.
 template <bool HALF>
 __device__ __forceinline__ uint32_t split2(float x, float y, uint32_t& lo) {
   if constexpr (HALF) {
-    const __half2 h = __floats2half2_rn(x, y);
-    const float2 f = __half22float2(h);
-    const __half2 l = __floats2half2_rn(x - f.x, y - f.y);
+    const float hx = __uint_as_float(__float_as_uint(x) & 0xffffe000u);
+    const float hy = __uint_as_float(__float_as_uint(y) & 0xffffe000u);
+    const __half2 h = __floats2half2_rn(hx, hy);
+    sub2(x, y, hx, hy);
+    const __half2 l = __floats2half2_rn(x, y);
     lo = *reinterpret_cast<const uint32_t*>(&l);
     return *reinterpret_cast<const uint32_t*>(&h);
   } else {
@@ -273,54 +340,46 @@ __device__ __forceinline__ void put_split8(uint8_t* hi, int r, int kb, int chunk
   *reinterpret_cast<uint4*>(hi + IterCfg<DP>::kMat + off) = l;
 }
 
-// 32 lanes x N consecutive 32-bit columns, N = 32 or 16.
+// 32 lanes x N consecutive 32-bit columns.
 template <int N>
-__device__ __forceinline__ void tmem_ld_cols(uint32_t taddr, float (&v)[N]) {
-  static_assert(N == 32 || N == 16);
-  if constexpr (N == 32) {
-    tmem_ld_32x32b_x32(taddr, v);
-  } else {
-    uint32_t r[16];
+__device__ __forceinline__ void tmem_ld_cols(uint32_t taddr, float* v) {
+  static_assert(N == 16 || N == 8);
+  if constexpr (N == 16) {
     asm volatile(
         "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
         "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
-        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]),
-          "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]),
-          "=r"(r[14]), "=r"(r[15])
+        : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]), "=f"(v[4]), "=f"(v[5]), "=f"(v[6]),
+          "=f"(v[7]), "=f"(v[8]), "=f"(v[9]), "=f"(v[10]), "=f"(v[11]), "=f"(v[12]), "=f"(v[13]),
+          "=f"(v[14]), "=f"(v[15])
         : "r"(taddr)
         : "memory");
-    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
-#pragma unroll
-    for (int i = 0; i < 16; ++i) v[i] = __uint_as_float(r[i]);
+  } else {
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
+                 : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]), "=f"(v[4]), "=f"(v[5]),
+                   "=f"(v[6]), "=f"(v[7])
+                 : "r"(taddr)
+                 : "memory");
   }
 }
+// Completes this warp's loads; v's values are read after it.
 template <int N>
-__device__ __forceinline__ void tmem_st_cols(uint32_t taddr, const uint32_t (&r)[N]) {
-  static_assert(N == 32 || N == 16 || N == 8);
-  if constexpr (N == 32) {
-    asm volatile(
-        "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], "
-        "{%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,"
-        "%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32};" ::"r"(taddr),
-        "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]),
-        "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]),
-        "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]),
-        "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]),
-        "r"(r[29]), "r"(r[30]), "r"(r[31])
-        : "memory");
-  } else if constexpr (N == 16) {
-    asm volatile(
-        "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], "
-        "{%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(taddr),
-        "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]),
-        "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]),
-        "r"(r[15])
-        : "memory");
-  } else {
+__device__ __forceinline__ void tmem_wait_ld(float* v) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+#pragma unroll
+  for (int k = 0; k < N; ++k) asm volatile("" : "+f"(v[k]));
+}
+template <int N>
+__device__ __forceinline__ void tmem_st_cols(uint32_t taddr, const uint32_t* r) {
+  static_assert(N == 8 || N == 4);
+  if constexpr (N == 8) {
     asm volatile(
         "tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"r"(taddr),
         "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
         : "memory");
+  } else {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x4.b32 [%0], {%1,%2,%3,%4};" ::"r"(taddr),
+                 "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3])
+                 : "memory");
   }
 }
 __device__ __forceinline__ void tmem_wait_st() {
@@ -364,13 +423,13 @@ __global__ void __launch_bounds__(kIterThreads, 1) heads_iterate_kernel(const He
   uint8_t* sQ = smem + 2 * Cfg::kMat;
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + 4 * Cfg::kMat);
   uint64_t* op_a = bars;        // operand A (or C in its place) written
-  uint64_t* op_p = bars + 1;    // P (and Q) written
-  uint64_t* op_c = bars + 2;
-  uint64_t* acc_sq = bars + 3;  // A² ready
-  uint64_t* acc_c = bars + 4;   // P·A
-  uint64_t* acc_q = bars + 5;   // P·Q
-  uint64_t* acc_a = bars + 6;   // P·C
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 7);
+  uint64_t* op_c = bars + 1;
+  uint64_t* op_p = bars + 2;    // [2]: P's column halves (and Q before them) written
+  uint64_t* acc_sq = bars + 4;  // A² ready
+  uint64_t* acc_c = bars + 5;   // P·A
+  uint64_t* acc_q = bars + 6;   // P·Q
+  uint64_t* acc_a = bars + 7;   // P·C
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 8);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
   int* s_done = reinterpret_cast<int*>(tmem_slot + 2);    // Q staged by every epilogue warp
   float* s_tr = reinterpret_cast<float*>(tmem_slot + 4);  // trace, one part per epilogue warp
@@ -378,8 +437,8 @@ __global__ void __launch_bounds__(kIterThreads, 1) heads_iterate_kernel(const He
   const int head = blockIdx.x;
 
   if (threadIdx.x == 0) {
-    for (int i = 0; i < 3; ++i) mbar_init(&bars[i], Cfg::kWarps);
-    for (int i = 3; i < 7; ++i) mbar_init(&bars[i], 1);
+    for (int i = 0; i < 4; ++i) mbar_init(&bars[i], Cfg::kWarps);
+    for (int i = 4; i < 8; ++i) mbar_init(&bars[i], 1);
     *abort_flag = 0;
     *s_done = 0;
     fence_barrier_init();
@@ -397,26 +456,30 @@ __global__ void __launch_bounds__(kIterThreads, 1) heads_iterate_kernel(const He
   pdl_wait();
   pdl_trigger();
 
-  // Epilogue warp: accumulator rows 32q.., columns col0 .. col0 + kPer - 1.
+  // Epilogue warp: accumulator rows 32q.. and, of each half of the columns, kPer
+  // from sub·kPer.
   const int q = warp & 3, sub = (warp >> 2) & 3;
   const int row = q * 32 + lane, col0 = sub * kPer;
   const bool worker = warp < kIterWarps && q * 32 < DP;
+  const uint32_t lanes = static_cast<uint32_t>(q * 32) << 16;
   // A is held as A' = DP·A, so P = c/DP² · (b·DP/c · A' + A'²)
   constexpr float kScale = static_cast<float>(DP);
   constexpr float kP = kNsC / (kScale * kScale), kPA = kNsB * kScale / kNsC;
-  float v[kPer];  // this thread's part of the matrix at hand
+  float v[2][kPer];  // this thread's part of the matrix at hand
   if (worker) {
-    const float* src = g.gram + static_cast<long long>(head) * g.split * (DP * DP);
-#pragma unroll
-    for (int k = 0; k < kPer; ++k) v[k] = __ldcg(src + gram_index<DP>(q, col0 + k, lane));
-    for (int s = 1; s < g.split; ++s) {
-      const float* ps = src + static_cast<long long>(s) * (DP * DP);
-#pragma unroll
-      for (int k = 0; k < kPer; ++k) v[k] += __ldcg(ps + gram_index<DP>(q, col0 + k, lane));
-    }
+    const float* src = g.gram + static_cast<long long>(head) * (DP * DP);
     float tr = 0.f;
 #pragma unroll
-    for (int k = 0; k < kPer; ++k) tr += col0 + k == row ? v[k] : 0.f;
+    for (int h = 0; h < 2; ++h) {
+#pragma unroll
+      for (int k = 0; k < kPer; ++k)
+        v[h][k] = __ldcg(src + gram_index<DP>(q, h * (DP / 2) + col0 + k, lane));
+    }
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+#pragma unroll
+      for (int k = 0; k < kPer; ++k) tr += h * (DP / 2) + col0 + k == row ? v[h][k] : 0.f;
+    }
     tr = warp_sum(tr);
     if (lane == 0) s_tr[warp] = tr;
   }
@@ -429,21 +492,32 @@ __global__ void __launch_bounds__(kIterThreads, 1) heads_iterate_kernel(const He
     const float inv = 1.f / (sqrtf(tr) + 1e-7f);
     if (threadIdx.x == 0) g.inv[head] = inv;
 
-    const uint32_t mine = col0 + (static_cast<uint32_t>(q * 32) << 16);
-    const int kb = col0 / 64, chunk0 = (col0 % 64) / 8;
-    auto put = [&](uint8_t* dst) {  // v into an operand
+    auto put = [&](uint8_t* dst, int h) {  // a half of v into an operand
+      const int c = h * (DP / 2) + col0;
 #pragma unroll
-      for (int c = 0; c < kPer / 8; ++c) put_split8<DP>(dst, row, kb, chunk0 + c, v + 8 * c);
+      for (int i = 0; i < kPer / 8; ++i)
+        put_split8<DP>(dst, row, c / 64, (c % 64) / 8 + i, v[h] + 8 * i);
     };
     auto get = [&](uint32_t d) {  // v from an accumulator
       tc_fence_after();
-      tmem_ld_cols<kPer>(d + mine, v);
+      tmem_ld_cols<kPer>(d + col0 + lanes, v[0]);
+      tmem_ld_cols<kPer>(d + DP / 2 + col0 + lanes, v[1]);
+      tmem_wait_ld<kPer>(v[0]);
+      tmem_wait_ld<kPer>(v[1]);
     };
-    auto start = [&](uint32_t d, float f) {  // f·v where an accumulator starts
-      uint32_t r[kPer];
+    auto start = [&](uint32_t d, int h, float f) {  // f·v where an accumulator starts
 #pragma unroll
-      for (int k = 0; k < kPer; ++k) r[k] = __float_as_uint(f * v[k]);
-      tmem_st_cols<kPer>(d + mine, r);
+      for (int i = 0; i < kPer / 8; ++i) {
+        uint32_t r[8];
+#pragma unroll
+        for (int k = 0; k < 8; k += 2) {
+          float x = v[h][8 * i + k], y = v[h][8 * i + k + 1];
+          mul2(x, y, f);
+          r[k] = __float_as_uint(x);
+          r[k + 1] = __float_as_uint(y);
+        }
+        tmem_st_cols<8>(d + h * (DP / 2) + col0 + 8 * i + lanes, r);
+      }
     };
     auto ready = [&](uint64_t* bar) {
       tmem_wait_st();
@@ -454,21 +528,28 @@ __global__ void __launch_bounds__(kIterThreads, 1) heads_iterate_kernel(const He
     };
     auto add_diag = [&](float f) {
 #pragma unroll
-      for (int k = 0; k < kPer; ++k)
-        if (col0 + k == row) v[k] += f;
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int k = 0; k < kPer; ++k)
+          if (h * (DP / 2) + col0 + k == row) v[h][k] += f;
     };
     bool ok = true;
     if (g.steps == 0) {  // Q = I
 #pragma unroll
-      for (int k = 0; k < kPer; ++k) v[k] = 0.f;
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int k = 0; k < kPer; ++k) v[h][k] = 0.f;
       add_diag(1.f);
     } else {
-      // inv twice: inv² alone may leave fp32's range where A does not
 #pragma unroll
-      for (int k = 0; k < kPer; ++k) v[k] = v[k] * inv * (inv * kScale);
-      put(sA);
-      start(d0, kPA);
-      start(d1, kNsA);
+      for (int h = 0; h < 2; ++h) {
+        // inv twice: inv² alone may leave fp32's range where A does not
+#pragma unroll
+        for (int k = 0; k < kPer; ++k) v[h][k] = v[h][k] * inv * (inv * kScale);
+        put(sA, h);
+        start(d0, h, kPA);
+        start(d1, h, kNsA);
+      }
       ready(op_a);
     }
 #pragma unroll 1
@@ -478,43 +559,55 @@ __global__ void __launch_bounds__(kIterThreads, 1) heads_iterate_kernel(const He
       if (!(ok = mbar_wait(acc_sq, ph, abort_flag, g.err, kErrWaitAccFull))) break;
       get(d0);
 #pragma unroll
-      for (int k = 0; k < kPer; ++k) v[k] *= kP;
-      {
-        uint32_t h[kPer / 2], l[kPer / 2];
+      for (int h = 0; h < 2; ++h) {
+        uint32_t hi[kPer / 2], lo[kPer / 2];
 #pragma unroll
-        for (int k = 0; k < kPer / 2; ++k) h[k] = split2<true>(v[2 * k], v[2 * k + 1], l[k]);
-        const uint32_t at = col0 / 2 + (static_cast<uint32_t>(q * 32) << 16);
-        tmem_st_cols<kPer / 2>(p_hi + at, h);
-        tmem_st_cols<kPer / 2>(p_lo + at, l);
+        for (int k = 0; k < kPer / 2; ++k) {
+          mul2(v[h][2 * k], v[h][2 * k + 1], kP);
+          hi[k] = split2<true>(v[h][2 * k], v[h][2 * k + 1], lo[k]);
+        }
+        const uint32_t at = (h * (DP / 2) + col0) / 2 + lanes;
+        tmem_st_cols<kPer / 2>(p_hi + at, hi);
+        tmem_st_cols<kPer / 2>(p_lo + at, lo);
+        if (it > 0 || !last) ready(op_p + h);
       }
-      if (it > 0) {
-        ready(op_p);
-      } else {  // Q = a·I + P
-        if (!last) ready(op_p);
+      if (it == 0) {  // Q = a·I + P
         add_diag(kNsA);
         if (last) break;
-        put(sQ);
-        start(d2, kNsA);
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          put(sQ, h);
+          start(d2, h, kNsA);
+        }
       }
       if (!last) {
         if (!(ok = mbar_wait(acc_c, ph, abort_flag, g.err, kErrWaitAccFull))) break;
         get(d1);
-        put(sA);
-        start(d0, kNsA);
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          put(sA, h);
+          start(d0, h, kNsA);
+        }
         ready(op_c);
         if (!(ok = mbar_wait(acc_a, ph, abort_flag, g.err, kErrWaitAccFull))) break;
         get(d0);
-        put(sA);
-        start(d0, kPA);
-        start(d1, kNsA);
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          put(sA, h);
+          start(d0, h, kPA);
+          start(d1, h, kNsA);
+        }
         ready(op_a);
       }
       if (it > 0) {
         if (!(ok = mbar_wait(acc_q, ph ^ 1, abort_flag, g.err, kErrWaitAccFull))) break;
         get(d2);
         if (!last) {
-          put(sQ);
-          start(d2, kNsA);
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            put(sQ, h);
+            start(d2, h, kNsA);
+          }
         }
       }
     }
@@ -522,8 +615,12 @@ __global__ void __launch_bounds__(kIterThreads, 1) heads_iterate_kernel(const He
       // Q as two terms of G's type, staged in the layout that heads_apply's MMAs
       // read and copied out as it is.  Every product is complete.
 #pragma unroll
-      for (int c = 0; c < kPer / 8; ++c)
-        put_split8<DP, HALF>(sQ, row, kb, chunk0 + c, v + 8 * c);
+      for (int h = 0; h < 2; ++h) {
+        const int c = h * (DP / 2) + col0;
+#pragma unroll
+        for (int i = 0; i < kPer / 8; ++i)
+          put_split8<DP, HALF>(sQ, row, c / 64, (c % 64) / 8 + i, v[h] + 8 * i);
+      }
       fence_proxy_async_shared();
       __syncwarp();
       if (lane == 0) {
@@ -552,7 +649,7 @@ __global__ void __launch_bounds__(kIterThreads, 1) heads_iterate_kernel(const He
     auto second = [](uint32_t base, int k) {  // 16 rows from 16·k, all columns
       return make_sdesc_sw128(base + k * 2048, DP * 128, 1024);
     };
-    // D += P·Y, terms hi·hi + hi·lo + lo·hi, K steps [k0, k1).
+    // D += P·Y over K steps [k0, k1): terms hi·hi + hi·lo + lo·hi.
     auto times_p = [&](uint32_t d, const uint8_t* y, int k0, int k1) {
       const uint32_t yb = smem_u32(y);
 #pragma unroll
@@ -581,22 +678,26 @@ __global__ void __launch_bounds__(kIterThreads, 1) heads_iterate_kernel(const He
       }
       tc_commit(acc_sq);
       if (it == 0 && last) break;
-      if (!mbar_wait(op_p, ph, abort_flag, g.err, kErrWaitFull)) break;
+      const uint8_t* y = last ? sQ : sA;  // C, or the last step's Q
+      const uint32_t d = last ? d2 : d1;
+      if (!mbar_wait(&op_p[0], ph, abort_flag, g.err, kErrWaitFull)) break;
       tc_fence_after();
-      if (!last) {
-        times_p(d1, sA, 0, kSteps);
-        tc_commit(acc_c);
-        if (it > 0) times_p(d2, sQ, 0, kSteps / 2);
-        if (!mbar_wait(op_c, ph, abort_flag, g.err, kErrWaitFull)) break;
-        tc_fence_after();
-        times_p(d0, sA, 0, kSteps);
-        tc_commit(acc_a);
-        if (it > 0) {
-          times_p(d2, sQ, kSteps / 2, kSteps);
-          tc_commit(acc_q);
-        }
-      } else {
-        times_p(d2, sQ, 0, kSteps);
+      times_p(d, y, 0, kSteps / 2);
+      if (!mbar_wait(&op_p[1], ph, abort_flag, g.err, kErrWaitFull)) break;
+      tc_fence_after();
+      times_p(d, y, kSteps / 2, kSteps);
+      if (last) {
+        tc_commit(acc_q);
+        break;
+      }
+      tc_commit(acc_c);
+      if (it > 0) times_p(d2, sQ, 0, kSteps / 2);
+      if (!mbar_wait(op_c, ph, abort_flag, g.err, kErrWaitFull)) break;
+      tc_fence_after();
+      times_p(d0, sA, 0, kSteps);
+      tc_commit(acc_a);
+      if (it > 0) {
+        times_p(d2, sQ, kSteps / 2, kSteps);
         tc_commit(acc_q);
       }
     }
