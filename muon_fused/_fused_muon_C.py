@@ -145,8 +145,6 @@ def newton_schulz_heads(G: torch.Tensor, heads: int, steps: int = 5, dim: int = 
     elif (out.shape != G.shape or out.dtype != torch.bfloat16 or not out.is_contiguous()
           or out.device != G.device):
         raise RuntimeError("out must be a contiguous bf16 tensor shaped like G on its device")
-    elif out.untyped_storage().data_ptr() == G.untyped_storage().data_ptr():
-        raise RuntimeError("out must not share memory with G")
     if G.numel() == 0:
         return out
     ld = G.stride(-2)

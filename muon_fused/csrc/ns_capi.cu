@@ -860,6 +860,32 @@ int heads_check(long long batch, long long rows, long long cols, long long heads
   return FM_OK;
 }
 
+// Whether a span that a call writes shares memory with another of its spans.
+// Spans are added as (first byte, bytes, written); `overlap` sorts them.
+struct SpanCheck {
+  struct Span {
+    uintptr_t lo, hi;
+    bool written;
+  };
+  std::vector<Span> spans;
+  void add(const void* p, long long bytes, bool written) {
+    const uintptr_t lo = reinterpret_cast<uintptr_t>(p);
+    if (bytes > 0) spans.push_back({lo, lo + uintptr_t(bytes), written});
+  }
+  bool overlap() {
+    auto less = [](const Span& a, const Span& b) { return a.lo < b.lo; };
+    if (!std::is_sorted(spans.begin(), spans.end(), less))
+      std::sort(spans.begin(), spans.end(), less);
+    uintptr_t end = 0, written_end = 0;  // furthest end so far, of all and of the written ones
+    for (const Span& s : spans) {
+      if (s.lo < written_end || (s.written && s.lo < end)) return true;
+      end = std::max(end, s.hi);
+      if (s.written) written_end = std::max(written_end, s.hi);
+    }
+    return false;
+  }
+};
+
 int heads_run(const void* G, int dtype, long long batch, long long rows, long long cols,
               long long ldg, long long bs_g, long long heads, int dim, void* out, int steps,
               void* workspace, uint64_t workspace_bytes, cudaStream_t st) {
@@ -879,6 +905,17 @@ int heads_run(const void* G, int dtype, long long batch, long long rows, long lo
   if (workspace_bytes < P.bytes)
     return fail(FM_E_WORKSPACE, "workspace too small: need %zu bytes, got %llu", P.bytes,
                 (unsigned long long)workspace_bytes);
+  try {  // no exception leaves a C entry
+    SpanCheck check;
+    const long long elem = dtype == FM_DT_F64 ? 8 : dtype == FM_DT_F32 ? 4 : 2;
+    check.add(G, ((batch - 1) * bs_g + (rows - 1) * ldg + cols) * elem, false);
+    check.add(out, batch * rows * cols * 2, true);
+    check.add(workspace, (long long)P.bytes, true);
+    if (check.overlap())
+      return fail(FM_E_INVALID, "G, out and the workspace must not share memory");
+  } catch (const std::exception& e) {
+    return fail(FM_E_INVALID, "fm_newton_schulz_heads: %s", e.what());
+  }
   DeviceState* ds;
   if (int rc = device_state(&ds)) return rc;
   char* ws = static_cast<char*>(workspace);
@@ -951,32 +988,6 @@ int heads_run(const void* G, int dtype, long long batch, long long rows, long lo
   return half ? FM_HEADS(128, false, true) : FM_HEADS(128, false, false);
 #undef FM_HEADS
 }
-
-// Whether a span that a call writes shares memory with another of its spans.
-// Spans are added as (first byte, bytes, written); `overlap` sorts them.
-struct SpanCheck {
-  struct Span {
-    uintptr_t lo, hi;
-    bool written;
-  };
-  std::vector<Span> spans;
-  void add(const void* p, long long bytes, bool written) {
-    const uintptr_t lo = reinterpret_cast<uintptr_t>(p);
-    if (bytes > 0) spans.push_back({lo, lo + uintptr_t(bytes), written});
-  }
-  bool overlap() {
-    auto less = [](const Span& a, const Span& b) { return a.lo < b.lo; };
-    if (!std::is_sorted(spans.begin(), spans.end(), less))
-      std::sort(spans.begin(), spans.end(), less);
-    uintptr_t end = 0, written_end = 0;  // furthest end so far, of all and of the written ones
-    for (const Span& s : spans) {
-      if (s.lo < written_end || (s.written && s.lo < end)) return true;
-      end = std::max(end, s.hi);
-      if (s.written) written_end = std::max(written_end, s.hi);
-    }
-    return false;
-  }
-};
 
 template <typename T, typename M, int CAP>
 int adamw_launch(const fm_adamw_tensor* ts, int64_t count, float decay, float w1, float w2,

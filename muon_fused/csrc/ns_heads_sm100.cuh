@@ -270,11 +270,11 @@ __global__ void __launch_bounds__(kGramThreads)
 // rest are P's epilogue (1k an iteration), hand-overs between the roles (0.4k each)
 // and shared memory shared by MMAs and epilogues.
 //
-// Tried: hi alone for A² and P in the last iteration: 1 % faster, but the cut-off hi
-// doubles the error of the result (3.2e-3 against 1.66e-3).  A CTA pair per head with cta_group::2 M = 128 (64 rows a CTA, two heads an
-// SM): its MMAs took as long as M = 128 on one CTA, and arrivals at the peer's
-// barrier cost more than the halved epilogue saved (330 against 326 µs on 384
-// heads of 128 x 4096).
+// Tried: hi alone for A² and P in the last iteration: 1 % faster, but the cut-off
+// hi doubles the error of the result (3.2e-3 against 1.66e-3).  A CTA pair per head
+// with cta_group::2 M = 128 (64 rows a CTA, two heads an SM): its MMAs took as long
+// as M = 128 on one CTA, and arrivals at the peer's barrier cost more than the
+// halved epilogue saved (330 against 326 µs on 384 heads of 128 x 4096).
 constexpr int kIterWarps = 16;                        // epilogue warps
 constexpr int kIterThreads = 32 * (kIterWarps + 1);   // and the MMA issuer
 

@@ -6,9 +6,19 @@ Same constructor, defaults, state keys and group semantics as the reference
 * groups with ``use_muon=True`` run SGD-momentum (nesterov by default), the
   Newton-Schulz orthogonalisation, decoupled weight decay and the
   ``0.2·sqrt(max(A, B))`` learning-rate scale (optimizer.py:120-163);
-* every other group runs the reference's AdamW variant unchanged
+* every other group runs the reference's AdamW variant
   (optimizer.py:165-200) — including the quirk that a plain parameter list
-  has no ``use_muon`` key and therefore takes the AdamW branch.
+  has no ``use_muon`` key and therefore takes the AdamW branch.  On CUDA the
+  whole group is one launch (``fused_adamw``) with the reference's results.
+
+Beyond the reference, a Muon group may name
+
+* ``heads`` and ``heads_dim``: its matrices are attention projections whose
+  heads are blocks of rows (``heads_dim=0``) or columns (``1``); each head is
+  orthogonalised by itself (``fused_newton_schulz_heads``) and the learning-rate
+  scale takes the head's shape;
+* ``normed_beta2``: the update is normalised per output neuron by a running
+  second moment (``fused_normed_update``; state key ``row_moment``).
 
 B200-specific behaviour:
 
@@ -31,11 +41,23 @@ from torch.optim import Optimizer
 
 from muon_fused import _fused_muon_C as _C
 from muon_fused import _lib
-from muon_fused.ns_step import workspace_size
+from muon_fused.ns_step import fused_newton_schulz_heads, workspace_size, workspace_size_heads
+from muon_fused.step_ops import (STEP_DTYPES, adamw_alpha, adamw_launch, fused_normed_update,
+                                 normed_workspace_size)
 
 # Parameter / gradient dtypes the fused elementwise kernels handle.
 _EW_DTYPES = {torch.float32: _lib.FM_DT_F32, torch.bfloat16: _lib.FM_DT_BF16,
               torch.float16: _lib.FM_DT_F16}
+
+
+# Tensor types whose memory is what data_ptr() says (a DTensor's is not).
+_PLAIN = (torch.Tensor, torch.nn.Parameter)
+
+
+def _overlapping(tensors) -> bool:
+    """Whether two of the contiguous tensors share memory."""
+    spans = sorted((t.data_ptr(), t.data_ptr() + t.nbytes) for t in tensors if t.numel())
+    return any(b[0] < a[1] for a, b in zip(spans, spans[1:]))
 
 
 def _ns_batched(G: torch.Tensor, steps: int, workspace: torch.Tensor, out: torch.Tensor):
@@ -44,12 +66,21 @@ def _ns_batched(G: torch.Tensor, steps: int, workspace: torch.Tensor, out: torch
     return _C.fused_newton_schulz_batched(G, steps, workspace, out=out)
 
 
+def _ns_heads_batched(G: torch.Tensor, heads: int, dim: int, steps: int, workspace: torch.Tensor,
+                      out: torch.Tensor):
+    """Per-head Newton-Schulz used by the optimizer (substituted like ``_ns_batched``)."""
+    return fused_newton_schulz_heads(G, heads, steps, workspace, dim=dim, out=out)
+
+
 class FusedMuon(Optimizer):
     """Muon optimizer with fused Newton-Schulz orthogonalisation.
 
     Args:
         param_groups: iterable of parameters or of group dicts; groups with
-            ``"use_muon": True`` take the Muon path, all others AdamW.
+            ``"use_muon": True`` take the Muon path, all others AdamW.  A Muon
+            group may also set ``"heads"`` (with ``"heads_dim"``, 0 or 1,
+            default 0) and ``"normed_beta2"``, see above; its matrices then
+            have 2-D shapes that divide into the heads.
         lr: base learning rate (default ``1e-3``).
         wd: decoupled weight decay (default ``0.1``).
         momentum: SGD momentum of Muon groups (default ``0.95``).
@@ -71,6 +102,9 @@ class FusedMuon(Optimizer):
             parameters' ``.data`` are moved into per-bucket flat buffers for
             this, see ``sharding.ParamStore``).  Both give bit-identical
             parameters.
+        adamw_state_dtype: type of the AdamW moments: ``None`` (default) is the
+            gradient's, as the reference; ``torch.float32`` keeps them in fp32
+            beside 16-bit parameters.
     """
 
     def __init__(
@@ -87,7 +121,12 @@ class FusedMuon(Optimizer):
         bucket_bytes: int = 256 << 20,
         batch_bytes: int = 4 << 30,
         collective: str = "nccl",
+        adamw_state_dtype: torch.dtype | None = None,
     ):
+        if adamw_state_dtype not in (None, torch.float32):
+            raise ValueError(f"adamw_state_dtype must be None or torch.float32, got "
+                             f"{adamw_state_dtype}")
+        self._adamw_state_dtype = adamw_state_dtype
         defaults: dict[str, Any] = dict(
             lr=lr, wd=wd, momentum=momentum, nesterov=nesterov, ns_steps=ns_steps,
             adamw_betas=adamw_betas, adamw_eps=adamw_eps,
@@ -106,6 +145,30 @@ class FusedMuon(Optimizer):
         # id(group) -> (params, owner rank per param, momentum dtype per param)
         # of the group's last sharded step (consolidate_state_dict)
         self._owners: dict[int, tuple] = {}
+
+    def add_param_group(self, param_group) -> None:
+        """As ``Optimizer.add_param_group``, checking a Muon group's options first."""
+        if not isinstance(param_group, dict):
+            super().add_param_group(param_group)  # raises as the base class does
+            return
+        heads, dim = param_group.get("heads"), param_group.get("heads_dim", 0)
+        beta2 = param_group.get("normed_beta2")
+        if (heads is not None or beta2 is not None) and not param_group.get("use_muon", False):
+            raise ValueError("heads and normed_beta2 are options of use_muon groups")
+        if beta2 is not None and not 0.0 <= beta2 < 1.0:
+            raise ValueError(f"normed_beta2 must be in [0, 1), got {beta2}")
+        if heads is not None:
+            if int(heads) < 1 or dim not in (0, 1):
+                raise ValueError(f"heads must be >= 1 and heads_dim 0 or 1, got {heads}, {dim}")
+            params = param_group["params"]
+            param_group["params"] = params = ([params] if isinstance(params, torch.Tensor)
+                                              else list(params))
+            for p in params:
+                p = p[1] if isinstance(p, tuple) else p  # a named parameter
+                if p.ndim != 2 or p.shape[dim] % heads:
+                    raise ValueError(f"a {tuple(p.shape)} parameter does not divide into {heads} "
+                                     f"heads along dimension {dim}")
+        super().add_param_group(param_group)
 
     # ------------------------------------------------------------------ helpers
     @staticmethod
@@ -167,10 +230,18 @@ class FusedMuon(Optimizer):
             self._arena[device] = buf
         return buf
 
-    def _batch_limit(self, rows: int, cols: int) -> int:
+    @staticmethod
+    def _ns_workspace(group, batch: int, rows: int, cols: int) -> int:
+        """Workspace bytes of a group's Newton-Schulz call on ``batch`` matrices."""
+        if group.get("heads") is None:
+            return _C.workspace_size_batched(batch, rows, cols)
+        return workspace_size_heads((batch, rows, cols), group["heads"],
+                                    dim=group.get("heads_dim", 0), steps=group["ns_steps"])
+
+    def _batch_limit(self, rows: int, cols: int, group=None) -> int:
         """Matrices per batched call so inputs, outputs and workspace of one
         batch stay within ``batch_bytes``."""
-        per = _C.workspace_size_batched(1, rows, cols) + 4 * rows * cols
+        per = self._ns_workspace(group or {}, 1, rows, cols) + 4 * rows * cols
         return max(1, min(64, self._batch_bytes // per))
 
     def _orthogonalise_batch(self, params, group, out=None) -> torch.Tensor:
@@ -184,7 +255,7 @@ class FusedMuon(Optimizer):
         dev = g0.device
         n_el = B * rows * cols
         dir_bytes = (2 * n_el + 255) // 256 * 256
-        ws_bytes = _C.workspace_size_batched(B, rows, cols)
+        ws_bytes = self._ns_workspace(group, B, rows, cols)
         out_bytes = 0 if out is not None else (2 * n_el + 255) // 256 * 256
         arena = self._scratch(dev, dir_bytes + out_bytes + ws_bytes)
         dirs = arena[:2 * n_el].view(torch.bfloat16).view(B, rows, cols)
@@ -196,16 +267,77 @@ class FusedMuon(Optimizer):
             if g.ndim > 2:
                 g = g.view(g.size(0), -1)
             self._momentum_into(p, g, dirs[b], group["momentum"], group["nesterov"])
-        _ns_batched(dirs, group["ns_steps"], ws, out)
+        if group.get("heads") is None:
+            _ns_batched(dirs, group["ns_steps"], ws, out)
+        else:
+            _ns_heads_batched(dirs, group["heads"], group.get("heads_dim", 0), group["ns_steps"],
+                              ws, out)
         return out
 
+    def _apply_updates(self, group, params, updates) -> None:
+        """Apply a batch's updates (``updates[b]`` to ``params[b]``, one shape)."""
+        beta2 = group.get("normed_beta2")
+        lr, wd = group["lr"], group["wd"]
+        if beta2 is None:
+            for p, u in zip(params, updates):
+                self._apply_update(p, u, lr, wd, self._update_shape(group, p))
+            return
+        by_type: dict[torch.dtype, list] = {}
+        for p, u in zip(params, updates):
+            state = self.state[p]
+            if "row_moment" not in state:
+                state["row_moment"] = torch.zeros(p.shape[0], dtype=torch.float32, device=p.device)
+            data, v = p.data, state["row_moment"]
+            if (data.is_cuda and data.dtype in STEP_DTYPES and data.is_contiguous()
+                    and type(p) in _PLAIN):
+                rows = data.shape[0]
+                by_type.setdefault(data.dtype, []).append((data.view(rows, -1), u.view(rows, -1), v))
+            else:
+                self._normed_update_torch(data, u, v, lr, wd, beta2)
+        for items in by_type.values():
+            data, us, vs = zip(*items)
+            ws = self._normed_scratch(data[0].device, len(data), data[0].shape[0])
+            fused_normed_update(data, us, vs, lr=lr, wd=wd, beta2=beta2, workspace=ws)
+
     @staticmethod
-    def _apply_update(p: torch.Tensor, u: torch.Tensor, lr: float, wd: float) -> None:
+    def _normed_update_torch(data, u, v, lr: float, wd: float, beta2: float,
+                             eps: float = 1e-8) -> None:
+        """``fused_normed_update`` of one matrix in torch ops (CPU tensors, fp64
+        and non-contiguous parameters)."""
+        o = u.reshape(u.shape[0], -1).to(torch.promote_types(data.dtype, torch.float32))
+        v.copy_(beta2 * v + (1 - beta2) * o.square().mean(1))
+        o = o / (v.to(o.dtype).sqrt() + eps)[:, None]
+        step = lr * 0.2 * math.sqrt(o.numel()) / (o.norm() + 1e-7)
+        data.copy_(data.to(o.dtype) * (1 - lr * wd) - (step * o).view(data.shape))
+
+    def _normed_scratch(self, device: torch.device, count: int, rows: int) -> torch.Tensor:
+        """Workspace of the normalised update, apart from the batch's arena (the
+        updates that it reads live there)."""
+        need = normed_workspace_size(count, rows)
+        key = (device, "normed")
+        buf = self._workspaces.get(key)
+        if buf is None or buf.numel() < need:
+            buf = torch.empty(need, dtype=torch.uint8, device=device)
+            self._workspaces[key] = buf
+        return buf
+
+    @staticmethod
+    def _update_shape(group, p: torch.Tensor):
+        """Shape that the learning-rate scale goes by: the parameter's, or a head's."""
+        heads = group.get("heads")
+        if heads is None:
+            return p.shape
+        shape = list(p.shape)
+        shape[group.get("heads_dim", 0)] //= heads
+        return torch.Size(shape)
+
+    @staticmethod
+    def _apply_update(p: torch.Tensor, u: torch.Tensor, lr: float, wd: float, shape=None) -> None:
         """p ← p·(1 − lr·wd) − lr'·u (optimizer.py:157-163), one fused pass
         (fm_muon_apply) on CUDA, bit-identical to the two torch ops."""
         if u.shape != p.shape:
             u = u.view_as(p)
-        alpha = -FusedMuon.adjust_lr_for_muon(lr, p.shape)
+        alpha = -FusedMuon.adjust_lr_for_muon(lr, p.shape if shape is None else shape)
         dt = _EW_DTYPES.get(p.dtype)
         data = p.data
         if (data.is_cuda and dt is not None and data.is_contiguous() and u.is_contiguous()
@@ -230,12 +362,11 @@ class FusedMuon(Optimizer):
             key = (p.grad.device, p.shape[0], p.grad.numel() // p.shape[0])
             by_shape.setdefault(key, []).append(p)
         for (_, rows, cols), plist in by_shape.items():
-            lim = self._batch_limit(rows, cols)
+            lim = self._batch_limit(rows, cols, group)
             for k in range(0, len(plist), lim):
                 chunk = plist[k:k + lim]
                 out = self._orthogonalise_batch(chunk, group)
-                for b, p in enumerate(chunk):
-                    self._apply_update(p, out[b], group["lr"], group["wd"])
+                self._apply_updates(group, chunk, out.unbind(0))
 
     def _muon_group_sharded(self, group, pg, rank: int, world: int) -> None:
         from muon_fused import sharding
@@ -254,16 +385,18 @@ class FusedMuon(Optimizer):
         for p, r in zip(params, plan.owner):
             if r != rank and p in self.state:  # e.g. after loading a consolidated checkpoint
                 self.state[p].pop("momentum_buffer", None)
+                if self._collective == "param_gather":  # only the owner applies updates
+                    self.state[p].pop("row_moment", None)
 
         def compute(indices, out) -> None:
             rows, cols = out.shape[1], out.shape[2]
-            lim = self._batch_limit(rows, cols)
+            lim = self._batch_limit(rows, cols, group)
             for k in range(0, len(indices), lim):
                 self._orthogonalise_batch([params[i] for i in indices[k:k + lim]], group,
                                           out[k:k + lim])
 
         def apply(i: int, u: torch.Tensor) -> None:
-            self._apply_update(params[i], u, group["lr"], group["wd"])
+            self._apply_updates(group, [params[i]], [u])
 
         dev = params[0].device
         store = self._stores.get(key)
@@ -281,10 +414,14 @@ class FusedMuon(Optimizer):
 
     # ------------------------------------------------------------------ AdamW
     def _adamw_group(self, group) -> None:
-        """Reference AdamW branch, unchanged (optimizer.py:165-200)."""
+        """Reference AdamW branch (optimizer.py:165-200): the tensors that the
+        fused kernel takes in one launch, the others in the reference's torch
+        ops.  Both give the same values."""
         lr, wd = group["lr"], group["wd"]
         beta1, beta2 = group["adamw_betas"]
         eps: float = group["adamw_eps"]
+        fused: dict[tuple, tuple] = {}
+        alphas: dict[int, float] = {}  # -lr/scale by step
         for p in group["params"]:
             g = p.grad
             if g is None:
@@ -292,19 +429,44 @@ class FusedMuon(Optimizer):
             state = self.state[p]
             if "step" not in state:
                 state["step"] = 0
-                state["moment1"] = torch.zeros_like(g)
-                state["moment2"] = torch.zeros_like(g)
+                state["moment1"] = torch.zeros_like(g, dtype=self._adamw_state_dtype)
+                state["moment2"] = torch.zeros_like(g, dtype=self._adamw_state_dtype)
             state["step"] += 1
             step: int = state["step"]
             buf1, buf2 = state["moment1"], state["moment2"]
+            dtype = p.dtype
+            if (p.is_cuda and dtype in STEP_DTYPES and g.dtype == dtype
+                    and type(p) in _PLAIN and type(g) in _PLAIN and not g.is_sparse
+                    and buf1.dtype == buf2.dtype and buf1.dtype in (dtype, torch.float32)
+                    and p.is_contiguous() and g.is_contiguous() and buf1.is_contiguous()
+                    and buf2.is_contiguous()):
+                alpha = alphas.get(step)
+                if alpha is None:
+                    alpha = alphas[step] = adamw_alpha(lr, (beta1, beta2), step)
+                lists = fused.setdefault((p.device, dtype, buf1.dtype), ([], [], [], [], []))
+                for ts, t in zip(lists, (p, g, buf1, buf2, alpha)):
+                    ts.append(t)
+                continue
+            data = p.data
+            if buf1.dtype != g.dtype:  # fp32 moments beside 16-bit parameters
+                g = g.to(buf1.dtype)
+                data = data.to(buf1.dtype)
             buf1.lerp_(g, 1 - beta1)
             buf2.lerp_(g.square(), 1 - beta2)
             g = buf1 / (eps + buf2.sqrt())
             bias_correction1 = 1 - beta1 ** step
             bias_correction2 = 1 - beta2 ** step
             scale = bias_correction1 / bias_correction2 ** 0.5
-            p.data.mul_(1 - lr * wd)
-            p.data.add_(g, alpha=-lr / scale)
+            data.mul_(1 - lr * wd)
+            data.add_(g, alpha=-lr / scale)
+            if data.dtype != dtype:
+                p.data.copy_(data)
+        for lists in fused.values():
+            if _overlapping(lists[0]):  # tied storage: one after the other, as listed
+                for one in zip(*lists):
+                    adamw_launch(*([t] for t in one), lr, wd, (beta1, beta2), eps)
+            else:
+                adamw_launch(*lists, lr, wd, (beta1, beta2), eps)
 
     # ------------------------------------------------------------------ step
     @torch.no_grad()
@@ -340,6 +502,29 @@ class FusedMuon(Optimizer):
                     st["momentum_buffer"] = buf
                 src = dist.get_global_rank(pg, r) if pg is not None else r
                 dist.broadcast(buf, src=src, group=pg)
+                if group.get("normed_beta2") is not None:
+                    v = st.get("row_moment")
+                    if v is None:
+                        v = torch.zeros(p.shape[0], dtype=torch.float32, device=p.device)
+                        st["row_moment"] = v
+                    dist.broadcast(v, src=src, group=pg)
+
+    def load_state_dict(self, state_dict) -> None:
+        """As ``Optimizer.load_state_dict``, which casts state to the parameter's
+        type, but the fp32 statistics stay fp32: ``row_moment``, and the AdamW
+        moments where ``adamw_state_dtype`` asks for it."""
+        super().load_state_dict(state_dict)
+        keys = ["row_moment"]
+        if self._adamw_state_dtype is not None:
+            keys += ["moment1", "moment2"]
+        ids = [i for group in state_dict["param_groups"] for i in group["params"]]
+        params = [p for group in self.param_groups for p in group["params"]]
+        for i, p in zip(ids, params):
+            saved = state_dict["state"].get(i, {})
+            for key in keys:
+                if key in saved and self.state[p][key].dtype != torch.float32:
+                    self.state[p][key] = saved[key].to(device=p.device, dtype=torch.float32,
+                                                       copy=True)
 
     def step(self, closure=None):
         """One optimisation step (optimizer.py:99-202)."""

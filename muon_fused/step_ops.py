@@ -49,7 +49,7 @@ def adamw_launch(params, grads, moments1, moments2, alphas, lr: float, wd: float
     with _on_device(p0):
         _lib.check(_lib.load().fm_adamw(
             table, len(params), STEP_DTYPES[p0.dtype], STEP_DTYPES[moments1[0].dtype],
-            1 - lr * wd, 1 - betas[0], 1 - betas[1], eps, _stream(p0)), "fm_adamw")
+            float(1 - lr * wd), 1 - betas[0], 1 - betas[1], float(eps), _stream(p0)), "fm_adamw")
 
 
 def adamw_alpha(lr: float, betas, step: int) -> float:
@@ -216,7 +216,7 @@ def fused_normed_update(
                          map(ptr, row_moments)))
     with _on_device(p0):
         _lib.check(_lib.load().fm_muon_apply_normed(
-            table, n, rows, cols, STEP_DTYPES[p0.dtype], 1 - lr * wd,
-            lr * 0.2 * math.sqrt(rows * cols), beta2, eps, workspace.data_ptr(), workspace.nbytes,
+            table, n, rows, cols, STEP_DTYPES[p0.dtype], float(1 - lr * wd),
+            float(lr * 0.2 * math.sqrt(rows * cols)), float(beta2), float(eps), workspace.data_ptr(), workspace.nbytes,
             _stream(p0)), "fm_muon_apply_normed")
     increment_version(params + row_moments)

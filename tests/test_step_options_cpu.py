@@ -1,0 +1,205 @@
+"""FusedMuon's per-head and normalised Muon groups and its fp32 AdamW state, on
+the CPU: option checks, formulas, checkpoints, and the sharded step on gloo."""
+
+import copy
+import math
+import os
+import tempfile
+
+import pytest
+import torch
+import torch.distributed as dist
+import torch.multiprocessing as mp
+
+import muon_fused.optimizer as opt_mod
+from muon_fused import FusedMuon
+from tests.test_sharding import _free_port, _patch_ns
+
+A, B, C = 3.4445, -4.7750, 2.0315
+
+
+def _ns64(x, steps):
+    x = x.double()
+    x = x / (x.norm() + 1e-7)
+    for _ in range(steps):
+        a = x @ x.T
+        x = A * x + (B * a + C * a @ a) @ x
+    return x
+
+
+def heads_on_cpu(G, heads, dim, steps, workspace, out):
+    for b in range(G.shape[0]):
+        out[b].copy_(torch.cat([_ns64(h, steps) for h in G[b].chunk(heads, dim)], dim))
+
+
+def _patch():
+    _patch_ns()
+    opt_mod._ns_heads_batched = heads_on_cpu
+    opt_mod.workspace_size_heads = lambda *a, **k: 256
+
+
+SHAPES = [(32, 48), (32, 48), (64, 16), (48, 24)]
+GROUPS = [{"heads": 4, "heads_dim": 0, "normed_beta2": 0.9}, {"heads": 2, "heads_dim": 1},
+          {"normed_beta2": 0.95}]
+
+
+def _params():
+    g = torch.Generator().manual_seed(0)
+    return [[torch.nn.Parameter(torch.randn(s, generator=g) * 0.02) for s in SHAPES]
+            for _ in GROUPS]
+
+
+def _groups(params):
+    return [{"params": ps, "use_muon": True, **opts} for ps, opts in zip(params, GROUPS)]
+
+
+def _set_grads(params, step):
+    g = torch.Generator().manual_seed(100 + step)
+    for ps in params:
+        for p in ps:
+            p.grad = torch.randn(p.shape, generator=g) * 1e-3
+
+
+def _run(steps, **kw):
+    params = _params()
+    opt = FusedMuon(_groups(params), lr=0.02, **kw)
+    for s in range(steps):
+        _set_grads(params, s)
+        opt.step()
+    return params, opt
+
+
+@pytest.fixture
+def patched(monkeypatch):
+    for name in ("_ns_batched", "_ns_heads_batched", "workspace_size_heads"):
+        monkeypatch.setattr(opt_mod, name, getattr(opt_mod, name))
+    from muon_fused import _fused_muon_C as _C
+
+    monkeypatch.setattr(_C, "workspace_size_batched", _C.workspace_size_batched)
+    _patch()
+
+
+def test_options_are_checked():
+    w = torch.nn.Parameter(torch.zeros(32, 48))
+    for bad in ({"heads": 5}, {"heads": 0}, {"heads": 4, "heads_dim": 2}, {"heads": 5, "heads_dim": 1},
+                {"normed_beta2": 1.0}):
+        with pytest.raises(ValueError):
+            FusedMuon([{"params": [w], "use_muon": True, **bad}])
+    with pytest.raises(ValueError, match="use_muon"):
+        FusedMuon([{"params": [w], "heads": 4}])
+    with pytest.raises(ValueError, match="divide"):
+        FusedMuon([{"params": torch.nn.Parameter(torch.zeros(8, 4, 4)), "use_muon": True, "heads": 4}])
+    with pytest.raises(ValueError, match="adamw_state_dtype"):
+        FusedMuon([w], adamw_state_dtype=torch.bfloat16)
+    opt = FusedMuon([{"params": (p for p in [w]), "use_muon": True, "heads": 4, "heads_dim": 0}])
+    assert opt.param_groups[0]["params"] == [w]
+
+
+def test_step_follows_the_formulas(patched):
+    """Two steps of each kind of group against the update written out: momentum,
+    per-head (or whole) Newton-Schulz rounded to bf16, row normalisation, decay."""
+    params, _ = _run(2)
+    want = _params()
+    for ps, opts in zip(want, GROUPS):
+        for k, p in enumerate(ps):
+            w, buf, v = p.detach().clone(), torch.zeros_like(p), torch.zeros(p.shape[0])
+            for s in range(2):
+                _set_grads(want, s)
+                buf = 0.95 * buf + p.grad
+                d = (p.grad + 0.95 * buf).bfloat16()
+                heads, dim = opts.get("heads", 1), opts.get("heads_dim", 0)
+                if opts.get("heads"):
+                    u = torch.cat([_ns64(h, 5) for h in d.chunk(heads, dim)], dim).bfloat16()
+                else:
+                    u = torch.empty(1, *p.shape, dtype=torch.bfloat16)
+                    opt_mod._ns_batched(d[None], 5, None, u)
+                    u = u[0]
+                shape = list(p.shape)
+                shape[dim] //= heads
+                beta2 = opts.get("normed_beta2")
+                if beta2 is None:
+                    w = w * (1 - 0.02 * 0.1) - 0.02 * 0.2 * math.sqrt(max(shape)) * u.float()
+                else:
+                    o = u.float()
+                    v = beta2 * v + (1 - beta2) * o.square().mean(1)
+                    o = o / (v.sqrt() + 1e-8)[:, None]
+                    w = w * (1 - 0.02 * 0.1) - 0.02 * 0.2 * math.sqrt(o.numel()) / o.norm() * o
+            torch.testing.assert_close(params[GROUPS.index(opts)][k].detach(), w, rtol=2e-5, atol=1e-7)
+
+
+def test_state_keeps_fp32_statistics_across_a_checkpoint(patched):
+    w = torch.nn.Parameter((torch.randn(32, 48) * 0.02).bfloat16())
+    e = torch.nn.Parameter((torch.randn(7, 5) * 0.02).bfloat16())
+
+    def make():
+        return FusedMuon([{"params": [w], "use_muon": True, "normed_beta2": 0.9}, {"params": [e]}],
+                         adamw_state_dtype=torch.float32)
+
+    opt = make()
+    w.grad, e.grad = torch.randn_like(w) * 1e-3, torch.randn_like(e) * 1e-3
+    opt.step()
+    assert opt.state[w]["row_moment"].dtype == torch.float32
+    assert opt.state[e]["moment1"].dtype == opt.state[e]["moment2"].dtype == torch.float32
+    saved = copy.deepcopy(opt.state_dict())
+    new = make()
+    new.load_state_dict(saved)
+    for p, keys in ((w, ["row_moment"]), (e, ["moment1", "moment2"])):
+        for k in keys:
+            assert new.state[p][k].dtype == torch.float32
+            assert torch.equal(new.state[p][k], opt.state[p][k])
+    assert new.param_groups[0]["normed_beta2"] == 0.9
+    new.step()
+
+
+def test_adamw_fp32_state_on_cpu():
+    """16-bit parameters with fp32 moments: computed in fp32, rounded once."""
+    p = torch.nn.Parameter((torch.randn(50) * 0.02).bfloat16())
+    g = (torch.randn(50) * 1e-3).bfloat16()
+    p0 = p.detach().double()
+    opt = FusedMuon([p], lr=0.01, adamw_state_dtype=torch.float32)
+    p.grad = g
+    opt.step()
+    m, v = 0.1 * g.double(), 0.05 * g.double() ** 2
+    want = p0 * (1 - 0.01 * 0.1) - 0.01 * (0.05 ** 0.5 / 0.1) * m / (1e-8 + v.sqrt())
+    err = (p.detach().double() - want).abs()
+    assert bool((err <= want.abs() * 2.0 ** -8 + 1e-6).all())
+
+
+def _worker(rank, world, port, outdir, collective):
+    os.environ["MASTER_ADDR"] = "127.0.0.1"
+    os.environ["MASTER_PORT"] = str(port)
+    import datetime
+
+    dist.init_process_group("gloo", rank=rank, world_size=world,
+                            timeout=datetime.timedelta(seconds=60))
+    _patch()
+    try:
+        params, opt = _run(2, bucket_bytes=8192, collective=collective)
+        rows = sum("row_moment" in opt.state[p] for ps in params for p in ps)
+        opt.consolidate_state_dict()
+        torch.save({"params": [p.detach() for ps in params for p in ps], "rows": rows,
+                    "state": opt.state_dict()["state"]}, os.path.join(outdir, f"rank{rank}.pt"))
+    finally:
+        dist.destroy_process_group()
+
+
+@pytest.mark.parametrize("collective", ["nccl", "param_gather"])
+def test_sharded_options_equal_single_process(patched, collective):
+    params, opt = _run(2)
+    ref = [p.detach() for ps in params for p in ps]
+    state = opt.state_dict()["state"]
+    outdir = tempfile.mkdtemp()
+    mp.spawn(_worker, args=(2, _free_port(), outdir, collective), nprocs=2, join=True)
+    rows = 0
+    for r in range(2):
+        res = torch.load(os.path.join(outdir, f"rank{r}.pt"))
+        for a, b in zip(res["params"], ref):
+            assert torch.equal(a, b)
+        for k, v in state.items():  # consolidated: every rank has every statistic
+            assert torch.equal(res["state"][k]["momentum_buffer"], v["momentum_buffer"])
+            if "row_moment" in v:
+                assert torch.equal(res["state"][k]["row_moment"], v["row_moment"])
+        rows += res["rows"]
+    # the all-gather applies every update on every rank, the owner's apply only its own
+    normed = 2 * len(SHAPES)
+    assert rows == (2 * normed if collective == "nccl" else normed)
