@@ -27,7 +27,7 @@ namespace fm {
 
 constexpr int kNormedThreads = 256;
 constexpr int kNormedList = 64;        // matrices per launch
-constexpr int kNormedMaxBlocks = 592;  // row blocks per matrix = F² partials per matrix
+constexpr int kNormedMaxBlocks = 16384;  // row blocks per matrix = shares of F² per matrix
 constexpr int kNormedUnits = 4;        // apply: 4-element units per thread
 constexpr int kNormedChunk = kNormedThreads * 4 * kNormedUnits;  // elements per apply block
 
@@ -41,7 +41,7 @@ struct NormedArgs {
   NormedEntry e[kNormedList];
   long long rows, cols;
   float* rinv;      // rows floats per matrix
-  float* partials;  // kNormedMaxBlocks per matrix
+  float* partials;  // row_blocks per matrix
   int row_blocks;
   float decay, step, beta2, eps;  // step = lr·0.2·sqrt(rows·cols)
 };
@@ -67,22 +67,22 @@ __device__ __forceinline__ float row_sumsq(const __nv_bfloat16* row, long long c
   const uint4* q = reinterpret_cast<const uint4*>(row + head);
   float acc[4] = {0.f, 0.f, 0.f, 0.f};
   long long i = t;
-  for (; i + 7ll * width < vecs; i += 8ll * width) {
-    uint4 a[8];
+  for (; i + 3ll * width < vecs; i += 4ll * width) {
+    uint4 a[4];
 #pragma unroll
-    for (int k = 0; k < 8; ++k) a[k] = __ldg(q + i + static_cast<long long>(k) * width);
+    for (int k = 0; k < 4; ++k) a[k] = __ldg(q + i + static_cast<long long>(k) * width);
 #pragma unroll
-    for (int k = 0; k < 8; ++k) acc[k & 3] = bf16x8_sumsq(a[k], acc[k & 3]);
+    for (int k = 0; k < 4; ++k) acc[k] = bf16x8_sumsq(a[k], acc[k]);
   }
-  {  // up to seven more, fetched together
-    uint4 a[7];
+  {  // up to three more, fetched together
+    uint4 a[3];
 #pragma unroll
-    for (int k = 0; k < 7; ++k) {
+    for (int k = 0; k < 3; ++k) {
       const long long j = i + static_cast<long long>(k) * width;
       a[k] = j < vecs ? __ldg(q + j) : make_uint4(0u, 0u, 0u, 0u);
     }
 #pragma unroll
-    for (int k = 0; k < 7; ++k) acc[k & 3] = bf16x8_sumsq(a[k], acc[k & 3]);
+    for (int k = 0; k < 3; ++k) acc[k] = bf16x8_sumsq(a[k], acc[k]);
   }
   if (t < head) {
     const float x = __bfloat162float(row[t]);
@@ -96,51 +96,60 @@ __device__ __forceinline__ float row_sumsq(const __nv_bfloat16* row, long long c
   return (acc[0] + acc[1]) + (acc[2] + acc[3]);
 }
 
+// v, r and the share of F² of one row whose Σ u² is s (one thread).
+__device__ __forceinline__ float normed_row(const NormedArgs& a, float* v, float* rinv, float v_old,
+                                            float s) {
+  const float x = fmaf(a.beta2, v_old, (1.f - a.beta2) * (s / static_cast<float>(a.cols)));
+  *v = x;
+  const float ri = 1.f / (sqrtf(x) + a.eps);
+  *rinv = ri;
+  return s * ri * ri;
+}
+
 // TPR threads per row: a warp where a row is short, the block where it is long.
 template <int TPR>
-__global__ void __launch_bounds__(kNormedThreads)
+__global__ void __launch_bounds__(kNormedThreads, 6)
     normed_rows_kernel(const __grid_constant__ NormedArgs a) {
+  constexpr int kWarps = kNormedThreads / 32;
   constexpr int kPer = kNormedThreads / TPR;  // rows per block and round
-  __shared__ float s_part[kNormedThreads / 32];
+  __shared__ float s_part[kWarps];
   pdl_wait();
   const NormedEntry e = a.e[blockIdx.y];
   float* rinv = a.rinv + a.rows * blockIdx.y;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int sub = threadIdx.x / TPR, t = threadIdx.x % TPR;
-  float f2 = 0.f;  // this thread's rows' share of F² (thread t == 0 of each row)
+  float f2 = 0.f;  // the share of F² of the rows that this thread finished
   for (long long r0 = static_cast<long long>(blockIdx.x) * kPer; r0 < a.rows;
        r0 += static_cast<long long>(gridDim.x) * kPer) {
     const long long r = r0 + sub;
     const bool ok = r < a.rows;
     const float v_old = ok && t == 0 ? e.v[r] : 0.f;  // fetched beside the row
-    float s = ok ? row_sumsq(e.u + r * a.cols, a.cols, t, TPR) : 0.f;
-    s = warp_sum(s);
+    float s = warp_sum(ok ? row_sumsq(e.u + r * a.cols, a.cols, t, TPR) : 0.f);
     if constexpr (TPR > 32) {
-      __syncthreads();
       if (lane == 0) s_part[warp] = s;
       __syncthreads();
-      s = 0.f;
+      if (threadIdx.x == 0) {
+        s = 0.f;
 #pragma unroll
-      for (int w = 0; w < TPR / 32; ++w) s += s_part[w];
-    }
-    if (ok && t == 0) {
-      const float v = fmaf(a.beta2, v_old, (1.f - a.beta2) * (s / static_cast<float>(a.cols)));
-      e.v[r] = v;
-      const float ri = 1.f / (sqrtf(v) + a.eps);
-      rinv[r] = ri;
-      f2 = fmaf(s * ri, ri, f2);
+        for (int w = 0; w < kWarps; ++w) s += s_part[w];
+        f2 += normed_row(a, e.v + r, rinv + r, v_old, s);
+      }
+      if (r0 + static_cast<long long>(gridDim.x) * kPer < a.rows) __syncthreads();
+    } else if (ok && lane == 0) {
+      f2 += normed_row(a, e.v + r, rinv + r, v_old, s);
     }
   }
-  f2 = warp_sum(f2);
-  __syncthreads();
-  if (lane == 0) s_part[warp] = f2;
-  __syncthreads();
-  if (threadIdx.x == 0) {
-    float x = 0.f;
+  if constexpr (TPR == 32) {
+    if (lane == 0) s_part[warp] = f2;
+    __syncthreads();
+    if (threadIdx.x == 0) {
+      f2 = 0.f;
 #pragma unroll
-    for (int w = 0; w < kNormedThreads / 32; ++w) x += s_part[w];
-    a.partials[static_cast<long long>(blockIdx.y) * kNormedMaxBlocks + blockIdx.x] = x;
+      for (int w = 0; w < kWarps; ++w) f2 += s_part[w];
+    }
   }
+  if (threadIdx.x == 0)
+    a.partials[static_cast<long long>(blockIdx.y) * a.row_blocks + blockIdx.x] = f2;
 }
 
 // Turns r into -step/(F + 1e-7) · r, every block adding up the shares in the
@@ -149,13 +158,18 @@ __global__ void __launch_bounds__(kNormedThreads)
     normed_scale_kernel(const __grid_constant__ NormedArgs a) {
   __shared__ float s_part[kNormedThreads / 32];
   pdl_wait();
-  const float* part = a.partials + static_cast<long long>(blockIdx.y) * kNormedMaxBlocks;
+  const float* part = a.partials + static_cast<long long>(blockIdx.y) * a.row_blocks;
   float* rinv = a.rinv + a.rows * blockIdx.y;
   float f2 = 0.f;
+  for (int i0 = 0; i0 < a.row_blocks; i0 += 8 * kNormedThreads) {
+    float x[8];
 #pragma unroll
-  for (int k = 0; k < (kNormedMaxBlocks + kNormedThreads - 1) / kNormedThreads; ++k) {
-    const int i = k * kNormedThreads + threadIdx.x;
-    f2 += i < a.row_blocks ? part[i] : 0.f;
+    for (int k = 0; k < 8; ++k) {
+      const int i = i0 + k * kNormedThreads + threadIdx.x;
+      x[k] = i < a.row_blocks ? part[i] : 0.f;
+    }
+#pragma unroll
+    for (int k = 0; k < 8; ++k) f2 += x[k];
   }
   f2 = warp_sum(f2);
   if ((threadIdx.x & 31) == 0) s_part[threadIdx.x >> 5] = f2;
@@ -209,6 +223,8 @@ __global__ void __launch_bounds__(kNormedThreads)
   const long long c0 = e0 - r0 * a.cols;  // offsets from it stay below cols + 4096
   const float* r = a.rinv + a.rows * blockIdx.y + r0;
   if (e0 + kNormedChunk <= n && aligned16(p) && aligned16(u)) {
+    const bool one_row = c0 + kNormedChunk <= a.cols;  // the whole chunk
+    const float f = *r;
     float pv[kNormedUnits][4], uv[kNormedUnits][4];
 #pragma unroll
     for (int w = 0; w < kNormedUnits; ++w) {
@@ -218,7 +234,12 @@ __global__ void __launch_bounds__(kNormedThreads)
 #pragma unroll
     for (int w = 0; w < kNormedUnits; ++w) {
       const int i = (w * kNormedThreads + threadIdx.x) * 4;
-      normed4<ROW4>(pv[w], uv[w], r, c0 + i, a.cols, a.decay, 4);
+      if (one_row) {
+#pragma unroll
+        for (int k = 0; k < 4; ++k) pv[w][k] = fmaf(f, uv[w][k], __fmul_rn(pv[w][k], a.decay));
+      } else {
+        normed4<ROW4>(pv[w], uv[w], r, c0 + i, a.cols, a.decay, 4);
+      }
       store4(p + i, pv[w]);
     }
   } else {

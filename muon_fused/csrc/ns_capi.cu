@@ -843,6 +843,20 @@ int heads_launch(const DeviceState& ds, const HeadsPlan& P, const CUtensorMap& g
   return FM_OK;
 }
 
+// The copy of G that TMA can address (heads_pack_kernel).
+template <typename S, typename T>
+int heads_pack(const DeviceState& ds, const HeadsPlan& P, const void* G, long long ldg,
+               long long bs_g, long long heads, long long head_stride, long long outer, int inner,
+               void* dst, cudaStream_t st) {
+  const long long want = (outer * (P.pack_ld / 8) + kPackThreads - 1) / kPackThreads;
+  const long long cap = std::max<long long>(1, ds.sm_count * 16ll / P.total);
+  const dim3 grid{unsigned(std::min(want, cap)), unsigned(P.total), 1};
+  FM_CUDA(launch_pdl(heads_pack_kernel<S, T>, grid, dim3(kPackThreads), 0, st, false,
+                     static_cast<const S*>(G), ldg, bs_g, int(heads), head_stride, outer, inner,
+                     static_cast<T*>(dst), int(P.pack_ld)));
+  return FM_OK;
+}
+
 int heads_check(long long batch, long long rows, long long cols, long long heads, int dim) {
   if (batch < 1 || rows < 1 || cols < 1 || heads < 1)
     return fail(FM_E_INVALID, "batch, rows, cols and heads must be positive");
@@ -940,23 +954,21 @@ int heads_run(const void* G, int dtype, long long batch, long long rows, long lo
   a.chunks = int((P.n + kApplyN - 1) / kApplyN);
   a.err = ds->err_word;
 
+  int rc;
   // strides of the G that the kernels read
   const void* src = G;
   long long ld = ldg, hs = cols_form ? P.d : P.d * ldg, ms = bs_g;
   if (!P.direct) {
     const long long outer = cols_form ? P.n : P.d;
     const int inner = int(cols_form ? P.d : P.n);
-    const long long blocks = std::min<long long>(outer, std::max<long long>(1, ds->sm_count * 8ll / P.total));
-    const dim3 grid(unsigned(blocks), unsigned(P.total));
-    if (half) {
-      FM_CUDA(launch_pdl(heads_pack_kernel<__half>, grid, dim3(256), 0, st, false, G, dtype, ldg,
-                         bs_g, int(heads), hs, outer, inner, reinterpret_cast<__half*>(ws + P.pack),
-                         P.pack_ld));
-    } else {
-      FM_CUDA(launch_pdl(heads_pack_kernel<__nv_bfloat16>, grid, dim3(256), 0, st, false, G, dtype,
-                         ldg, bs_g, int(heads), hs, outer, inner,
-                         reinterpret_cast<__nv_bfloat16*>(ws + P.pack), P.pack_ld));
+    void* dst = ws + P.pack;
+    switch (dtype) {
+      case FM_DT_BF16: rc = heads_pack<__nv_bfloat16, __nv_bfloat16>(*ds, P, G, ldg, bs_g, heads, hs, outer, inner, dst, st); break;
+      case FM_DT_F16: rc = heads_pack<__half, __half>(*ds, P, G, ldg, bs_g, heads, hs, outer, inner, dst, st); break;
+      case FM_DT_F32: rc = heads_pack<float, __nv_bfloat16>(*ds, P, G, ldg, bs_g, heads, hs, outer, inner, dst, st); break;
+      default: rc = heads_pack<double, __nv_bfloat16>(*ds, P, G, ldg, bs_g, heads, hs, outer, inner, dst, st);
     }
+    if (rc) return rc;
     src = ws + P.pack;
     ld = P.pack_ld;
     hs = outer * ld;
@@ -964,7 +976,6 @@ int heads_run(const void* G, int dtype, long long batch, long long rows, long lo
   }
   const long long inner = cols_form ? P.d : P.n, outer = cols_form ? P.n : P.d;
   CUtensorMap gram_map, g_map, o_map;
-  int rc;
   if ((rc = heads_map(&gram_map, src, inner, outer, heads, batch, ld, hs, ms, 64,
                       cols_form ? kHeadsK : P.dp)))
     return rc;
@@ -1050,10 +1061,12 @@ int normed_launch(const fm_normed_matrix* mats, int64_t count,
   constexpr long long kL2Keep = 64ll << 20;
   const long long group = std::max<long long>(
       1, std::min<long long>(kNormedList, kL2Keep / std::max<long long>(1, 2 * rows * cols)));
-  // A warp per row where the launch has rows for 16 warps an SM (or rows are
-  // short), a block per row where it has fewer and longer ones.
-  const bool wide = cols > 1024 && rows * std::min<long long>(group, count) < 148 * 16;
+  // A warp per row up to 4096 columns (16 loads of 16 bytes a lane), a block per
+  // longer row: the blocks of one wave then end apart, which streams faster than
+  // one wave of warps with long rows (bf16 4096 x 14336: 20 against 24 µs).
+  const bool wide = cols > 4096;
   const long long per = wide ? 1 : kNormedThreads / 32;
+  const long long blocks = std::min<long long>(kNormedMaxBlocks, (rows + per - 1) / per);
   const long long chunks = (rows * cols + kNormedChunk - 1) / kNormedChunk;
   if (chunks > 0x7fffffffll) return fail(FM_E_INVALID, "matrix %lld x %lld too large", rows, cols);
   for (int64_t i = 0; i < count; i += group) {
@@ -1067,8 +1080,8 @@ int normed_launch(const fm_normed_matrix* mats, int64_t count,
     a.rows = rows;
     a.cols = cols;
     a.rinv = ws + i * rows;
-    a.partials = ws + count * rows + i * kNormedMaxBlocks;
-    a.row_blocks = int(std::min<long long>(kNormedMaxBlocks, (rows + per - 1) / per));
+    a.partials = ws + count * rows + i * blocks;
+    a.row_blocks = int(blocks);
     a.decay = decay;
     a.step = step;
     a.beta2 = beta2;
@@ -1325,7 +1338,8 @@ int fm_normed_workspace_size(int64_t count, int64_t rows, uint64_t* bytes) {
   if (!bytes) return fail(FM_E_INVALID, "bytes is null");
   if (count < 0 || rows < 0 || count > (1 << 20) || rows > (1ll << 40))
     return fail(FM_E_INVALID, "count %lld / rows %lld out of range", (long long)count, (long long)rows);
-  *bytes = uint64_t(count) * (uint64_t(rows) + kNormedMaxBlocks) * 4;
+  // a factor per row, and a share of F² per block of the row pass
+  *bytes = uint64_t(count) * (uint64_t(rows) + std::min<uint64_t>(rows, kNormedMaxBlocks)) * 4;
   return FM_OK;
 }
 

@@ -937,26 +937,35 @@ __global__ void __launch_bounds__(kApplyThreads, 1)
 // ------------------------------------------------------------------- pack
 // Copy of G that TMA can address, for inputs it cannot (other types, unaligned
 // rows or heads): outer x inner blocks per head with a row stride of ld
-// elements, values rounded to T.  Padding columns are never read.
-template <typename T>
-__global__ void __launch_bounds__(256)
-    heads_pack_kernel(const void* __restrict__ G, int dtype, long long ldg, long long mat_stride,
-                      int heads, long long head_stride, long long outer, int inner, T* dst,
-                      long long ld) {
+// elements (a multiple of 8), values rounded to T.  A thread gathers eight
+// elements and stores 16 bytes; padding columns are never read.
+__device__ __forceinline__ float as_16(__nv_bfloat16 x) { return __bfloat162float(x); }
+__device__ __forceinline__ float as_16(__half x) { return __half2float(x); }
+__device__ __forceinline__ float as_16(float x) { return x; }
+__device__ __forceinline__ float as_16(double x) { return __bfloat162float(__double2bfloat16(x)); }
+
+constexpr int kPackThreads = 256;
+
+template <typename S, typename T>
+__global__ void __launch_bounds__(kPackThreads)
+    heads_pack_kernel(const S* __restrict__ G, long long ldg, long long mat_stride, int heads,
+                      long long head_stride, long long outer, int inner, T* __restrict__ dst,
+                      int ld) {
   pdl_wait();
   const int head = blockIdx.y;
-  const long long base = (head / heads) * mat_stride + (head % heads) * head_stride;
-  T* out = dst + head * outer * ld;
-  for (long long r = blockIdx.x; r < outer; r += gridDim.x) {
-    for (int c = threadIdx.x; c < inner; c += blockDim.x) {
-      const long long i = base + r * ldg + c;
-      float x;
-      if (dtype == 0) x = __bfloat162float(static_cast<const __nv_bfloat16*>(G)[i]);
-      else if (dtype == 1) x = __half2float(static_cast<const __half*>(G)[i]);
-      else if (dtype == 2) x = static_cast<const float*>(G)[i];
-      else x = __bfloat162float(__double2bfloat16(static_cast<const double*>(G)[i]));
-      out[r * ld + c] = from_f<T>(x);
-    }
+  const S* src = G + (head / heads) * mat_stride + (head % heads) * head_stride;
+  uint4* out = reinterpret_cast<uint4*>(dst + head * outer * ld);
+  const unsigned chunks = static_cast<unsigned>(ld) / 8;
+  const long long n = outer * chunks;
+  for (long long i = static_cast<long long>(blockIdx.x) * kPackThreads + threadIdx.x; i < n;
+       i += static_cast<long long>(gridDim.x) * kPackThreads) {
+    const long long r = n <= 0xffffffffll ? static_cast<unsigned>(i) / chunks : i / chunks;
+    const int c = static_cast<int>(i - r * chunks) * 8;
+    const S* p = src + r * ldg + c;
+    __align__(16) T v[8];
+#pragma unroll
+    for (int k = 0; k < 8; ++k) v[k] = from_f<T>(c + k < inner ? as_16(p[k]) : 0.f);
+    out[i] = *reinterpret_cast<const uint4*>(v);
   }
 }
 

@@ -15,6 +15,7 @@ from __future__ import annotations
 
 import ctypes
 import math
+import operator
 from collections.abc import Sequence
 
 import torch
@@ -25,6 +26,9 @@ from muon_fused._fused_muon_C import _check_cuda, _on_device, _stream
 
 STEP_DTYPES = {torch.float32: _lib.FM_DT_F32, torch.bfloat16: _lib.FM_DT_BF16,
                torch.float16: _lib.FM_DT_F16}
+
+
+_DTYPE = operator.attrgetter("dtype")
 
 
 def _check_list(tensors, name: str, count: int | None = None) -> list[torch.Tensor]:
@@ -115,17 +119,18 @@ def fused_adamw(
         raise RuntimeError("fused_adamw needs contiguous tensors")
     if not all(all(map(torch.Tensor.is_same_size, params, ts)) for ts in lists[1:]):
         raise RuntimeError("params, grads and moments must have the same shapes")
-    types = [(p.dtype, g.dtype, m.dtype, v.dtype) for p, g, m, v in zip(*lists)]
-    for pt, gt, mt, vt in set(types):
+    types = list(zip(*(map(_DTYPE, ts) for ts in lists)))
+    kinds = set(types)
+    for pt, gt, mt, vt in kinds:
         if pt not in STEP_DTYPES or gt != pt:
             raise RuntimeError(f"params and grads must be fp32, bf16 or fp16 of one type, got "
                                f"{pt} and {gt}")
         if mt != vt or mt not in (pt, torch.float32):
             raise RuntimeError(f"moments must have the parameter's type or fp32, got {mt} and {vt}")
-    for kind in dict.fromkeys(types):
-        if types.count(kind) == n:
-            adamw_launch(*lists, alphas, lr, wd, betas, eps)
-        else:
+    if len(kinds) == 1:
+        adamw_launch(*lists, alphas, lr, wd, betas, eps)
+    else:
+        for kind in dict.fromkeys(types):
             idx = [i for i in range(n) if types[i] == kind]
             adamw_launch(*([ts[i] for i in idx] for ts in lists), [alphas[i] for i in idx], lr, wd,
                          betas, eps)
