@@ -22,7 +22,14 @@ _DTYPE_CODE = {
 }
 
 
+# torch's own shortcut to the current stream's handle: the public call builds a
+# Stream object first, 2 µs of a 25 µs call on a small matrix.
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+
+
 def _stream(t: torch.Tensor) -> int:
+    if _raw_stream is not None:
+        return _raw_stream(t.get_device())
     return torch.cuda.current_stream(t.device).cuda_stream
 
 

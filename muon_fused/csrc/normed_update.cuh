@@ -183,24 +183,27 @@ __global__ void __launch_bounds__(kNormedThreads)
     rinv[r] *= eta;
 }
 
-// Four elements from offset o of the block's first row: p = p·decay + f·u, where
-// f is the factor of each element's row.  A unit of four lies in one row where
-// cols divides by 4 (ROW4); else the rows of its elements are found singly.
+// Four elements, the i-th.. of a chunk whose first row ends after `rem` elements
+// of it: p = p·decay + f·u, where f is the factor of each element's row.  The four
+// lie in one row where cols divides by 4 (ROW4), else in two at most where a row
+// has four elements.
 template <bool ROW4>
-__device__ __forceinline__ void normed4(float (&p)[4], const float (&u)[4], const float* r,
-                                        long long o, long long cols, float decay, int cnt) {
+__device__ __forceinline__ void normed4(float (&p)[4], const float (&u)[4], const float* r, int i,
+                                        int rem, unsigned cols, float decay, int cnt) {
   float f[4];
+  const unsigned past = static_cast<unsigned>(i - rem);
+  const unsigned q = i < rem ? 0u : 1u + past / cols;
   if constexpr (ROW4) {
-    const unsigned q = o < cols ? 0u : static_cast<unsigned>(o) / static_cast<unsigned>(cols);
-    f[0] = r[q];
-    f[1] = f[2] = f[3] = f[0];
+    f[0] = f[1] = f[2] = f[3] = r[q];
+  } else if (cols >= 4) {
+    const unsigned left = i < rem ? static_cast<unsigned>(rem - i) : cols - past % cols;
+    const float f0 = r[q], f1 = left < static_cast<unsigned>(min(4, cnt)) ? r[q + 1] : f0;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) f[k] = static_cast<unsigned>(k) < left ? f0 : f1;
   } else {
 #pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      const unsigned q =
-          o + k < cols ? 0u : static_cast<unsigned>(o + k) / static_cast<unsigned>(cols);
-      f[k] = k < cnt ? r[q] : 0.f;
-    }
+    for (int k = 0; k < 4; ++k)
+      f[k] = k < cnt ? r[i + k < rem ? 0u : 1u + static_cast<unsigned>(i + k - rem) / cols] : 0.f;
   }
 #pragma unroll
   for (int k = 0; k < 4; ++k) p[k] = fmaf(f[k], u[k], __fmul_rn(p[k], decay));
@@ -220,10 +223,13 @@ __global__ void __launch_bounds__(kNormedThreads)
   const long long r0 = n <= 0xffffffffll
                            ? static_cast<unsigned>(e0) / static_cast<unsigned>(a.cols)
                            : e0 / a.cols;
-  const long long c0 = e0 - r0 * a.cols;  // offsets from it stay below cols + 4096
+  // elements of the chunk in its first row, and a row's length, in 32 bits (a row
+  // past that is longer than any chunk)
+  const int rem = static_cast<int>(min((r0 + 1) * a.cols - e0, 0x7fffffffll));
+  const unsigned cols = static_cast<unsigned>(min(a.cols, 0xffffffffll));
   const float* r = a.rinv + a.rows * blockIdx.y + r0;
   if (e0 + kNormedChunk <= n && aligned16(p) && aligned16(u)) {
-    const bool one_row = c0 + kNormedChunk <= a.cols;  // the whole chunk
+    const bool one_row = rem >= kNormedChunk;  // the whole chunk
     const float f = *r;
     float pv[kNormedUnits][4], uv[kNormedUnits][4];
 #pragma unroll
@@ -238,7 +244,7 @@ __global__ void __launch_bounds__(kNormedThreads)
 #pragma unroll
         for (int k = 0; k < 4; ++k) pv[w][k] = fmaf(f, uv[w][k], __fmul_rn(pv[w][k], a.decay));
       } else {
-        normed4<ROW4>(pv[w], uv[w], r, c0 + i, a.cols, a.decay, 4);
+        normed4<ROW4>(pv[w], uv[w], r, i, rem, cols, a.decay, 4);
       }
       store4(p + i, pv[w]);
     }
@@ -251,7 +257,7 @@ __global__ void __launch_bounds__(kNormedThreads)
         pv[k] = i + k < cnt ? to_f(p[i + k]) : 0.f;
         uv[k] = i + k < cnt ? __bfloat162float(u[i + k]) : 0.f;
       }
-      normed4<ROW4>(pv, uv, r, c0 + i, a.cols, a.decay, cnt - i);
+      normed4<ROW4>(pv, uv, r, i, rem, cols, a.decay, cnt - i);
 #pragma unroll
       for (int k = 0; k < 4; ++k)
         if (i + k < cnt) p[i + k] = from_f<T>(pv[k]);

@@ -241,8 +241,11 @@ class FusedMuon(Optimizer):
     def _batch_limit(self, rows: int, cols: int, group=None) -> int:
         """Matrices per batched call so inputs, outputs and workspace of one
         batch stay within ``batch_bytes``."""
-        per = self._ns_workspace(group or {}, 1, rows, cols) + 4 * rows * cols
-        return max(1, min(64, self._batch_bytes // per))
+        group = group or {}
+        per = self._ns_workspace(group, 1, rows, cols) + 4 * rows * cols
+        # at most 65535 heads in one per-head call
+        most = min(64, 65535 // (group.get("heads") or 1))
+        return max(1, min(most, self._batch_bytes // per))
 
     def _orthogonalise_batch(self, params, group, out=None) -> torch.Tensor:
         """Momentum + Newton-Schulz for same-shape parameters in one batched

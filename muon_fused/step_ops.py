@@ -97,7 +97,8 @@ def fused_adamw(
     moments2 = _check_list(moments2, "moments2", n)
     if not all(0.0 <= b < 1.0 for b in betas):
         raise RuntimeError(f"betas must be in [0, 1), got {betas}")
-    if isinstance(steps, int):
+    if not isinstance(steps, Sequence):
+        steps = int(steps)
         if steps < 1:
             raise RuntimeError("steps must be >= 1")
         alphas = [adamw_alpha(lr, betas, steps)] * n

@@ -186,6 +186,45 @@ def test_many_heads_across_waves(cuda_lib):
         check(fused_newton_schulz_heads(G, 64, dim=dim), G, 64, 5, dim)
 
 
+@pytest.mark.parametrize("heads", [1, 18, 20, 24, 29, 37, 49, 74, 75])
+def test_every_split_of_the_long_side(cuda_lib, heads):
+    """148 // heads splits, 8 at most, at least 256 elements each: cluster sizes 8 to 1."""
+    from muon_fused import fused_newton_schulz_heads
+
+    for n in (2048, 1900):
+        G = rand((heads * 24, n), heads)
+        check(fused_newton_schulz_heads(G, heads), G, heads, 5, 0)
+
+
+@pytest.mark.parametrize("d,n", [(128, 65536), (64, 200001)])
+def test_long_sides(cuda_lib, d, n):
+    from muon_fused import fused_newton_schulz_heads
+
+    G = rand((2 * d, n), 1)
+    check(fused_newton_schulz_heads(G, 2), G, 2, 5, 0)
+    T = G.T.contiguous()
+    check(fused_newton_schulz_heads(T, 2, dim=1), T, 2, 5, 1)
+
+
+def test_two_calls_at_once(cuda_lib):
+    """Calls that overlap on two streams, with their own workspaces."""
+    from muon_fused import fused_newton_schulz_heads
+
+    Gs = [rand((16 * 128, 1024), s) for s in (1, 2)]
+    want = [fused_newton_schulz_heads(G, 16) for G in Gs]
+    streams = [torch.cuda.Stream() for _ in Gs]
+    torch.cuda.synchronize()
+    got = [[], []]
+    for _ in range(20):
+        for k, st in enumerate(streams):
+            with torch.cuda.stream(st):
+                got[k].append(fused_newton_schulz_heads(Gs[k], 16))
+    torch.cuda.synchronize()
+    for k in range(2):
+        for o in got[k]:
+            assert torch.equal(o, want[k])
+
+
 @pytest.mark.parametrize("dim", [0, 1])
 def test_wide_heads_run_as_a_batch(cuda_lib, dim):
     """Heads of 256: the bf16 path's accuracy (1e-2, as its own tests)."""
