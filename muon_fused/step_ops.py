@@ -41,6 +41,16 @@ def _check_list(tensors, name: str, count: int | None = None) -> list[torch.Tens
     return tensors
 
 
+def _same_shapes(lists) -> bool:
+    """Whether the lists' shapes agree: by sizes and dimensions, and for more than
+    one dimension by the shapes themselves (their objects are slow to make)."""
+    first = lists[0]
+    numels, dims = list(map(torch.Tensor.numel, first)), list(map(torch.Tensor.dim, first))
+    many = [i for i, d in enumerate(dims) if d > 1]
+    return all(list(map(torch.Tensor.numel, ts)) == numels and list(map(torch.Tensor.dim, ts)) == dims
+               and all(first[i].is_same_size(ts[i]) for i in many) for ts in lists[1:])
+
+
 def adamw_launch(params, grads, moments1, moments2, alphas, lr: float, wd: float, betas,
                  eps: float) -> None:
     """The call after the checks: tensors of one device, one parameter type and
@@ -118,7 +128,7 @@ def fused_adamw(
         raise RuntimeError("fused_adamw needs all tensors on one device")
     if not all(all(map(torch.Tensor.is_contiguous, ts)) for ts in lists):
         raise RuntimeError("fused_adamw needs contiguous tensors")
-    if not all(all(map(torch.Tensor.is_same_size, params, ts)) for ts in lists[1:]):
+    if not _same_shapes(lists):
         raise RuntimeError("params, grads and moments must have the same shapes")
     types = list(zip(*(map(_DTYPE, ts) for ts in lists)))
     kinds = set(types)
@@ -144,6 +154,19 @@ def normed_workspace_size(count: int, rows: int) -> int:
     _lib.check(_lib.load().fm_normed_workspace_size(int(count), int(rows), ctypes.byref(out)),
                "fm_normed_workspace_size")
     return int(out.value)
+
+
+def _refuse_normed(p0, p, u, v, rows) -> None:
+    """Name what is wrong with one matrix of a fused_normed_update call."""
+    if not (p.device == u.device == v.device == p0.device):
+        raise RuntimeError("fused_normed_update needs all tensors on one device")
+    if p.dtype != p0.dtype or p.shape != p0.shape:
+        raise RuntimeError("the params of one call must have one shape and type")
+    if u.dtype != torch.bfloat16 or u.numel() != p.numel() or not u.dim() or u.size(0) != rows:
+        raise RuntimeError("updates must be bf16 and shaped like the parameters")
+    if v.dtype != torch.float32 or v.shape != (rows,):
+        raise RuntimeError("row_moments must be fp32 vectors of one element per row")
+    raise RuntimeError("fused_normed_update needs contiguous tensors")
 
 
 def fused_normed_update(
@@ -190,23 +213,18 @@ def fused_normed_update(
     _check_cuda(p0, "params")
     if p0.dim() < 2:
         raise RuntimeError("fused_normed_update needs matrices")
-    if p0.dtype not in STEP_DTYPES:
-        raise RuntimeError(f"params must be fp32, bf16 or fp16, got {p0.dtype}")
-    rows = p0.size(0)
-    cols = p0.numel() // rows if rows else 0
-    if len(set().union(*(map(torch.Tensor.get_device, ts)
-                         for ts in (params, updates, row_moments)))) != 1:
-        raise RuntimeError("fused_normed_update needs all tensors on one device")
+    dtype, numel, rows = p0.dtype, p0.numel(), p0.size(0)
+    if dtype not in STEP_DTYPES:
+        raise RuntimeError(f"params must be fp32, bf16 or fp16, got {dtype}")
+    device, cols = p0.get_device(), numel // rows if rows else 0
     for p, u, v in zip(params, updates, row_moments):
-        if p.dtype != p0.dtype or not p.is_same_size(p0):
-            raise RuntimeError("the params of one call must have one shape and type")
-        if u.dtype != torch.bfloat16 or u.numel() != p.numel() or (u.dim() and u.size(0) != rows):
-            raise RuntimeError("updates must be bf16 and shaped like the parameters")
-        if v.dtype != torch.float32 or v.dim() != 1 or v.numel() != rows:
-            raise RuntimeError("row_moments must be fp32 vectors of one element per row")
-        if not (p.is_contiguous() and u.is_contiguous() and v.is_contiguous()):
-            raise RuntimeError("fused_normed_update needs contiguous tensors")
-    if p0.numel() == 0:
+        if not (p.dtype is dtype and p.is_same_size(p0) and u.dtype is torch.bfloat16
+                and u.numel() == numel and (u.size(0) if u.dim() else -1) == rows
+                and v.dtype is torch.float32 and v.dim() == 1 and v.numel() == rows
+                and p.get_device() == u.get_device() == v.get_device() == device
+                and p.is_contiguous() and u.is_contiguous() and v.is_contiguous()):
+            _refuse_normed(p0, p, u, v, rows)
+    if numel == 0:
         return
     need = normed_workspace_size(n, rows)
     if workspace is None:
