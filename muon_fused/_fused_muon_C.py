@@ -140,6 +140,12 @@ def newton_schulz_heads(G: torch.Tensor, heads: int, steps: int = 5, dim: int = 
     """Newton-Schulz of each head of a (rows, cols) or (batch, rows, cols)
     projection (heads are blocks of rows, or of columns for dim=1); returns a
     bf16 tensor of G's shape (or writes ``out``, contiguous, bf16, that shape)."""
+    # the plain case in one call; anything else is checked or copied here
+    res = _lib.step_ext().heads(G, heads, dim, steps, workspace, out)
+    if isinstance(res, int):
+        _lib.check(res, "fm_newton_schulz_heads")
+    elif res is not None:
+        return res
     _check_cuda(G, "G")
     if G.dim() not in (2, 3):
         raise RuntimeError("G must be 2D or 3D (batch, rows, cols)")

@@ -86,6 +86,30 @@ def load() -> ctypes.CDLL:
     return _lib
 
 
+_ext = None
+
+
+def step_ext():
+    """Import (once) and return the extension that reads torch's tensors for the
+    step operators' C calls (csrc/step_ext.cpp), raising if it is absent."""
+    global _ext
+    if _ext is None:
+        lib = load()
+        with _lock:
+            try:
+                from muon_fused import _step_ext as ext
+            except ImportError as e:
+                raise ImportError(
+                    f"muon_fused/_step_ext.so is missing or does not fit this torch ({e}); build it "
+                    "with `python -m muon_fused.build`") from e
+            ext.bind(*(ctypes.cast(fn, _vp).value
+                       for fn in (lib.fm_adamw, lib.fm_muon_apply_normed,
+                                  lib.fm_normed_workspace_size, lib.fm_newton_schulz_heads,
+                                  lib.fm_heads_workspace_size)))
+            _ext = ext
+    return _ext
+
+
 def check(rc: int, what: str) -> None:
     if rc != FM_OK:
         msg = load().fm_last_error().decode(errors="replace")

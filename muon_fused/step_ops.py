@@ -41,20 +41,16 @@ def _check_list(tensors, name: str, count: int | None = None) -> list[torch.Tens
     return tensors
 
 
-def _same_shapes(lists) -> bool:
-    """Whether the lists' shapes agree: by sizes and dimensions, and for more than
-    one dimension by the shapes themselves (their objects are slow to make)."""
-    first = lists[0]
-    numels, dims = list(map(torch.Tensor.numel, first)), list(map(torch.Tensor.dim, first))
-    many = [i for i, d in enumerate(dims) if d > 1]
-    return all(list(map(torch.Tensor.numel, ts)) == numels and list(map(torch.Tensor.dim, ts)) == dims
-               and all(first[i].is_same_size(ts[i]) for i in many) for ts in lists[1:])
-
-
 def adamw_launch(params, grads, moments1, moments2, alphas, lr: float, wd: float, betas,
                  eps: float) -> None:
     """The call after the checks: tensors of one device, one parameter type and
-    one moment type, all contiguous; ``alphas`` holds each tensor's -lr/scale."""
+    one moment type, all contiguous; ``alphas`` holds each tensor's -lr/scale.
+    Version counters stay as they are."""
+    rc = _lib.step_ext().adamw(params, grads, moments1, moments2, alphas, float(1 - lr * wd),
+                               1 - betas[0], 1 - betas[1], float(eps), False)
+    if rc is not None:
+        _lib.check(rc, "fm_adamw")
+        return
     ptr = torch.Tensor.data_ptr
     table = b"".join(map(_lib.ADAMW_TENSOR.pack, map(ptr, params), map(ptr, grads),
                          map(ptr, moments1), map(ptr, moments2),
@@ -100,35 +96,40 @@ def fused_adamw(
     A list may mix types and sizes; tensors of zero elements are skipped.  What
     a call writes must not share memory with another of its tensors.
     """
+    if not all(0.0 <= b < 1.0 for b in betas):
+        raise RuntimeError(f"betas must be in [0, 1), got {betas}")
+    if isinstance(steps, Sequence):
+        if any(t < 1 for t in steps):
+            raise RuntimeError("steps must be >= 1")
+        alphas = [adamw_alpha(lr, betas, int(t)) for t in steps]
+    else:
+        if steps < 1:
+            raise RuntimeError("steps must be >= 1")
+        alphas = adamw_alpha(lr, betas, int(steps))
+    # the plain case in one call; anything else is checked here and taken apart
+    rc = _lib.step_ext().adamw(params, grads, moments1, moments2, alphas, float(1 - lr * wd),
+                               1 - betas[0], 1 - betas[1], float(eps), True)
+    if rc is not None:
+        _lib.check(rc, "fm_adamw")
+        return
     params = _check_list(params, "params")
     n = len(params)
     grads = _check_list(grads, "grads", n)
     moments1 = _check_list(moments1, "moments1", n)
     moments2 = _check_list(moments2, "moments2", n)
-    if not all(0.0 <= b < 1.0 for b in betas):
-        raise RuntimeError(f"betas must be in [0, 1), got {betas}")
-    if not isinstance(steps, Sequence):
-        steps = int(steps)
-        if steps < 1:
-            raise RuntimeError("steps must be >= 1")
-        alphas = [adamw_alpha(lr, betas, steps)] * n
-    else:
-        steps = [int(t) for t in steps]
-        if len(steps) != n:
-            raise RuntimeError(f"steps must be an int or one per parameter, got {len(steps)} for {n}")
-        if any(t < 1 for t in steps):
-            raise RuntimeError("steps must be >= 1")
-        alphas = [adamw_alpha(lr, betas, t) for t in steps]
+    if not isinstance(alphas, list):
+        alphas = [alphas] * n
+    elif len(alphas) != n:
+        raise RuntimeError(f"steps must be an int or one per parameter, got {len(alphas)} for {n}")
     if n == 0:
         return
     _check_cuda(params[0], "params")
     lists = (params, grads, moments1, moments2)
-    # bulk checks: a long list of small tensors is bound by this loop, not the kernel
     if len(set().union(*(map(torch.Tensor.get_device, ts) for ts in lists))) != 1:
         raise RuntimeError("fused_adamw needs all tensors on one device")
     if not all(all(map(torch.Tensor.is_contiguous, ts)) for ts in lists):
         raise RuntimeError("fused_adamw needs contiguous tensors")
-    if not _same_shapes(lists):
+    if not all(all(map(torch.Tensor.is_same_size, params, ts)) for ts in lists[1:]):
         raise RuntimeError("params, grads and moments must have the same shapes")
     types = list(zip(*(map(_DTYPE, ts) for ts in lists)))
     kinds = set(types)
@@ -200,13 +201,19 @@ def fused_normed_update(
         workspace: optional CUDA buffer of at least
             ``normed_workspace_size(count, rows)`` bytes.
     """
+    if not 0.0 <= beta2 < 1.0:
+        raise RuntimeError(f"beta2 must be in [0, 1), got {beta2}")
+    # the plain case in one call; anything else is checked here
+    rc = _lib.step_ext().normed(params, updates, row_moments, float(1 - lr * wd), float(lr * 0.2),
+                                float(beta2), float(eps), workspace)
+    if rc is not None:
+        _lib.check(rc, "fm_muon_apply_normed")
+        return
     params = _check_list(params, "params")
     n = len(params)
     updates = list(updates.unbind(0)) if isinstance(updates, torch.Tensor) else list(updates)
     updates = _check_list(updates, "updates", n)
     row_moments = _check_list(row_moments, "row_moments", n)
-    if not 0.0 <= beta2 < 1.0:
-        raise RuntimeError(f"beta2 must be in [0, 1), got {beta2}")
     if n == 0:
         return
     p0 = params[0]

@@ -122,6 +122,30 @@ def test_adamw_mixed_types_views_and_long_lists(cuda_lib):
             assert _same(x, y)
 
 
+def test_adamw_accepts_what_it_documents(cuda_lib):
+    """Tuples, parameters, subclasses of tensors and a count per tensor, in the
+    plain case (one C++ call) and beside it, give the same values."""
+    from muon_fused import fused_adamw
+
+    class Sub(torch.Tensor):
+        pass
+
+    st = _adam_state([(33,), (5, 7)], torch.float32, torch.float32)
+    want = [[t.clone() for t in ts] for ts in st]
+    fused_adamw(*want, [3, 4], lr=LR, wd=WD)
+    for wrap in (lambda t: torch.nn.Parameter(t, requires_grad=False), lambda t: t.as_subclass(Sub)):
+        got = [[t.clone() for t in ts] for ts in st]
+        got[0] = [wrap(t) for t in got[0]]
+        fused_adamw(*map(tuple, got), (3, 4), lr=LR, wd=WD)
+        for xs, ys in zip(got, want):
+            for x, y in zip(xs, ys):
+                assert torch.equal(x.detach().as_subclass(torch.Tensor), y)
+    with pytest.raises(RuntimeError, match="one per parameter"):
+        fused_adamw(*st, [1, 2, 3], lr=LR)
+    with pytest.raises(RuntimeError, match="one tensor per parameter"):
+        fused_adamw(st[0], st[1][:1], st[2], st[3], 1, lr=LR)
+
+
 def test_adamw_nonfinite_values_stay_in_place(cuda_lib):
     """inf and NaN gradients give what torch gives, in their elements only."""
     from muon_fused import fused_adamw

@@ -182,6 +182,17 @@ def test_adamw_group_keeps_its_results(cuda_lib, dtype):
         assert torch.equal(p.detach(), r.detach()), i
 
 
+def test_adamw_group_leaves_version_counters(cuda_lib):
+    """The branch writes through .data: a graph kept across a step can still run backward."""
+    from muon_fused import FusedMuon
+
+    p = torch.nn.Parameter(torch.ones(64, device=DEV))
+    loss = (p * p).sum()
+    loss.backward(retain_graph=True)
+    FusedMuon([p], lr=0.01).step()
+    loss.backward()
+
+
 def test_checkpoint_resumes_bit_for_bit(cuda_lib):
     from muon_fused import FusedMuon
 
