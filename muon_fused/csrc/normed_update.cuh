@@ -152,14 +152,9 @@ __global__ void __launch_bounds__(kNormedThreads, 6)
     a.partials[static_cast<long long>(blockIdx.y) * a.row_blocks + blockIdx.x] = f2;
 }
 
-// Turns r into -step/(F + 1e-7) · r, every block adding up the shares in the
-// same order.
-__global__ void __launch_bounds__(kNormedThreads)
-    normed_scale_kernel(const __grid_constant__ NormedArgs a) {
-  __shared__ float s_part[kNormedThreads / 32];
-  pdl_wait();
+// -step / (F + 1e-7) from the shares of F², added by the whole block in one order.
+__device__ __forceinline__ float normed_eta(const NormedArgs& a, float* s_part) {
   const float* part = a.partials + static_cast<long long>(blockIdx.y) * a.row_blocks;
-  float* rinv = a.rinv + a.rows * blockIdx.y;
   float f2 = 0.f;
   for (int i0 = 0; i0 < a.row_blocks; i0 += 8 * kNormedThreads) {
     float x[8];
@@ -177,19 +172,28 @@ __global__ void __launch_bounds__(kNormedThreads)
   f2 = 0.f;
 #pragma unroll
   for (int w = 0; w < kNormedThreads / 32; ++w) f2 += s_part[w];
-  const float eta = -a.step / (sqrtf(f2) + 1e-7f);
+  return -a.step / (sqrtf(f2) + 1e-7f);
+}
+
+// Turns r into -step/(F + 1e-7) · r.
+__global__ void __launch_bounds__(kNormedThreads)
+    normed_scale_kernel(const __grid_constant__ NormedArgs a) {
+  __shared__ float s_part[kNormedThreads / 32];
+  pdl_wait();
+  float* rinv = a.rinv + a.rows * blockIdx.y;
+  const float eta = normed_eta(a, s_part);
   for (long long r = static_cast<long long>(blockIdx.x) * kNormedThreads + threadIdx.x; r < a.rows;
        r += static_cast<long long>(gridDim.x) * kNormedThreads)
     rinv[r] *= eta;
 }
 
 // Four elements, the i-th.. of a chunk whose first row ends after `rem` elements
-// of it: p = p·decay + f·u, where f is the factor of each element's row.  The four
+// of it: p = p·decay + eta·f·u, where f is the factor of each element's row.  The four
 // lie in one row where cols divides by 4 (ROW4), else in two at most where a row
 // has four elements.
 template <bool ROW4>
 __device__ __forceinline__ void normed4(float (&p)[4], const float (&u)[4], const float* r, int i,
-                                        int rem, unsigned cols, float decay, int cnt) {
+                                        int rem, unsigned cols, float decay, float eta, int cnt) {
   float f[4];
   const unsigned past = static_cast<unsigned>(i - rem);
   const unsigned q = i < rem ? 0u : 1u + past / cols;
@@ -206,13 +210,16 @@ __device__ __forceinline__ void normed4(float (&p)[4], const float (&u)[4], cons
       f[k] = k < cnt ? r[i + k < rem ? 0u : 1u + static_cast<unsigned>(i + k - rem) / cols] : 0.f;
   }
 #pragma unroll
-  for (int k = 0; k < 4; ++k) p[k] = fmaf(f[k], u[k], __fmul_rn(p[k], decay));
+  for (int k = 0; k < 4; ++k) p[k] = fmaf(eta * f[k], u[k], __fmul_rn(p[k], decay));
 }
 
-// One block per chunk of 4096 consecutive elements, the last chunk first.
-template <typename T, bool ROW4>
+// One block per chunk of 4096 consecutive elements, the last chunk first.  FOLD:
+// r is not scaled yet, and every block adds up the shares itself: for matrices of
+// a few blocks an SM, where that chain costs less than the launch it replaces.
+template <typename T, bool ROW4, bool FOLD>
 __global__ void __launch_bounds__(kNormedThreads)
     normed_apply_kernel(const __grid_constant__ NormedArgs a) {
+  __shared__ float s_part[kNormedThreads / 32];
   pdl_wait();
   const NormedEntry e = a.e[blockIdx.y];
   const long long n = a.rows * a.cols;
@@ -230,13 +237,15 @@ __global__ void __launch_bounds__(kNormedThreads)
   const float* r = a.rinv + a.rows * blockIdx.y + r0;
   if (e0 + kNormedChunk <= n && aligned16(p) && aligned16(u)) {
     const bool one_row = rem >= kNormedChunk;  // the whole chunk
-    const float f = *r;
+    float f = *r;
     float pv[kNormedUnits][4], uv[kNormedUnits][4];
 #pragma unroll
     for (int w = 0; w < kNormedUnits; ++w) {
       load4(p + (w * kNormedThreads + threadIdx.x) * 4, pv[w]);
       load4(u + (w * kNormedThreads + threadIdx.x) * 4, uv[w]);
     }
+    const float eta = FOLD ? normed_eta(a, s_part) : 1.f;
+    f *= eta;
 #pragma unroll
     for (int w = 0; w < kNormedUnits; ++w) {
       const int i = (w * kNormedThreads + threadIdx.x) * 4;
@@ -244,12 +253,13 @@ __global__ void __launch_bounds__(kNormedThreads)
 #pragma unroll
         for (int k = 0; k < 4; ++k) pv[w][k] = fmaf(f, uv[w][k], __fmul_rn(pv[w][k], a.decay));
       } else {
-        normed4<ROW4>(pv[w], uv[w], r, i, rem, cols, a.decay, 4);
+        normed4<ROW4>(pv[w], uv[w], r, i, rem, cols, a.decay, eta, 4);
       }
       store4(p + i, pv[w]);
     }
   } else {
     const int cnt = static_cast<int>(min(static_cast<long long>(kNormedChunk), n - e0));
+    const float eta = FOLD ? normed_eta(a, s_part) : 1.f;
     for (int i = threadIdx.x * 4; i < cnt; i += kNormedThreads * 4) {
       float pv[4], uv[4];
 #pragma unroll
@@ -257,7 +267,7 @@ __global__ void __launch_bounds__(kNormedThreads)
         pv[k] = i + k < cnt ? to_f(p[i + k]) : 0.f;
         uv[k] = i + k < cnt ? __bfloat162float(u[i + k]) : 0.f;
       }
-      normed4<ROW4>(pv, uv, r, i, rem, cols, a.decay, cnt - i);
+      normed4<ROW4>(pv, uv, r, i, rem, cols, a.decay, eta, cnt - i);
 #pragma unroll
       for (int k = 0; k < 4; ++k)
         if (i + k < cnt) p[i + k] = from_f<T>(pv[k]);
