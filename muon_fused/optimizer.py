@@ -451,7 +451,7 @@ class FusedMuon(Optimizer):
                     ts.append(t)
                 continue
             data = p.data
-            if buf1.dtype != g.dtype:  # fp32 moments beside 16-bit parameters
+            if buf1.dtype != g.dtype and buf1.dtype == torch.float32:  # beside 16-bit parameters
                 g = g.to(buf1.dtype)
                 data = data.to(buf1.dtype)
             buf1.lerp_(g, 1 - beta1)

@@ -41,6 +41,11 @@ def _check_list(tensors, name: str, count: int | None = None) -> list[torch.Tens
     return tensors
 
 
+def _bump(tensors) -> None:
+    """Tell autograd of the writes; inference tensors keep no version."""
+    increment_version([t for t in tensors if not t.is_inference()])
+
+
 def adamw_launch(params, grads, moments1, moments2, alphas, lr: float, wd: float, betas,
                  eps: float) -> None:
     """The call after the checks: tensors of one device, one parameter type and
@@ -146,7 +151,7 @@ def fused_adamw(
             idx = [i for i in range(n) if types[i] == kind]
             adamw_launch(*([ts[i] for i in idx] for ts in lists), [alphas[i] for i in idx], lr, wd,
                          betas, eps)
-    increment_version(params + moments1 + moments2)
+    _bump(params + moments1 + moments2)
 
 
 def normed_workspace_size(count: int, rows: int) -> int:
@@ -250,4 +255,4 @@ def fused_normed_update(
             table, n, rows, cols, STEP_DTYPES[p0.dtype], float(1 - lr * wd),
             float(lr * 0.2 * math.sqrt(rows * cols)), float(beta2), float(eps), workspace.data_ptr(), workspace.nbytes,
             _stream(p0)), "fm_muon_apply_normed")
-    increment_version(params + row_moments)
+    _bump(params + row_moments)

@@ -342,6 +342,19 @@ def test_step_ops_on_a_side_stream_and_in_a_graph(cuda_lib):
     assert torch.equal(p, p2) and torch.equal(v, v2)
 
 
+def test_inference_tensors(cuda_lib):
+    from muon_fused import fused_adamw, fused_normed_update
+
+    with torch.inference_mode():
+        st = _adam_state([(9,)], torch.float32, torch.float32)
+        p, u, v = _rand((4, 8), 0), _rand((1, 4, 8), 1, 0.1, torch.bfloat16), torch.zeros(4, device=DEV)
+        want = [[t.clone() for t in ts] for ts in st]
+        fused_adamw(*st, 1, lr=LR)
+        fused_normed_update([p], u, [v], lr=LR)
+    _torch_chain(*[ts[0].clone() for ts in want], 1, LR, 0.1, (0.9, 0.95), 1e-8)
+    assert bool(v.all()) and not torch.equal(st[0][0], want[0][0])
+
+
 def test_writes_are_seen_by_autograd(cuda_lib):
     """A backward through a value saved before the step fails instead of using the new one."""
     from muon_fused import fused_adamw
