@@ -837,7 +837,8 @@ int heads_launch(const DeviceState& ds, const HeadsPlan& P, const CUtensorMap& g
                      IterCfg<DP>::kSmem, st, false, a));
   const long long units = P.total * a.chunks;
   FM_CUDA(launch_pdl(heads_apply_kernel<DP, COLS, HALF>,
-                     dim3(unsigned(std::min<long long>(units, ds.sm_count))), dim3(kApplyThreads),
+                     dim3(unsigned(std::min<long long>(units, ds.sm_count * ApplyCfg<DP>::kCtas))),
+                     dim3(kApplyThreads),
                      ApplyCfg<DP>::kSmem, st, false, g_map, o_map, a));
   timer_end(tm, st);
   return FM_OK;

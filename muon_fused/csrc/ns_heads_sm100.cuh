@@ -71,7 +71,6 @@ __host__ __device__ constexpr uint32_t make_idesc_16(bool half, int M, int N, in
 constexpr int kHeadsMaxDim = 128;
 constexpr int kHeadsMaxSteps = 8;
 constexpr int kHeadsK = 64;        // reduction columns per gram stage (one swizzle row)
-constexpr int kGramStages = 6;
 constexpr int kGramMaxSplit = 8;   // portable cluster size
 constexpr int kGramThreads = 192;  // producer, MMA, 4 epilogue warps
 constexpr int kApplyN = 128;       // long-side elements per apply unit
@@ -115,10 +114,12 @@ struct HeadsArgs {
 // ------------------------------------------------------------------- gram
 template <int DP>
 struct GramCfg {
+  // Two CTAs an SM for DP = 128, four for 64.
+  static constexpr int kStages = DP == 128 ? 6 : 5;
   static constexpr int kStage = DP * kHeadsK * 2;
   // MMAs of M = 128 on DP = 64 read one stage past the last
-  static constexpr int kSmem = (kGramStages + (DP == 64 ? 1 : 0)) * kStage + 1024 + 256;
-  static_assert(DP * DP * 4 <= kGramStages * kStage, "the fp32 partial reuses the stages");
+  static constexpr int kSmem = (kStages + (DP == 64 ? 1 : 0)) * kStage + 1024 + 256;
+  static_assert(DP * DP * 4 <= kStages * kStage, "the fp32 partial reuses the stages");
 };
 
 // A cluster of g.split CTAs per head, each with a range of n; its CTAs then add
@@ -133,16 +134,16 @@ __global__ void __launch_bounds__(kGramThreads)
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
                                              ~static_cast<uintptr_t>(1023));
-  constexpr int kStage = GramCfg<DP>::kStage;
-  uint64_t* full = reinterpret_cast<uint64_t*>(smem + (kGramStages + (DP == 64 ? 1 : 0)) * kStage);
-  uint64_t* empty = full + kGramStages;
-  uint64_t* acc_bar = empty + kGramStages;
+  constexpr int kStage = GramCfg<DP>::kStage, kStages = GramCfg<DP>::kStages;
+  uint64_t* full = reinterpret_cast<uint64_t*>(smem + (kStages + (DP == 64 ? 1 : 0)) * kStage);
+  uint64_t* empty = full + kStages;
+  uint64_t* acc_bar = empty + kStages;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(acc_bar + 1);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
   if (threadIdx.x == 0) {
-    for (int s = 0; s < kGramStages; ++s) {
+    for (int s = 0; s < kStages; ++s) {
       mbar_init(&full[s], 1);
       mbar_init(&empty[s], 1);
     }
@@ -168,8 +169,8 @@ __global__ void __launch_bounds__(kGramThreads)
   if (warp == 0) {
     if (lane == 0) {
       for (int kb = kb0; kb < kb1; ++kb) {
-        const int i = kb - kb0, s = i % kGramStages;
-        if (!mbar_wait(&empty[s], ((i / kGramStages) & 1) ^ 1, abort_flag, g.err, kErrWaitEmpty))
+        const int i = kb - kb0, s = i % kStages;
+        if (!mbar_wait(&empty[s], ((i / kStages) & 1) ^ 1, abort_flag, g.err, kErrWaitEmpty))
           break;
         mbar_arrive_expect_tx(&full[s], kStage);
         uint8_t* dst = smem + s * kStage;
@@ -188,8 +189,8 @@ __global__ void __launch_bounds__(kGramThreads)
       constexpr uint32_t idesc = make_idesc_16(HALF, 128, DP, COLS ? 1 : 0, COLS ? 1 : 0);
       bool ok = true;
       for (int kb = kb0; kb < kb1; ++kb) {
-        const int i = kb - kb0, s = i % kGramStages;
-        if (!mbar_wait(&full[s], (i / kGramStages) & 1, abort_flag, g.err, kErrWaitFull)) {
+        const int i = kb - kb0, s = i % kStages;
+        if (!mbar_wait(&full[s], (i / kStages) & 1, abort_flag, g.err, kErrWaitFull)) {
           ok = false;
           break;
         }
@@ -714,11 +715,16 @@ __global__ void __launch_bounds__(kIterThreads, DP == 64 ? 2 : 1) heads_iterate_
 // ------------------------------------------------------------------ apply
 template <int DP>
 struct ApplyCfg {
+  // CTAs an SM.  Two at 64, where one has half the rows to write and the loads in
+  // flight did not cover memory's latency (512 heads of 64 x 4096: 216 -> 193 µs,
+  // with the gram kernel's four); at 128 shared memory holds one.
+  static constexpr int kCtas = DP == 128 ? 1 : 2;
   static constexpr int kStage = DP * kApplyN * 2;
-  static constexpr int kQ = 2 * DP * DP * 2;          // both terms of one head
-  static constexpr int kStaging = 8 * 32 * 64 * 2 * 2;  // per epilogue warp: two 32 x 64 blocks
-  static constexpr int kSmem = kApplyStages * kStage + kQ + (DP == 64 ? DP * 128 : 0) + kStaging +
-                               1024 + 256;
+  static constexpr int kQ = 2 * DP * DP * 2;            // both terms of one head
+  static constexpr int kWriters = DP / 16;              // epilogue warps with output
+  static constexpr int kStaging = kWriters * 32 * 64 * 2 * 2;  // two 32 x 64 blocks each
+  // MMAs of M = 128 on DP = 64 read 8 KB past Q, which the staging covers
+  static constexpr int kSmem = kApplyStages * kStage + kQ + kStaging + 1024 + 256;
 };
 
 // Stores one staged 32 x 64 bf16 block (128-byte rows, 16-byte chunks XORed
@@ -741,7 +747,7 @@ __device__ __forceinline__ void store_block_plain(const uint8_t* blk, __nv_bfloa
 // (rows of the head x 128 columns).  Column heads: D = G·Q (128 rows x columns
 // of the head), Q being symmetric.
 template <int DP, bool COLS, bool HALF>
-__global__ void __launch_bounds__(kApplyThreads, 1)
+__global__ void __launch_bounds__(kApplyThreads, ApplyCfg<DP>::kCtas)
     heads_apply_kernel(const __grid_constant__ CUtensorMap tmG,
                        const __grid_constant__ CUtensorMap tmO, const HeadsArgs g) {
   using Cfg = ApplyCfg<DP>;
@@ -750,7 +756,7 @@ __global__ void __launch_bounds__(kApplyThreads, 1)
                                              ~static_cast<uintptr_t>(1023));
   uint8_t* sG = smem;
   uint8_t* sQ = smem + kApplyStages * Cfg::kStage;
-  uint8_t* staging = sQ + Cfg::kQ + (DP == 64 ? DP * 128 : 0);
+  uint8_t* staging = sQ + Cfg::kQ;
   uint64_t* full = reinterpret_cast<uint64_t*>(staging + Cfg::kStaging);
   uint64_t* empty = full + kApplyStages;
   uint64_t* q_full = empty + kApplyStages;
@@ -873,7 +879,9 @@ __global__ void __launch_bounds__(kApplyThreads, 1)
     const bool worker = COLS ? half * 64 < DP : q * 32 < DP;
     pdl_wait();
     if (worker || COLS) {
-      uint8_t* buf = staging + warp * (32 * 64 * 2 * 2);
+      // writers are numbered by lane quarter, then column half
+      const int writer = half * (COLS ? 4 : DP / 32) + q;
+      uint8_t* buf = staging + (worker ? writer : 0) * (32 * 64 * 2 * 2);
       int i = 0;
       for (long long u = u0; u < u1; ++u, ++i) {
         const int head = static_cast<int>(u / g.chunks), chunk = static_cast<int>(u % g.chunks);
@@ -889,21 +897,21 @@ __global__ void __launch_bounds__(kApplyThreads, 1)
         const bool any = worker && rows > 0 && cols > 0;
         uint8_t* blk = buf + (i & 1) * (32 * 64 * 2);
         if (any) {
-          float v[2][32];
-#pragma unroll
-          for (int c = 0; c < 2; ++c)
-            tmem_ld_32x32b_x32(
-                tmem + acc * 128 + half * 64 + c * 32 + (static_cast<uint32_t>(q * 32) << 16), v[c]);
           if (g.tma_out) {
             if (lane == 0) bulk_wait_read<1>();  // the block of two units ago has been read
             __syncwarp();
           }
 #pragma unroll
-          for (int c = 0; c < 8; ++c) {
-            float t[8];
+          for (int c = 0; c < 2; ++c) {
+            float v[32];
+            tmem_ld_32x32b_x32(
+                tmem + acc * 128 + half * 64 + c * 32 + (static_cast<uint32_t>(q * 32) << 16), v);
 #pragma unroll
-            for (int k = 0; k < 8; ++k) t[k] = v[c / 4][(c % 4) * 8 + k] * inv;
-            *reinterpret_cast<uint4*>(blk + lane * 128 + ((c ^ (lane & 7)) << 4)) = pack8_bf16(t);
+            for (int k = 0; k < 32; k += 2) mul2(v[k], v[k + 1], inv);
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+              *reinterpret_cast<uint4*>(blk + lane * 128 + (((4 * c + k) ^ (lane & 7)) << 4)) =
+                  pack8_bf16(v + 8 * k);
           }
         }
         tc_fence_before();
