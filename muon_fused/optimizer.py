@@ -441,6 +441,8 @@ class FusedMuon(Optimizer):
             if (p.is_cuda and dtype in STEP_DTYPES and g.dtype == dtype
                     and type(p) in _PLAIN and type(g) in _PLAIN and not g.is_sparse
                     and buf1.dtype == buf2.dtype and buf1.dtype in (dtype, torch.float32)
+                    and g.device == buf1.device == buf2.device == p.device
+                    and g.shape == buf1.shape == buf2.shape == p.shape
                     and p.is_contiguous() and g.is_contiguous() and buf1.is_contiguous()
                     and buf2.is_contiguous()):
                 alpha = alphas.get(step)

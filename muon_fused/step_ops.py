@@ -46,16 +46,38 @@ def _bump(tensors) -> None:
     increment_version([t for t in tensors if not t.is_inference()])
 
 
+def _check_adamw(params, grads, moments1, moments2) -> list[tuple]:
+    """Raise unless the kernel may work on the tensors; their types otherwise."""
+    _check_cuda(params[0], "params")
+    lists = (params, grads, moments1, moments2)
+    if len(set().union(*(map(torch.Tensor.get_device, ts) for ts in lists))) != 1:
+        raise RuntimeError("fused_adamw needs all tensors on one device")
+    if not all(all(map(torch.Tensor.is_contiguous, ts)) for ts in lists):
+        raise RuntimeError("fused_adamw needs contiguous tensors")
+    if any(any(map(torch.Tensor.is_neg, ts)) for ts in lists):
+        raise RuntimeError("fused_adamw needs tensors that are not negative views")
+    if not all(all(map(torch.Tensor.is_same_size, params, ts)) for ts in lists[1:]):
+        raise RuntimeError("params, grads and moments must have the same shapes")
+    types = list(zip(*(map(_DTYPE, ts) for ts in lists)))
+    for pt, gt, mt, vt in set(types):
+        if pt not in STEP_DTYPES or gt != pt:
+            raise RuntimeError(f"params and grads must be fp32, bf16 or fp16 of one type, got "
+                               f"{pt} and {gt}")
+        if mt != vt or mt not in (pt, torch.float32):
+            raise RuntimeError(f"moments must have the parameter's type or fp32, got {mt} and {vt}")
+    return types
+
+
 def adamw_launch(params, grads, moments1, moments2, alphas, lr: float, wd: float, betas,
                  eps: float) -> None:
-    """The call after the checks: tensors of one device, one parameter type and
-    one moment type, all contiguous; ``alphas`` holds each tensor's -lr/scale.
-    Version counters stay as they are."""
+    """One call: lists of one parameter type and one moment type; ``alphas``
+    holds each tensor's -lr/scale.  Version counters stay as they are."""
     rc = _lib.step_ext().adamw(params, grads, moments1, moments2, alphas, float(1 - lr * wd),
                                1 - betas[0], 1 - betas[1], float(eps), False)
     if rc is not None:
         _lib.check(rc, "fm_adamw")
         return
+    _check_adamw(params, grads, moments1, moments2)
     ptr = torch.Tensor.data_ptr
     table = b"".join(map(_lib.ADAMW_TENSOR.pack, map(ptr, params), map(ptr, grads),
                          map(ptr, moments1), map(ptr, moments2),
@@ -128,23 +150,9 @@ def fused_adamw(
         raise RuntimeError(f"steps must be an int or one per parameter, got {len(alphas)} for {n}")
     if n == 0:
         return
-    _check_cuda(params[0], "params")
     lists = (params, grads, moments1, moments2)
-    if len(set().union(*(map(torch.Tensor.get_device, ts) for ts in lists))) != 1:
-        raise RuntimeError("fused_adamw needs all tensors on one device")
-    if not all(all(map(torch.Tensor.is_contiguous, ts)) for ts in lists):
-        raise RuntimeError("fused_adamw needs contiguous tensors")
-    if not all(all(map(torch.Tensor.is_same_size, params, ts)) for ts in lists[1:]):
-        raise RuntimeError("params, grads and moments must have the same shapes")
-    types = list(zip(*(map(_DTYPE, ts) for ts in lists)))
-    kinds = set(types)
-    for pt, gt, mt, vt in kinds:
-        if pt not in STEP_DTYPES or gt != pt:
-            raise RuntimeError(f"params and grads must be fp32, bf16 or fp16 of one type, got "
-                               f"{pt} and {gt}")
-        if mt != vt or mt not in (pt, torch.float32):
-            raise RuntimeError(f"moments must have the parameter's type or fp32, got {mt} and {vt}")
-    if len(kinds) == 1:
+    types = _check_adamw(*lists)
+    if len(set(types)) == 1:
         adamw_launch(*lists, alphas, lr, wd, betas, eps)
     else:
         for kind in dict.fromkeys(types):

@@ -231,3 +231,33 @@ def test_mixed_types_of_one_shape_in_a_normed_group(cuda_lib):
         rms = float(d.square().mean().sqrt())
         assert abs(rms - 0.2 * LR) <= 0.02 * 0.2 * LR
         assert opt.state[p]["row_moment"].shape == (p.shape[0],)
+
+
+@pytest.mark.parametrize("what", ["device", "shape"])
+def test_adamw_state_that_no_longer_fits_is_refused(cuda_lib, what):
+    """A moment left on the CPU, or of the size that the parameter had before."""
+    from muon_fused import FusedMuon
+
+    p = torch.nn.Parameter(_rand((64, 16), 1, 0.02))
+    q = torch.nn.Parameter(_rand((33,), 2, 0.02))
+    opt = FusedMuon([{"params": [p, q]}])
+    for x in (p, q):
+        x.grad = _rand(x.shape, 3, 1e-3)
+    opt.step()
+    state = opt.state[p]
+    if what == "device":
+        state["moment2"] = state["moment2"].cpu()
+    else:
+        state["moment1"] = state["moment1"][:32].clone()
+    with pytest.raises(RuntimeError):
+        opt.step()
+
+
+def test_adamw_launch_checks_what_it_cannot_take(cuda_lib):
+    from muon_fused.step_ops import adamw_launch
+
+    p, g, m, v = (_rand((64,), i, 1.0) for i in range(4))
+    for bad in ([p], [g], [m], [v.cpu()]), ([p], [g], [m], [v[:32]]), ([p], [g[::2]], [m], [v]):
+        with pytest.raises(RuntimeError):
+            adamw_launch(*bad, [-0.1], 0.1, 0.0, (0.9, 0.95), 1e-8)
+    assert torch.equal(p, _rand((64,), 0, 1.0))
