@@ -181,6 +181,8 @@ def newton_schulz_heads(G: torch.Tensor, heads: int, steps: int = 5, dim: int = 
                 G.data_ptr(), _DTYPE_CODE[G.dtype], batch, rows, cols, ld, bs, int(heads), int(dim),
                 out.data_ptr(), int(steps), workspace.data_ptr(), workspace.nbytes, _stream(G)),
             "fm_newton_schulz_heads")
+    if not out.is_inference():
+        torch.autograd.graph.increment_version(out)
     return out
 
 

@@ -239,6 +239,7 @@ PyObject* heads(PyObject*, PyObject* args) {
                            out.data_ptr(), steps, ws.data_ptr(), ws.nbytes(), current_stream(g));
     if (rc != FM_OK) return PyLong_FromLong(rc);
     if (oo != Py_None) {
+      if (!out.is_inference()) out.unsafeGetTensorImpl()->bump_version();
       Py_INCREF(oo);
       return oo;
     }

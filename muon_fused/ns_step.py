@@ -117,6 +117,8 @@ def fused_newton_schulz_heads(
     d = _check_heads(G.shape, heads, dim)
     if _heads_gram_form(d, steps):
         return _C.newton_schulz_heads(G, heads, steps, dim, workspace, out)
+    if G.numel() == 0:
+        return torch.empty(G.shape, dtype=torch.bfloat16, device=G.device) if out is None else out
     blocks = G.unflatten(G.ndim - 2 + dim, (heads, d))
     if dim == 1:
         blocks = blocks.movedim(-2, -3)  # heads before rows

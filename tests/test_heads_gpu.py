@@ -301,3 +301,23 @@ def test_graph_replay(cuda_lib, dim):
         graph.replay()
         torch.cuda.synchronize()
         assert torch.equal(out, fused_newton_schulz_heads(G.clone(), 4, dim=dim))
+
+
+def test_out_bumps_its_version(cuda_lib):
+    """A backward pass through values that the call overwrote fails."""
+    from muon_fused import fused_newton_schulz_heads
+
+    G = torch.randn(128, 64, device="cuda", dtype=torch.bfloat16)
+    for A in (G, G.t().contiguous().t()):  # taken as it is, copied first
+        out = torch.empty(128, 64, device="cuda", dtype=torch.bfloat16)
+        before = out._version
+        fused_newton_schulz_heads(A, 2, out=out)
+        assert out._version > before
+
+
+@pytest.mark.parametrize("shape", [(0, 512, 64), (512, 0), (2, 512, 0)])
+def test_empty_wide_heads(cuda_lib, shape):
+    from muon_fused import fused_newton_schulz_heads
+
+    G = torch.empty(shape, device="cuda", dtype=torch.bfloat16)
+    assert fused_newton_schulz_heads(G, 2).shape == G.shape
