@@ -315,12 +315,12 @@ class FusedMuon(Optimizer):
 
     def _normed_scratch(self, device: torch.device, count: int, rows: int) -> torch.Tensor:
         """Workspace of the normalised update, apart from the batch's arena (the
-        updates that it reads live there)."""
-        need = normed_workspace_size(count, rows)
-        key = (device, "normed")
+        updates that it reads live there).  One per size, kept: a captured step
+        goes on using the ones that it was captured with."""
+        key = (device, "normed", count, rows)
         buf = self._workspaces.get(key)
-        if buf is None or buf.numel() < need:
-            buf = torch.empty(need, dtype=torch.uint8, device=device)
+        if buf is None:
+            buf = torch.empty(normed_workspace_size(count, rows), dtype=torch.uint8, device=device)
             self._workspaces[key] = buf
         return buf
 
