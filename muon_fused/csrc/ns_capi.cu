@@ -1083,6 +1083,7 @@ int normed_launch(const fm_normed_matrix* mats, int64_t count,
     a.rinv = ws + i * rows;
     a.partials = ws + count * rows + i * blocks;
     a.row_blocks = int(blocks);
+    a.first = i == 0;
     a.decay = decay;
     a.step = step;
     a.beta2 = beta2;
