@@ -321,3 +321,43 @@ def test_empty_wide_heads(cuda_lib, shape):
 
     G = torch.empty(shape, device="cuda", dtype=torch.bfloat16)
     assert fused_newton_schulz_heads(G, 2).shape == G.shape
+
+
+@pytest.mark.parametrize("steps", [1, 2, 3, 4, 5, 6])
+@pytest.mark.parametrize("heads,d,n", [(149, 128, 200), (300, 65, 131)])
+def test_more_heads_than_sms(cuda_lib, heads, d, n, steps):
+    """Two and three rounds of heads on the GPU; runs repeat."""
+    from muon_fused import fused_newton_schulz_heads
+
+    for dim, dtype in ((0, torch.bfloat16), (1, torch.float16)):
+        G = rand((heads * d, n) if dim == 0 else (n, heads * d), steps, dtype)
+        out = fused_newton_schulz_heads(G, heads, steps, dim=dim)
+        check(out, G, heads, steps, dim)
+        assert torch.equal(out, fused_newton_schulz_heads(G, heads, steps, dim=dim))
+
+
+@pytest.mark.parametrize("dim", [0, 1])
+@pytest.mark.parametrize("steps", [2, 5])
+def test_ill_conditioned_heads_among_many(cuda_lib, dim, steps):
+    """Condition 1 to 1e5, rank 8 and a zero head among 160; NaN stays in its head."""
+    from muon_fused import fused_newton_schulz_heads
+
+    heads, d, n = 160, 128, 256
+    gen = torch.Generator().manual_seed(11)
+    u = torch.linalg.qr(torch.randn(heads, d, d, generator=gen))[0]
+    v = torch.linalg.qr(torch.randn(heads, n, d, generator=gen))[0]
+    s = torch.stack([torch.logspace(0, -5.0 * h / heads, d) for h in range(heads)])
+    s[7, 8:] = 0
+    s[9] = 0
+    blocks = (u * s[:, None]) @ v.mT
+    G = blocks.reshape(heads * d, n).bfloat16().to(DEV)
+    G = G if dim == 0 else G.T.contiguous()
+    out = fused_newton_schulz_heads(G, heads, steps, dim=dim)
+    check(out, G, heads, steps, dim)
+    assert not bool(out.narrow(dim, 9 * d, d).any())
+    G2 = G.clone()
+    G2.narrow(dim, 150 * d, d)[3, 5] = math.nan
+    out2 = fused_newton_schulz_heads(G2, heads, steps, dim=dim)
+    assert bool(out2.narrow(dim, 150 * d, d).isnan().all())
+    assert torch.equal(out2.narrow(dim, 0, 150 * d), out.narrow(dim, 0, 150 * d))
+    assert torch.equal(out2.narrow(dim, 151 * d, 9 * d), out.narrow(dim, 151 * d, 9 * d))
