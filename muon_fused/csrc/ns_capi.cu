@@ -879,23 +879,25 @@ int heads_check(long long batch, long long rows, long long cols, long long heads
 // Spans are added as (first byte, bytes, written); `overlap` sorts them.
 struct SpanCheck {
   struct Span {
-    uintptr_t lo, hi;
-    bool written;
+    uint64_t key;  // 2 · first byte + written, to sort by one word
+    uint64_t hi;
   };
   std::vector<Span> spans;
   void add(const void* p, long long bytes, bool written) {
-    const uintptr_t lo = reinterpret_cast<uintptr_t>(p);
-    if (bytes > 0) spans.push_back({lo, lo + uintptr_t(bytes), written});
+    const uint64_t lo = reinterpret_cast<uintptr_t>(p);
+    if (bytes > 0) spans.push_back({lo * 2 + (written ? 1 : 0), lo + uint64_t(bytes)});
   }
   bool overlap() {
-    auto less = [](const Span& a, const Span& b) { return a.lo < b.lo; };
+    auto less = [](const Span& a, const Span& b) { return a.key < b.key; };
     if (!std::is_sorted(spans.begin(), spans.end(), less))
       std::sort(spans.begin(), spans.end(), less);
-    uintptr_t end = 0, written_end = 0;  // furthest end so far, of all and of the written ones
+    uint64_t end = 0, written_end = 0;  // furthest end so far, of all and of the written ones
     for (const Span& s : spans) {
-      if (s.lo < written_end || (s.written && s.lo < end)) return true;
+      const uint64_t lo = s.key / 2;
+      const bool written = s.key & 1;
+      if (lo < written_end || (written && lo < end)) return true;
       end = std::max(end, s.hi);
-      if (s.written) written_end = std::max(written_end, s.hi);
+      if (written) written_end = std::max(written_end, s.hi);
     }
     return false;
   }

@@ -1,8 +1,9 @@
 // CPython side of the step operators (fused_adamw, fused_normed_update,
 // fused_newton_schulz_heads): reads the tensors' pointers and sizes in C++ and
 // makes the C-ABI call.  A list of small tensors is bound by this and not by the
-// kernel: 20 vectors took 45 µs through Python's attribute calls and ctypes (10
-// here), the kernel 4.
+// kernel: 20 vectors took 45 µs through Python's attribute calls and ctypes (7
+// here), the kernel 4.  The tensors are not copied: their reference counts alone
+// cost 3 µs.
 //
 // Only the plain case is handled here: ordinary CUDA tensors, the lists contiguous
 // and of one device and type, that agree in their shapes.  For anything else a
@@ -59,20 +60,20 @@ class TensorList {
       if (!t.defined() || !t.is_cuda() || t.layout() != at::kStrided || t.is_inference() ||
           !t.is_contiguous() || t.is_neg() || t.is_conj())
         return;
-      if (i > 0 && (t.scalar_type() != t_[0].scalar_type() || t.device() != t_[0].device())) return;
-      t_.push_back(t);
+      if (i > 0 && (t.scalar_type() != t_[0]->scalar_type() || t.device() != t_[0]->device())) return;
+      t_.push_back(&t);
     }
     ok_ = true;
   }
   bool ok() const { return ok_; }
   size_t size() const { return t_.size(); }
-  const at::Tensor& operator[](size_t i) const { return t_[i]; }
+  const at::Tensor& operator[](size_t i) const { return *t_[i]; }
   void bump() const {
-    for (const at::Tensor& t : t_) t.unsafeGetTensorImpl()->bump_version();
+    for (const at::Tensor* t : t_) t->unsafeGetTensorImpl()->bump_version();
   }
 
  private:
-  std::vector<at::Tensor> t_;
+  std::vector<const at::Tensor*> t_;  // the Python objects hold them throughout the call
   bool ok_ = false;
 };
 

@@ -125,7 +125,7 @@ def fused_adamw(
     """
     if not all(0.0 <= b < 1.0 for b in betas):
         raise RuntimeError(f"betas must be in [0, 1), got {betas}")
-    if isinstance(steps, Sequence):
+    if type(steps) is not int and isinstance(steps, Sequence):
         if any(t < 1 for t in steps):
             raise RuntimeError("steps must be >= 1")
         alphas = [adamw_alpha(lr, betas, int(t)) for t in steps]
