@@ -852,9 +852,16 @@ int heads_pack(const DeviceState& ds, const HeadsPlan& P, const void* G, long lo
   const long long want = (outer * (P.pack_ld / 8) + kPackThreads - 1) / kPackThreads;
   const long long cap = std::max<long long>(1, ds.sm_count * 16ll / P.total);
   const dim3 grid{unsigned(std::min(want, cap)), unsigned(P.total), 1};
-  FM_CUDA(launch_pdl(heads_pack_kernel<S, T>, grid, dim3(kPackThreads), 0, st, false,
-                     static_cast<const S*>(G), ldg, bs_g, int(heads), head_stride, outer, inner,
-                     static_cast<T*>(dst), int(P.pack_ld)));
+  auto kernel = heads_pack_kernel<S, T, false>;
+  if constexpr (sizeof(S) > 2) {
+    const long long v = 16 / sizeof(S);  // elements of a 16-byte load
+    if ((reinterpret_cast<uintptr_t>(G) & 15) == 0 && ldg % v == 0 && bs_g % v == 0 &&
+        head_stride % v == 0 && inner % 8 == 0)
+      kernel = heads_pack_kernel<S, T, true>;
+  }
+  FM_CUDA(launch_pdl(kernel, grid, dim3(kPackThreads), 0, st, false, static_cast<const S*>(G), ldg,
+                     bs_g, int(heads), head_stride, outer, inner, static_cast<T*>(dst),
+                     int(P.pack_ld)));
   return FM_OK;
 }
 
