@@ -23,9 +23,11 @@
 // products hi·hi + hi·lo + lo·hi in one fp32 accumulator; A is held scaled by
 // DP so that its average diagonal is 1 and lo stays clear of fp16's subnormals.
 // Q enters the last product as two terms of G's type.  The result is then within
-// its bf16 rounding of the exact one for Gaussian, ill-conditioned (1e5) and
-// rank-deficient heads.  fp16's range bounds Q, at most a^steps = 3.4445^steps:
-// steps <= 8.
+// its bf16 rounding of the exact one for Gaussian and ill-conditioned (1e5) heads.
+// What leaks into directions that a head does not span still grows by a² a step in A
+// and from there by a in Q: with rank 8, 4, 2, 1 of 128 the error after 5 steps is
+// 0.2, 0.25, 0.4, 0.7 %, after 6 already twice that and after 8 anything, so
+// steps <= 5 (a third term of Q in the last product changed none of these).
 //
 // d is padded to DP = 64 or 128 by TMA's zero fill; padded rows and columns of A
 // stay zero and change nothing.  tcgen05.mma always runs M = 128 here: with DP =
@@ -69,7 +71,7 @@ __host__ __device__ constexpr uint32_t make_idesc_16(bool half, int M, int N, in
 }
 
 constexpr int kHeadsMaxDim = 128;
-constexpr int kHeadsMaxSteps = 8;
+constexpr int kHeadsMaxSteps = 5;
 constexpr int kHeadsK = 64;        // reduction columns per gram stage (one swizzle row)
 constexpr int kGramMaxSplit = 8;   // portable cluster size
 constexpr int kGramThreads = 192;  // producer, MMA, 4 epilogue warps

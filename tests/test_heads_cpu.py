@@ -24,7 +24,8 @@ def test_workspace_holds_the_copy_and_the_matrices(shape, heads, dim):
     batch = shape[0] if len(shape) == 3 else 1
     rows, cols = shape[-2:]
     need = workspace_size_heads(shape, heads, dim=dim)
-    dp = 64 if (rows, cols)[dim] // heads <= 64 else 128
+    side = min((rows, cols)[dim] // heads, (rows, cols)[1 - dim])  # the matrices' side
+    dp = 64 if side <= 64 else 128
     assert need >= batch * heads * dp * dp * (4 + 4) + 2 * batch * rows * cols
     assert need % 256 == 0
 

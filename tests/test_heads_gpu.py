@@ -32,7 +32,7 @@ def ref64(G, heads, steps, dim):
     return torch.cat(x.unbind(1), 1 + dim).reshape(G.shape)
 
 
-def check(out, G, heads, steps, dim, fro=FRO):
+def check(out, G, heads, steps, dim, fro=FRO, elem=4e-3):
     assert out.dtype == torch.bfloat16 and out.shape == G.shape
     ref = ref64(G, heads, steps, dim)
     diff = out.double() - ref
@@ -41,7 +41,7 @@ def check(out, G, heads, steps, dim, fro=FRO):
     rel = blocks.flatten(2).norm(dim=2) / rblocks.flatten(2).norm(dim=2).clamp_min(1e-30)
     assert float(rel.max()) <= fro, (float(rel.max()), int(rel.argmax()))
     big = float(ref.abs().max())
-    assert bool((diff.abs() <= 2.0 ** -8 * ref.abs() + 4e-3 * big).all()), float(diff.abs().max()) / big
+    assert bool((diff.abs() <= 2.0 ** -8 * ref.abs() + elem * big).all()), float(diff.abs().max()) / big
 
 
 def rand(shape, seed, dtype=torch.bfloat16):
@@ -84,7 +84,7 @@ def test_wide_types_are_rounded_to_bf16_first(cuda_lib, dtype, dim):
     assert torch.equal(out, fused_newton_schulz_heads(G.bfloat16(), 2, dim=dim))
 
 
-@pytest.mark.parametrize("steps", [0, 1, 2, 3, 8])
+@pytest.mark.parametrize("steps", [0, 1, 2, 3, 4])
 @pytest.mark.parametrize("d", [48, 128])
 def test_steps(cuda_lib, steps, d):
     from muon_fused import fused_newton_schulz_heads
@@ -323,7 +323,7 @@ def test_empty_wide_heads(cuda_lib, shape):
     assert fused_newton_schulz_heads(G, 2).shape == G.shape
 
 
-@pytest.mark.parametrize("steps", [1, 2, 3, 4, 5, 6])
+@pytest.mark.parametrize("steps", [1, 2, 3, 4, 5])
 @pytest.mark.parametrize("heads,d,n", [(149, 128, 200), (300, 65, 131)])
 def test_more_heads_than_sms(cuda_lib, heads, d, n, steps):
     """Two and three rounds of heads on the GPU; runs repeat."""
@@ -361,3 +361,75 @@ def test_ill_conditioned_heads_among_many(cuda_lib, dim, steps):
     assert bool(out2.narrow(dim, 150 * d, d).isnan().all())
     assert torch.equal(out2.narrow(dim, 0, 150 * d), out.narrow(dim, 0, 150 * d))
     assert torch.equal(out2.narrow(dim, 151 * d, 9 * d), out.narrow(dim, 151 * d, 9 * d))
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float64])
+@pytest.mark.parametrize("dim", [0, 1])
+def test_views_of_wide_types(cuda_lib, dtype, dim):
+    """Rows on and off 16-byte boundaries, whole and broken chunks of eight."""
+    from muon_fused import fused_newton_schulz_heads
+
+    base = rand((3, 300, 404), 12, torch.float32).to(dtype)
+    for v in (base[:, :256, :384], base[:, 1:257, 4:388], base[:, :256, 1:385], base[::2, :252, :324],
+              base[1, :256, :384], base[0, :1, :400]):
+        heads = 4 if dim == 1 or v.shape[-2] > 1 else 1
+        out = fused_newton_schulz_heads(v, heads, dim=dim)
+        assert torch.equal(out, fused_newton_schulz_heads(v.bfloat16().contiguous(), heads, dim=dim))
+        check(out, v.bfloat16(), heads, 5, dim)
+
+
+@pytest.mark.parametrize("steps", [6, 8])
+@pytest.mark.parametrize("dim", [0, 1])
+def test_more_steps_run_as_a_batch(cuda_lib, steps, dim):
+    """The Gram form would blow up what a head does not span."""
+    from muon_fused import fused_newton_schulz, fused_newton_schulz_heads
+
+    G = rand((256, 320) if dim == 0 else (320, 256), 16)
+    out = fused_newton_schulz_heads(G, 4, steps, dim=dim)
+    for b, o in zip(G.chunk(4, dim), out.chunk(4, dim)):
+        ref = ref64(b, 1, steps, dim)
+        # two bf16 iterations that differ in nothing but their batch: 2e-2 between them
+        assert float((o.double() - ref).norm() / ref.norm()) <= 2e-2
+        assert float((o.double() - fused_newton_schulz(b.contiguous(), steps).double()).norm()
+                     / ref.norm()) <= 2e-2
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("dim", [0, 1])
+@pytest.mark.parametrize("d,n", [(128, 1), (128, 2), (100, 9), (64, 63), (128, 127), (17, 16)])
+def test_heads_wider_than_long(cuda_lib, d, n, dim, dtype):
+    """The long side is the shorter one: full rank there, so exact up to the rounding."""
+    from muon_fused import fused_newton_schulz_heads, workspace_size_heads
+
+    for batch in (None, 3):
+        shape = (5 * d, n) if dim == 0 else (n, 5 * d)
+        G = rand(shape if batch is None else (batch, *shape), d + n, dtype)
+        out = fused_newton_schulz_heads(G, 5, dim=dim)
+        check(out, G, 5, 5, dim)
+        buf = torch.empty_like(out)
+        ws = torch.empty(workspace_size_heads(G.shape, 5, dim=dim), dtype=torch.uint8, device=DEV)
+        assert fused_newton_schulz_heads(G, 5, workspace=ws, dim=dim, out=buf) is buf
+        assert torch.equal(buf, out)
+        with pytest.raises(RuntimeError, match="out must be"):
+            fused_newton_schulz_heads(G, 5, dim=dim, out=buf.float())
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("dim", [0, 1])
+@pytest.mark.parametrize("rank", [1, 2, 4, 8])
+def test_low_rank_heads(cuda_lib, rank, dim, dtype):
+    """What a head does not span carries rounding of 2^-22 a product from A into Q, there
+    times 3.4445 for every step that follows: at most five steps' worth of 3.4445^5 · 2^-22
+    · sqrt(d) against singular values that end at 0.7 or above, beside the output's 2^-8
+    (and as much of the largest value in an element, whose row of Q has d such roundings)."""
+    from muon_fused import fused_newton_schulz_heads
+
+    heads, d, n = 4, 128, 512
+    gen = torch.Generator().manual_seed(rank)
+    u = torch.randint(-3, 4, (heads * d, rank), generator=gen).double()  # exact in 16 bits
+    v = torch.randint(-3, 4, (rank, n), generator=gen).double()
+    G = (u @ v).to(dtype).to(DEV)
+    assert torch.equal(G.double().cpu(), u @ v)
+    G = G if dim == 0 else G.T.contiguous()
+    leak = 5 * A ** 5 * 2.0 ** -22 * d ** 0.5 / 0.7
+    check(fused_newton_schulz_heads(G, heads, dim=dim), G, heads, 5, dim, 2.0 ** -8 + leak, leak)
