@@ -894,6 +894,10 @@ __global__ void __launch_bounds__(kApplyThreads, ApplyCfg<DP>::kCtas)
       const int writer = half * (COLS ? 4 : DP / 32) + q;
       uint8_t* buf = staging + (worker ? writer : 0) * (32 * 64 * 2 * 2);
       int i = 0;
+      // Blocks that this warp wrote.  The two buffers alternate by it and not by the unit:
+      // a warp whose block lies past the matrix's end skips a unit, and the store of the
+      // unit before is then the newest one, which the wait below lets go on reading.
+      int written = 0;
       for (long long u = u0; u < u1; ++u, ++i) {
         const int head = static_cast<int>(u / g.chunks), chunk = static_cast<int>(u % g.chunks);
         const int h = head % g.heads, mat = head / g.heads;
@@ -906,10 +910,11 @@ __global__ void __launch_bounds__(kApplyThreads, ApplyCfg<DP>::kCtas)
         if (!mbar_wait(&accf[acc], (i >> 1) & 1, abort_flag, g.err, kErrWaitAccFull)) break;
         tc_fence_after();
         const bool any = worker && rows > 0 && cols > 0;
-        uint8_t* blk = buf + (i & 1) * (32 * 64 * 2);
+        uint8_t* blk = buf + (written & 1) * (32 * 64 * 2);
         if (any) {
+          ++written;
           if (g.tma_out) {
-            if (lane == 0) bulk_wait_read<1>();  // the block of two units ago has been read
+            if (lane == 0) bulk_wait_read<1>();  // the block written before the last has been read
             __syncwarp();
           }
 #pragma unroll

@@ -433,3 +433,19 @@ def test_low_rank_heads(cuda_lib, rank, dim, dtype):
     G = G if dim == 0 else G.T.contiguous()
     leak = 5 * A ** 5 * 2.0 ** -22 * d ** 0.5 / 0.7
     check(fused_newton_schulz_heads(G, heads, dim=dim), G, heads, 5, dim, 2.0 ** -8 + leak, leak)
+
+
+@pytest.mark.parametrize("dim", [0, 1])
+@pytest.mark.parametrize("heads,d,n", [(300, 128, 192), (160, 128, 2880), (310, 64, 1048), (600, 64, 176)])
+def test_blocks_past_the_end_among_many_heads(cuda_lib, heads, d, n, dim):
+    """The last 128 elements of the long side are half or a quarter there, so that some
+    warps skip their block of that unit, and every CTA of the output product goes on to the
+    next head: the staged blocks of the skipping warps must not be overwritten while a store
+    still reads them.  Runs repeat bit for bit."""
+    from muon_fused import fused_newton_schulz_heads
+
+    G = rand((heads * d, n) if dim == 0 else (n, heads * d), n)
+    out = fused_newton_schulz_heads(G, heads, dim=dim)
+    check(out, G, heads, 5, dim)
+    for _ in range(20):
+        assert torch.equal(out, fused_newton_schulz_heads(G, heads, dim=dim))
