@@ -322,8 +322,8 @@ __device__ __forceinline__ bool stash_partial(const GemmArgs& g, uint32_t tmem_a
 // Stores: with g.tma_out, each 32 x 32 chunk is staged in the warp's shared
 // buffers `sbuf` (8 KB: two parities x {row-major, transposed}) and written
 // by TMA tile stores through `tm_out` at matrix index `bz`; lane 0 issues
-// them and keeps at most one older chunk's stores in flight, so the warp
-// moves on while the copies drain.  Otherwise every lane stores its own row
+// them and keeps at most one older chunk's stores of the same tile in flight, so
+// the warp moves on while the copies drain.  Otherwise every lane stores its own row
 // (unaligned outputs).  The caller waits for outstanding stores
 // (bulk_wait_all) before the results are consumed or the CTA exits.
 template <int MODE, bool FROM_PARTIALS = false, int TBN = kBN>
@@ -396,7 +396,12 @@ __device__ __forceinline__ bool epilogue_tile(const GemmArgs& g, uint32_t tmem_a
     if (use_tma) {
       __nv_bfloat16* bd = sbuf + (c & 1) * 2 * kEpiBlock;
       __nv_bfloat16* bt = bd + kEpiBlock;
-      if (lane == 0) bulk_wait_read<1>();  // chunk c-2's stores have read this parity
+      if (lane == 0) {
+        // this parity's stores have read it: chunk c-2's, or, for the tile's first
+        // chunk, the last ones of the tile before (an odd number of chunks ends on
+        // this parity too)
+        if (c == 0) bulk_wait_read<0>(); else bulk_wait_read<1>();
+      }
       __syncwarp();
       bool st_rows = true, st_cols = false;
       if constexpr (MODE != kBX) {

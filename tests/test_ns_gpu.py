@@ -275,3 +275,22 @@ def test_single_cta_and_pair_kernels_bit_identical(cuda_lib, m, n):
     torch.cuda.synchronize()
     for a, b, name in zip(res[1], res[2], ("A", "Boff", "diag", "X_new")):
         assert torch.equal(a, b), name
+
+
+@pytest.mark.parametrize("path", [1, 2])
+@pytest.mark.parametrize("m,n", [(2080, 4128), (4096, 4096)])
+def test_staged_tiles_repeat(cuda_lib, path, m, n):
+    """Tiles with an odd number of 32-column chunks (the diagonal ones, and the last of 2080
+    or 4128 columns) before others of the same CTA: a staged chunk must not be overwritten
+    while its store still reads it.  Runs repeat bit for bit and stay at the path's accuracy."""
+    from muon_fused import _lib, fused_newton_schulz
+
+    G = _seeded(m, n, 77).cuda()
+    try:
+        _lib.set_gemm_path(path)
+        out = fused_newton_schulz(G)
+        for _ in range(10):
+            assert torch.equal(out, fused_newton_schulz(G))
+    finally:
+        _lib.set_gemm_path(0)
+    assert O.rel_fro(out.float().cpu(), _fp32_gpu(G).cpu()) <= 1e-2
