@@ -220,7 +220,8 @@ int fm_adamw(const fm_adamw_tensor* tensors, int64_t count, int dtype, int momen
  *   s_i = mean_j u_ij^2;  v_i = beta2 v_i + (1 - beta2) s_i
  *   r_i = 1 / (sqrt(v_i) + eps);  F = |diag(r) u|_F
  *   p_ij = p_ij * decay - step / (F + 1e-7) * r_i * u_ij
- * with decay = 1 - lr*wd and step = lr * 0.2 * sqrt(rows * cols).  param has
+ * with decay = 1 - lr*wd and step = lr * 0.2 * sqrt(rows * cols); beta2 is a
+ * double, so that 1 - beta2 is rounded to fp32 once.  param has
  * type dtype (FM_DT_F32 / BF16 / F16) and, like update, rows x cols contiguous
  * elements; row_moment holds rows floats.  workspace: at least
  * fm_normed_workspace_size() bytes, 256-byte aligned.  The list is read during
@@ -234,7 +235,7 @@ typedef struct {
 } fm_normed_matrix;
 int fm_normed_workspace_size(int64_t count, int64_t rows, uint64_t* bytes);
 int fm_muon_apply_normed(const fm_normed_matrix* mats, int64_t count, int64_t rows, int64_t cols,
-                         int dtype, float decay, float step, float beta2, float eps,
+                         int dtype, float decay, float step, double beta2, float eps,
                          void* workspace, uint64_t workspace_bytes, void* stream);
 
 /*

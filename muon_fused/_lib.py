@@ -46,7 +46,7 @@ SIGNATURES = {
                           ctypes.c_float, ctypes.c_float, _vp]),
     "fm_normed_workspace_size": (_c_int, [_i64, _i64, ctypes.POINTER(_u64)]),
     "fm_muon_apply_normed": (_c_int, [_vp, _i64, _i64, _i64, _c_int, ctypes.c_float,
-                                      ctypes.c_float, ctypes.c_float, ctypes.c_float, _vp, _u64,
+                                      ctypes.c_float, ctypes.c_double, ctypes.c_float, _vp, _u64,
                                       _vp]),
     "fm_set_gemm_path": (_c_int, [_c_int]),
     "fm_stage_timing": (_c_int, [_c_int]),

@@ -51,7 +51,7 @@ struct NormedArgs {
   float* partials;  // row_blocks per matrix
   int row_blocks;
   int first;        // the call's first row pass
-  float decay, step, beta2, eps;  // step = lr·0.2·sqrt(rows·cols)
+  float decay, step, beta2, w2, eps;  // step = lr·0.2·sqrt(rows·cols), w2 = 1 - beta2
 };
 
 __device__ __forceinline__ float bf16x8_sumsq(uint4 u, float acc) {
@@ -107,7 +107,9 @@ __device__ __forceinline__ float row_sumsq(const __nv_bfloat16* row, long long c
 // v, r and the share of F² of one row whose Σ u² is s (one thread).
 __device__ __forceinline__ float normed_row(const NormedArgs& a, float* v, float* rinv, float v_old,
                                             float s) {
-  const float x = fmaf(a.beta2, v_old, (1.f - a.beta2) * (s / static_cast<float>(a.cols)));
+  // w2 comes from the host, rounded once: 1 - beta2 of a beta2 already rounded to fp32 is
+  // off by 1.3e-5 at 0.999 and 1.7e-4 at 0.9999
+  const float x = fmaf(a.beta2, v_old, a.w2 * (s / static_cast<float>(a.cols)));
   *v = x;
   const float ri = 1.f / (sqrtf(x) + a.eps);
   *rinv = ri;

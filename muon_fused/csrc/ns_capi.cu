@@ -1064,7 +1064,7 @@ int adamw_any(const fm_adamw_tensor* ts, int64_t count, float decay, float w1, f
 
 template <typename T>
 int normed_launch(const fm_normed_matrix* mats, int64_t count,
-                  long long rows, long long cols, float decay, float step, float beta2, float eps,
+                  long long rows, long long cols, float decay, float step, double beta2, float eps,
                   float* ws, cudaStream_t st) {
   // Matrices per pair of launches: few enough that their updates stay in L2
   // between the row pass and the apply pass.
@@ -1095,7 +1095,8 @@ int normed_launch(const fm_normed_matrix* mats, int64_t count,
     a.first = i == 0;
     a.decay = decay;
     a.step = step;
-    a.beta2 = beta2;
+    a.beta2 = float(beta2);
+    a.w2 = float(1.0 - beta2);
     a.eps = eps;
     const dim3 g1(unsigned(a.row_blocks), unsigned(k));
     const dim3 g2{unsigned(chunks), unsigned(k), 1};
@@ -1362,7 +1363,7 @@ int fm_normed_workspace_size(int64_t count, int64_t rows, uint64_t* bytes) {
 }
 
 int fm_muon_apply_normed(const fm_normed_matrix* mats, int64_t count, int64_t rows, int64_t cols,
-                         int dtype, float decay, float step, float beta2, float eps,
+                         int dtype, float decay, float step, double beta2, float eps,
                          void* workspace, uint64_t workspace_bytes, void* stream) {
   if (count < 0 || rows < 0 || cols < 0) return fail(FM_E_INVALID, "negative size");
   if (count == 0 || rows == 0 || cols == 0) return FM_OK;

@@ -180,7 +180,7 @@ PyObject* normed(PyObject*, PyObject* args) {
     }
     const c10::cuda::CUDAGuard guard(p[0].device());
     const int rc = g_normed(table.data(), n, rows, numel / rows, dtype_code(p[0].scalar_type()),
-                            float(decay), float(step * std::sqrt(double(numel))), float(beta2),
+                            float(decay), float(step * std::sqrt(double(numel))), beta2,
                             float(eps), ws.data_ptr(), ws.nbytes(), current_stream(p[0]));
     if (rc == FM_OK) {
       p.bump();

@@ -366,3 +366,22 @@ def test_writes_are_seen_by_autograd(cuda_lib):
         fused_adamw([p], [torch.ones(8, device=DEV)], [z.clone()], [z.clone()], 1, lr=LR)
     with pytest.raises(RuntimeError, match="modified by an inplace operation"):
         loss.backward()
+
+
+@pytest.mark.parametrize("beta2", [0.9, 0.999, 0.9999])
+def test_normed_row_moment_of_slow_decays(cuda_lib, beta2):
+    """v takes (1 - beta2) of a row's mean square, with the weight rounded once: from v = 0
+    the result is the mean square (cols/128 + 60 sums at most, and 6 roundings for the mean,
+    the weight and the mix) and no more, and so after 30 steps of it."""
+    from muon_fused import fused_normed_update
+
+    rows, cols = 40, 96
+    u = _rand((1, rows, cols), 3, 0.1, torch.bfloat16)
+    p, v = _rand((rows, cols), 4, 0.02), torch.zeros(rows, device=DEV)
+    v64 = torch.zeros(rows, device=DEV, dtype=torch.float64)
+    for step in range(1, 31):
+        fused_normed_update([p], u, [v], lr=LR, wd=WD, beta2=beta2)
+        v64 = beta2 * v64 + (1 - beta2) * u[0].double().square().mean(1)
+        # a step's own roundings, and beta2's and the sum's for each step before
+        tol = (cols / 128 + 60 + 6 + 2 * step) * U32
+        assert ((v.double() - v64).abs() <= tol * v64).all(), step
