@@ -76,6 +76,7 @@ def fused_newton_schulz(G: torch.Tensor, steps: int = 5, workspace=None) -> torc
         raise RuntimeError("G must be 2D")
     if G.dtype not in _DTYPE_CODE:
         raise RuntimeError(f"unsupported dtype {G.dtype}; expected a floating type")
+    G = G.resolve_neg()  # the kernels read memory as it is
     if G.stride(1) != 1:
         G = G.contiguous()
     rows, cols = G.shape
@@ -107,13 +108,14 @@ def fused_newton_schulz_batched(G: torch.Tensor, steps: int = 5, workspace=None,
         raise RuntimeError("G must be 3D (batch, rows, cols)")
     if G.dtype not in _DTYPE_CODE:
         raise RuntimeError(f"unsupported dtype {G.dtype}; expected a floating type")
+    G = G.resolve_neg()
     if G.stride(2) != 1 or G.stride(0) < G.shape[1] * G.stride(1):
         G = G.contiguous()
     batch, rows, cols = G.shape
     if out is None:
         out = torch.empty((batch, rows, cols), dtype=torch.bfloat16, device=G.device)
     elif (out.shape != G.shape or out.dtype != torch.bfloat16 or not out.is_contiguous()
-          or out.device != G.device):
+          or out.is_neg() or out.device != G.device):
         raise RuntimeError("out must be a contiguous bf16 tensor shaped like G on its device")
     if G.numel() == 0:
         return out
@@ -151,12 +153,13 @@ def newton_schulz_heads(G: torch.Tensor, heads: int, steps: int = 5, dim: int = 
         raise RuntimeError("G must be 2D or 3D (batch, rows, cols)")
     if G.dtype not in _DTYPE_CODE:
         raise RuntimeError(f"unsupported dtype {G.dtype}; expected a floating type")
+    G = G.resolve_neg()
     rows, cols = G.shape[-2:]
     batch = G.shape[0] if G.dim() == 3 else 1
     if out is None:
         out = torch.empty(G.shape, dtype=torch.bfloat16, device=G.device)
     elif (out.shape != G.shape or out.dtype != torch.bfloat16 or not out.is_contiguous()
-          or out.device != G.device):
+          or out.is_neg() or out.device != G.device):
         raise RuntimeError("out must be a contiguous bf16 tensor shaped like G on its device")
     if G.numel() == 0:
         return out

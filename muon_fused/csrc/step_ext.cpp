@@ -149,8 +149,8 @@ PyObject* normed(PyObject*, PyObject* args) {
     };
     if (THPVariable_CheckExact(uo)) {
       const at::Tensor& u = THPVariable_Unpack(uo);
-      if (!u.is_cuda() || u.layout() != at::kStrided || !u.is_contiguous() || !update_ok(u) ||
-          u.dim() < 2 || u.size(0) != n || u.size(1) != rows || u.numel() != n * numel)
+      if (!u.is_cuda() || u.layout() != at::kStrided || !u.is_contiguous() || u.is_neg() ||
+          !update_ok(u) || u.dim() < 2 || u.size(0) != n || u.size(1) != rows || u.numel() != n * numel)
         Py_RETURN_NONE;
       for (int64_t i = 0; i < n; ++i)
         table[i].update = static_cast<const char*>(u.data_ptr()) + 2 * i * numel;
@@ -222,7 +222,8 @@ PyObject* heads(PyObject*, PyObject* args) {
       if (!THPVariable_CheckExact(oo)) Py_RETURN_NONE;
       out = THPVariable_Unpack(oo);
       if (out.scalar_type() != at::kBFloat16 || out.device() != g.device() ||
-          out.layout() != at::kStrided || !out.is_contiguous() || out.sizes() != g.sizes())
+          out.layout() != at::kStrided || !out.is_contiguous() || out.is_neg() ||
+          out.sizes() != g.sizes())
         Py_RETURN_NONE;
     } else {
       out = at::empty(g.sizes(), options.dtype(at::kBFloat16));

@@ -132,7 +132,8 @@ def fused_newton_schulz_heads(
     if form == "gram":
         return _C.newton_schulz_heads(G, heads, steps, dim, workspace, out)
     if out is not None and (out.shape != G.shape or out.dtype != torch.bfloat16
-                            or not out.is_contiguous() or out.device != G.device):
+                            or not out.is_contiguous() or out.is_neg()
+                            or out.device != G.device):
         raise RuntimeError("out must be a contiguous bf16 tensor shaped like G on its device")
     if G.numel() == 0:
         return torch.empty(G.shape, dtype=torch.bfloat16, device=G.device) if out is None else out

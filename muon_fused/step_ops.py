@@ -180,6 +180,8 @@ def _refuse_normed(p0, p, u, v, rows) -> None:
         raise RuntimeError("updates must be bf16 and shaped like the parameters")
     if v.dtype != torch.float32 or v.shape != (rows,):
         raise RuntimeError("row_moments must be fp32 vectors of one element per row")
+    if p.is_neg() or u.is_neg() or v.is_neg():
+        raise RuntimeError("fused_normed_update needs tensors that are not negative views")
     raise RuntimeError("fused_normed_update needs contiguous tensors")
 
 
@@ -242,7 +244,8 @@ def fused_normed_update(
                 and u.numel() == numel and (u.size(0) if u.dim() else -1) == rows
                 and v.dtype is torch.float32 and v.dim() == 1 and v.numel() == rows
                 and p.get_device() == u.get_device() == v.get_device() == device
-                and p.is_contiguous() and u.is_contiguous() and v.is_contiguous()):
+                and p.is_contiguous() and u.is_contiguous() and v.is_contiguous()
+                and not (p.is_neg() or u.is_neg() or v.is_neg())):
             _refuse_normed(p0, p, u, v, rows)
     if numel == 0:
         return

@@ -449,3 +449,20 @@ def test_blocks_past_the_end_among_many_heads(cuda_lib, heads, d, n, dim):
     check(out, G, heads, 5, dim)
     for _ in range(20):
         assert torch.equal(out, fused_newton_schulz_heads(G, heads, dim=dim))
+
+
+@pytest.mark.parametrize("shape,heads,steps", [((128, 256), 2, 5), ((128, 16), 2, 5), ((512, 64), 2, 5),
+                                               ((128, 256), 2, 7)])
+@pytest.mark.parametrize("dim", [0, 1])
+def test_negative_views(cuda_lib, shape, heads, steps, dim):
+    """Torch's negative bit is in the view, not in memory: every route takes the values."""
+    from muon_fused import fused_newton_schulz, fused_newton_schulz_heads
+
+    G = rand(shape if dim == 0 else shape[::-1], 21)
+    neg = torch._neg_view(G)
+    assert neg.is_neg() and neg.is_contiguous()
+    want = fused_newton_schulz_heads(-G, heads, steps, dim=dim)
+    assert torch.equal(fused_newton_schulz_heads(neg, heads, steps, dim=dim), want)
+    assert torch.equal(fused_newton_schulz(neg), fused_newton_schulz(-G))
+    with pytest.raises(RuntimeError, match="out must be"):
+        fused_newton_schulz_heads(G, heads, steps, dim=dim, out=torch._neg_view(want))

@@ -385,3 +385,15 @@ def test_normed_row_moment_of_slow_decays(cuda_lib, beta2):
         # a step's own roundings, and beta2's and the sum's for each step before
         tol = (cols / 128 + 60 + 6 + 2 * step) * U32
         assert ((v.double() - v64).abs() <= tol * v64).all(), step
+
+
+def test_normed_refuses_negative_views(cuda_lib):
+    """Torch's negative bit is in the view, not in memory, which is what the kernels use."""
+    from muon_fused import fused_normed_update
+
+    neg = torch._neg_view
+    p, u, v = _rand((8, 16), 1), _rand((1, 8, 16), 2, 0.1, torch.bfloat16), torch.ones(8, device=DEV)
+    for args in ([neg(p)], u, [v]), ([p], neg(u), [v]), ([p], [neg(u[0])], [v]), ([p], u, [neg(v)]):
+        with pytest.raises(RuntimeError, match="negative"):
+            fused_normed_update(*args, lr=LR)
+    assert torch.equal(p, _rand((8, 16), 1)) and bool((v == 1).all())
