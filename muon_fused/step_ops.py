@@ -46,6 +46,21 @@ def _bump(tensors) -> None:
     increment_version([t for t in tensors if not t.is_inference()])
 
 
+def _overlap(written, read) -> bool:
+    """Whether one of the contiguous tensors ``written`` shares memory with another tensor of
+    either list (as the C entries check within a call)."""
+    spans = sorted((t.data_ptr(), t.data_ptr() + t.nbytes, w) for ts, w in ((written, 1), (read, 0))
+                   for t in ts if t.numel())
+    end = written_end = 0  # furthest end so far, of all and of the written ones
+    for lo, hi, w in spans:
+        if lo < written_end or (w and lo < end):
+            return True
+        end = max(end, hi)
+        if w:
+            written_end = max(written_end, hi)
+    return False
+
+
 def _check_adamw(params, grads, moments1, moments2) -> list[tuple]:
     """Raise unless the kernel may work on the tensors; their types otherwise."""
     _check_cuda(params[0], "params")
@@ -152,14 +167,15 @@ def fused_adamw(
         return
     lists = (params, grads, moments1, moments2)
     types = _check_adamw(*lists)
-    if len(set(types)) == 1:
-        adamw_launch(*lists, alphas, lr, wd, betas, eps)
-    else:
-        for kind in dict.fromkeys(types):
-            idx = [i for i in range(n) if types[i] == kind]
-            adamw_launch(*([ts[i] for i in idx] for ts in lists), [alphas[i] for i in idx], lr, wd,
-                         betas, eps)
-    _bump(params + moments1 + moments2)
+    kinds = dict.fromkeys(types)
+    # a launch sees the tensors of its own kind only
+    if len(kinds) > 1 and _overlap(params + moments1 + moments2, grads):
+        raise RuntimeError("fused_adamw: tensors overlap in memory")
+    for kind in kinds:
+        idx = [i for i in range(n) if types[i] == kind]
+        some = [[ts[i] for i in idx] for ts in lists]
+        adamw_launch(*some, [alphas[i] for i in idx], lr, wd, betas, eps)
+        _bump(some[0] + some[2] + some[3])
 
 
 def normed_workspace_size(count: int, rows: int) -> int:

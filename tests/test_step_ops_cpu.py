@@ -99,3 +99,14 @@ def test_normed_workspace_size(count, rows):
 def test_struct_sizes_match_the_header():
     # 4 pointers, int64, float and its padding; 3 pointers
     assert _lib.ADAMW_TENSOR.size == 48 and _lib.NORMED_MATRIX.size == 24
+
+
+def test_overlap_of_written_and_read_tensors():
+    from muon_fused.step_ops import _overlap
+
+    x = torch.zeros(64)
+    assert not _overlap([x[:16], x[16:32]], [x[32:], x[40:48]])  # reads may overlap
+    assert not _overlap([x[8:8]], [x])
+    assert _overlap([x[:16], x[15:32].view(torch.bfloat16)], [])
+    assert _overlap([x[:16]], [x[15:]])
+    assert _overlap([x[40:41]], [x[:64], x[2:3]])  # inside a longer span before its neighbour

@@ -397,3 +397,30 @@ def test_normed_refuses_negative_views(cuda_lib):
         with pytest.raises(RuntimeError, match="negative"):
             fused_normed_update(*args, lr=LR)
     assert torch.equal(p, _rand((8, 16), 1)) and bool((v == 1).all())
+
+
+def test_adamw_mixed_types_are_checked_together(cuda_lib):
+    """Tensors of different kinds that share memory are refused before anything is written;
+    where a call is good, autograd sees the writes of every kind."""
+    from muon_fused import fused_adamw
+
+    st = [a + b + c for a, b, c in zip(*(_adam_state([(64,)], dt, torch.float32, seed=k) for k, dt in
+                                         enumerate((torch.float32, torch.bfloat16, torch.float16))))]
+    before = [[t.clone() for t in ts] for ts in st]
+    versions = [[t._version for t in ts] for ts in st]
+    bad = [list(ts) for ts in st]
+    bad[0][1] = st[2][0].view(torch.bfloat16)[:64]  # a bf16 parameter in an fp32 moment
+    read = [list(ts) for ts in st]
+    read[1][2] = st[0][0].view(torch.float16)[64:]  # an fp16 gradient in an fp32 parameter
+    same = [list(ts) for ts in st]
+    same[2][2] = same[3][2]  # wrong within the last kind only
+    for args in (bad, read, same):
+        with pytest.raises(RuntimeError, match="overlap"):
+            fused_adamw(*args, 1, lr=LR)
+    for xs, ys, vs in zip(st, before, versions):
+        for x, y, v in zip(xs, ys, vs):
+            assert torch.equal(x, y) and x._version == v
+    fused_adamw(*st, 1, lr=LR)
+    for k, (xs, vs) in enumerate(zip(st, versions)):
+        for x, v in zip(xs, vs):
+            assert (x._version > v) == (k != 1)
