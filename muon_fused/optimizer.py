@@ -210,7 +210,7 @@ class FusedMuon(Optimizer):
         buf = state["momentum_buffer"]
         dt = _EW_DTYPES.get(g.dtype)
         if g.is_cuda and dt is not None and buf.is_contiguous() and dst.is_contiguous():
-            gc = g if g.is_contiguous() else g.contiguous()
+            gc = g.contiguous().resolve_neg()
             with torch.cuda.device(g.device):
                 _lib.check(_lib.load().fm_muon_momentum(
                     buf.data_ptr(), gc.data_ptr(), dst.data_ptr(), g.numel(), dt,
@@ -292,7 +292,7 @@ class FusedMuon(Optimizer):
                 state["row_moment"] = torch.zeros(p.shape[0], dtype=torch.float32, device=p.device)
             data, v = p.data, state["row_moment"]
             if (data.is_cuda and data.dtype in STEP_DTYPES and data.is_contiguous()
-                    and type(p) in _PLAIN):
+                    and not data.is_neg() and type(p) in _PLAIN):
                 rows = data.shape[0]
                 by_type.setdefault(data.dtype, []).append((data.view(rows, -1), u.view(rows, -1), v))
             else:
@@ -444,7 +444,9 @@ class FusedMuon(Optimizer):
                     and g.device == buf1.device == buf2.device == p.device
                     and g.shape == buf1.shape == buf2.shape == p.shape
                     and p.is_contiguous() and g.is_contiguous() and buf1.is_contiguous()
-                    and buf2.is_contiguous()):
+                    and buf2.is_contiguous()
+                    # the kernel reads memory without torch's negative bit
+                    and not (p.is_neg() or g.is_neg() or buf1.is_neg() or buf2.is_neg())):
                 alpha = alphas.get(step)
                 if alpha is None:
                     alpha = alphas[step] = adamw_alpha(lr, (beta1, beta2), step)

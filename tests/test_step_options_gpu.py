@@ -261,3 +261,25 @@ def test_adamw_launch_checks_what_it_cannot_take(cuda_lib):
         with pytest.raises(RuntimeError):
             adamw_launch(*bad, [-0.1], 0.1, 0.0, (0.9, 0.95), 1e-8)
     assert torch.equal(p, _rand((64,), 0, 1.0))
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_gradients_with_the_negative_bit(cuda_lib, dtype):
+    """A contiguous gradient that torch negates in the view gives what its values give, in
+    every kind of group."""
+    from muon_fused import FusedMuon
+
+    results = []
+    for negate in (torch.neg, torch._neg_view):
+        groups = _groups(dtype)
+        opt = FusedMuon(groups, lr=LR)
+        for step in range(2):
+            _set_grads(groups, step)
+            for g in groups:
+                for p in g["params"]:
+                    p.grad = negate(p.grad)
+                    assert p.grad.is_neg() == (negate is torch._neg_view) and p.grad.is_contiguous()
+            opt.step()
+        results.append([p.detach() for g in groups for p in g["params"]])
+    for a, b in zip(*results):
+        assert torch.equal(a, b)
