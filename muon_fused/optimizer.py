@@ -55,8 +55,14 @@ _PLAIN = (torch.Tensor, torch.nn.Parameter)
 
 
 def _overlapping(tensors) -> bool:
-    """Whether two of the contiguous tensors share memory."""
-    spans = sorted((t.data_ptr(), t.data_ptr() + t.nbytes) for t in tensors if t.numel())
+    """Whether two of the tensors reach into the same memory (strided ones: from their first
+    to their last element)."""
+    spans = []
+    for t in tensors:
+        if type(t) in _PLAIN and t.layout == torch.strided and t.numel():
+            size = 1 + sum((n - 1) * st for n, st in zip(t.shape, t.stride()))
+            spans.append((t.data_ptr(), t.data_ptr() + size * t.element_size()))
+    spans.sort()
     return any(b[0] < a[1] for a, b in zip(spans, spans[1:]))
 
 
@@ -416,15 +422,28 @@ class FusedMuon(Optimizer):
         sharding.run_sharded(plan, rank, pg, dev, compute, apply)
 
     # ------------------------------------------------------------------ AdamW
+    @staticmethod
+    def _adamw_kind(p, g, buf1, buf2):
+        """What the fused kernel groups these tensors by; None where it does not take them."""
+        dtype = p.dtype
+        if (p.is_cuda and dtype in STEP_DTYPES and g.dtype == dtype
+                and type(p) in _PLAIN and type(g) in _PLAIN and not g.is_sparse
+                and buf1.dtype == buf2.dtype and buf1.dtype in (dtype, torch.float32)
+                and g.device == buf1.device == buf2.device == p.device
+                and g.shape == buf1.shape == buf2.shape == p.shape
+                and p.is_contiguous() and g.is_contiguous() and buf1.is_contiguous()
+                and buf2.is_contiguous()
+                # the kernel reads memory without torch's negative bit
+                and not (p.is_neg() or g.is_neg() or buf1.is_neg() or buf2.is_neg())):
+            return p.device, dtype, buf1.dtype
+        return None
+
     def _adamw_group(self, group) -> None:
         """Reference AdamW branch (optimizer.py:165-200): the tensors that the
         fused kernel takes in one launch, the others in the reference's torch
         ops.  Both give the same values."""
-        lr, wd = group["lr"], group["wd"]
-        beta1, beta2 = group["adamw_betas"]
-        eps: float = group["adamw_eps"]
-        fused: dict[tuple, tuple] = {}
-        alphas: dict[int, float] = {}  # -lr/scale by step
+        kinds: dict[Any, list] = {}  # tensors of a kind, in the group's order
+        items = []
         for p in group["params"]:
             g = p.grad
             if g is None:
@@ -435,45 +454,58 @@ class FusedMuon(Optimizer):
                 state["moment1"] = torch.zeros_like(g, dtype=self._adamw_state_dtype)
                 state["moment2"] = torch.zeros_like(g, dtype=self._adamw_state_dtype)
             state["step"] += 1
-            step: int = state["step"]
-            buf1, buf2 = state["moment1"], state["moment2"]
-            dtype = p.dtype
-            if (p.is_cuda and dtype in STEP_DTYPES and g.dtype == dtype
-                    and type(p) in _PLAIN and type(g) in _PLAIN and not g.is_sparse
-                    and buf1.dtype == buf2.dtype and buf1.dtype in (dtype, torch.float32)
-                    and g.device == buf1.device == buf2.device == p.device
-                    and g.shape == buf1.shape == buf2.shape == p.shape
-                    and p.is_contiguous() and g.is_contiguous() and buf1.is_contiguous()
-                    and buf2.is_contiguous()
-                    # the kernel reads memory without torch's negative bit
-                    and not (p.is_neg() or g.is_neg() or buf1.is_neg() or buf2.is_neg())):
-                alpha = alphas.get(step)
-                if alpha is None:
-                    alpha = alphas[step] = adamw_alpha(lr, (beta1, beta2), step)
-                lists = fused.setdefault((p.device, dtype, buf1.dtype), ([], [], [], [], []))
-                for ts, t in zip(lists, (p, g, buf1, buf2, alpha)):
-                    ts.append(t)
-                continue
-            data = p.data
-            if buf1.dtype != g.dtype and buf1.dtype == torch.float32:  # beside 16-bit parameters
-                g = g.to(buf1.dtype)
-                data = data.to(buf1.dtype)
-            buf1.lerp_(g, 1 - beta1)
-            buf2.lerp_(g.square(), 1 - beta2)
-            g = buf1 / (eps + buf2.sqrt())
-            bias_correction1 = 1 - beta1 ** step
-            bias_correction2 = 1 - beta2 ** step
-            scale = bias_correction1 / bias_correction2 ** 0.5
-            data.mul_(1 - lr * wd)
-            data.add_(g, alpha=-lr / scale)
-            if data.dtype != dtype:
-                p.data.copy_(data)
-        for lists in fused.values():
-            if _overlapping(lists[0]):  # tied storage: one after the other, as listed
-                for one in zip(*lists):
-                    adamw_launch(*([t] for t in one), lr, wd, (beta1, beta2), eps)
-            else:
-                adamw_launch(*lists, lr, wd, (beta1, beta2), eps)
+            item = p, g, state["moment1"], state["moment2"], state["step"]
+            items.append(item)
+            kinds.setdefault(self._adamw_kind(*item[:4]), []).append(item)
+        if len(kinds) > 1 and _overlapping([item[0] for item in items]):
+            # tied storage, perhaps of two kinds: one after the other, as listed
+            for item in items:
+                self._adamw_items(self._adamw_kind(*item[:4]), [item], group)
+            return
+        for kind, some in kinds.items():
+            self._adamw_items(kind, some, group)
+
+    def _adamw_items(self, kind, items, group) -> None:
+        """Step of tensors of one kind, as if one after the other."""
+        lr, wd, betas, eps = group["lr"], group["wd"], group["adamw_betas"], group["adamw_eps"]
+        if kind is not None:
+            alphas: dict[int, float] = {}  # -lr/scale by step
+            for *_, step in items:
+                if step not in alphas:
+                    alphas[step] = adamw_alpha(lr, betas, step)
+            *lists, steps = map(list, zip(*items))
+            try:
+                adamw_launch(*lists, [alphas[t] for t in steps], lr, wd, betas, eps)
+                return
+            except _lib.FusedMuonError as e:
+                if "overlap" not in str(e):
+                    raise
+            # some share memory, and nothing was written
+            if len(items) > 1:
+                for item in items:
+                    self._adamw_items(kind, [item], group)
+                return
+        for item in items:
+            self._adamw_torch(*item, lr, wd, betas, eps)
+
+    @staticmethod
+    def _adamw_torch(p, g, buf1, buf2, step: int, lr: float, wd: float, betas, eps: float) -> None:
+        """The branch's torch ops on one tensor."""
+        beta1, beta2 = betas
+        data = p.data
+        if buf1.dtype != g.dtype and buf1.dtype == torch.float32:  # beside 16-bit parameters
+            g = g.to(buf1.dtype)
+            data = data.to(buf1.dtype)
+        buf1.lerp_(g, 1 - beta1)
+        buf2.lerp_(g.square(), 1 - beta2)
+        g = buf1 / (eps + buf2.sqrt())
+        bias_correction1 = 1 - beta1 ** step
+        bias_correction2 = 1 - beta2 ** step
+        scale = bias_correction1 / bias_correction2 ** 0.5
+        data.mul_(1 - lr * wd)
+        data.add_(g, alpha=-lr / scale)
+        if data.dtype != p.dtype:
+            p.data.copy_(data)
 
     # ------------------------------------------------------------------ step
     @torch.no_grad()

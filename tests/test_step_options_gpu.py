@@ -283,3 +283,40 @@ def test_gradients_with_the_negative_bit(cuda_lib, dtype):
         results.append([p.detach() for g in groups for p in g["params"]])
     for a, b in zip(*results):
         assert torch.equal(a, b)
+
+
+def test_adamw_tensors_that_share_memory(cuda_lib):
+    """Tied storage of which the kernel takes one view only, gradients that are a parameter's
+    or a moment's own memory, a moment used twice: the values of the torch ops in the group's
+    order, bit for bit."""
+    from muon_fused import FusedMuon
+
+    def make():
+        w = _rand((24, 40), 1, 0.02)
+        flat = _rand((64,), 2, 0.02)
+        ts = [w, w.T, _rand((30,), 3, 0.02), w[:, ::2], flat[:32], _rand((5,), 4, 0.02, torch.bfloat16),
+              flat[16:48], _rand((7, 3), 5, 0.02)]
+        return [torch.nn.Parameter(t) for t in ts]
+
+    def set_grads(ps, step):
+        for i, p in enumerate(ps):
+            p.grad = _rand(p.shape, 100 * step + i, 1e-3, p.dtype)
+        ps[2].grad = ps[2].detach()  # the parameter itself
+        ps[4].grad = ps[6].detach()  # the values of another one that is written
+
+    a, b = make(), make()
+    opt = FusedMuon([{"params": a}], lr=0.5, wd=0.3)
+    state = {}
+    for step in (1, 2, 3):
+        set_grads(a, step)
+        set_grads(b, step)
+        opt.step()
+        for p in b:
+            _chain([p], state, step, 0.5, 0.3)
+        if step == 1:  # two parameters of one size that share a moment from here on
+            opt.state[a[2]]["moment2"] = opt.state[a[7]]["moment2"].view(-1)[:1].expand(30).clone()
+            state[b[2]] = (state[b[2]][0], state[b[7]][1].view(-1)[:1].expand(30).clone())
+            opt.state[a[6]]["moment1"] = opt.state[a[4]]["moment1"]
+            state[b[6]] = (state[b[4]][0], state[b[6]][1])
+    for i, (p, r) in enumerate(zip(a, b)):
+        assert torch.equal(p.detach(), r.detach()), i
