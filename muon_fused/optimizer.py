@@ -42,8 +42,8 @@ from torch.optim import Optimizer
 from muon_fused import _fused_muon_C as _C
 from muon_fused import _lib
 from muon_fused.ns_step import fused_newton_schulz_heads, workspace_size, workspace_size_heads
-from muon_fused.step_ops import (STEP_DTYPES, adamw_alpha, adamw_launch, fused_normed_update,
-                                 normed_workspace_size)
+from muon_fused.step_ops import (STEP_DTYPES, adamw_alpha, adamw_launch, adamw_ready,
+                                 fused_normed_update, normed_workspace_size)
 
 # Parameter / gradient dtypes the fused elementwise kernels handle.
 _EW_DTYPES = {torch.float32: _lib.FM_DT_F32, torch.bfloat16: _lib.FM_DT_BF16,
@@ -434,7 +434,8 @@ class FusedMuon(Optimizer):
                 and p.is_contiguous() and g.is_contiguous() and buf1.is_contiguous()
                 and buf2.is_contiguous()
                 # the kernel reads memory without torch's negative bit
-                and not (p.is_neg() or g.is_neg() or buf1.is_neg() or buf2.is_neg())):
+                and not (p.is_neg() or g.is_neg() or buf1.is_neg() or buf2.is_neg())
+                and adamw_ready(p.get_device())):
             return p.device, dtype, buf1.dtype
         return None
 

@@ -14,8 +14,10 @@ saved before the call fails instead of using the new ones.
 from __future__ import annotations
 
 import ctypes
+import functools
 import math
 import operator
+import warnings
 from collections.abc import Sequence
 
 import torch
@@ -81,6 +83,20 @@ def _check_adamw(params, grads, moments1, moments2) -> list[tuple]:
         if mt != vt or mt not in (pt, torch.float32):
             raise RuntimeError(f"moments must have the parameter's type or fp32, got {mt} and {vt}")
     return types
+
+
+@functools.cache
+def adamw_ready(device: int) -> bool:
+    """Whether the kernels run here: an sm_100 device, and the library built.  FusedMuon's
+    AdamW groups, which need nothing else of the library, use torch's ops otherwise."""
+    if torch.cuda.get_device_capability(device) != (10, 0):
+        return False
+    try:
+        _lib.step_ext()
+    except (ImportError, OSError) as e:
+        warnings.warn(f"AdamW groups run as torch ops: {e}", RuntimeWarning, stacklevel=2)
+        return False
+    return True
 
 
 def adamw_launch(params, grads, moments1, moments2, alphas, lr: float, wd: float, betas,

@@ -203,3 +203,20 @@ def test_sharded_options_equal_single_process(patched, collective):
     # the all-gather applies every update on every rank, the owner's apply only its own
     normed = 2 * len(SHAPES)
     assert rows == (2 * normed if collective == "nccl" else normed)
+
+
+def test_adamw_groups_need_neither_the_library_nor_an_sm100_device(monkeypatch):
+    from muon_fused import _lib, step_ops
+
+    def missing():
+        raise ImportError("libfused_muon.so is missing")
+
+    capability = [(10, 0)]
+    monkeypatch.setattr(torch.cuda, "get_device_capability", lambda d=None: capability[0])
+    monkeypatch.setattr(_lib, "step_ext", lambda: None)
+    assert step_ops.adamw_ready.__wrapped__(0)
+    monkeypatch.setattr(_lib, "step_ext", missing)
+    with pytest.warns(RuntimeWarning, match="torch ops"):
+        assert not step_ops.adamw_ready.__wrapped__(0)
+    capability[0] = (9, 0)
+    assert not step_ops.adamw_ready.__wrapped__(0)

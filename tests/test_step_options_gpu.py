@@ -320,3 +320,28 @@ def test_adamw_tensors_that_share_memory(cuda_lib):
             state[b[6]] = (state[b[4]][0], state[b[6]][1])
     for i, (p, r) in enumerate(zip(a, b)):
         assert torch.equal(p.detach(), r.detach()), i
+
+
+def test_adamw_group_without_the_extension(cuda_lib, monkeypatch):
+    """The torch ops where the kernels cannot run, the same values."""
+    from muon_fused import FusedMuon, _lib, step_ops
+
+    def missing():
+        raise ImportError("not built")
+
+    a = [torch.nn.Parameter(_rand(s, i, 0.02)) for i, s in enumerate([(33, 17), (9,), (4, 5, 6)])]
+    b = [torch.nn.Parameter(p.detach().clone()) for p in a]
+    opts = [FusedMuon([{"params": ps}], lr=0.01) for ps in (a, b)]
+    for step in range(2):
+        for i, (p, q) in enumerate(zip(a, b)):
+            p.grad = _rand(p.shape, 10 * step + i, 1e-3)
+            q.grad = p.grad.clone()
+        opts[0].step()
+        with monkeypatch.context() as m:
+            m.setattr(_lib, "step_ext", missing)
+            step_ops.adamw_ready.cache_clear()
+            with pytest.warns(RuntimeWarning, match="not built"):
+                opts[1].step()
+        step_ops.adamw_ready.cache_clear()
+    for p, q in zip(a, b):
+        assert torch.equal(p.detach(), q.detach())
