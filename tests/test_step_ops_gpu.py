@@ -424,3 +424,37 @@ def test_adamw_mixed_types_are_checked_together(cuda_lib):
     for k, (xs, vs) in enumerate(zip(st, versions)):
         for x, v in zip(xs, vs):
             assert (x._version > v) == (k != 1)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("mdtype", ["own", torch.float32])
+def test_values_of_inference_tensors(cuda_lib, dtype, mdtype):
+    """Inference tensors leave the one-call route for the checked one: every value is that of
+    ordinary tensors, which the other tests hold against the chain and the formulas."""
+    from muon_fused import fused_adamw, fused_normed_update
+
+    mt = dtype if mdtype == "own" else mdtype
+    plain = _adam_state(SHAPES, dtype, mt, seed=30)
+    chain = [[t.clone() for t in ts] for ts in plain]
+    rows, cols, n = 37, 129, 3
+    ps = [_rand((rows, cols), i, 0.02, dtype) for i in range(n)]
+    us = _rand((n, rows, cols), 10, 0.1, torch.bfloat16)
+    vs = [_rand((rows,), 20 + i, 0.1).square() for i in range(n)]
+    with torch.inference_mode():
+        inf = [[t.clone() for t in ts] for ts in plain]
+        ps2, us2, vs2 = [p.clone() for p in ps], us.clone(), [v.clone() for v in vs]
+        assert all(t.is_inference() for ts in (*inf, ps2, [us2], vs2) for t in ts)
+        for step in (1, 2):
+            fused_adamw(*inf, step, lr=LR, wd=WD)
+            fused_normed_update(ps2, us2, vs2, lr=LR, wd=WD)
+    for step in (1, 2):
+        fused_adamw(*plain, step, lr=LR, wd=WD)
+        fused_normed_update(ps, us, vs, lr=LR, wd=WD)
+        if mt == dtype:
+            for p, g, m, v in zip(*chain):
+                _torch_chain(p, g, m, v, step, LR, WD, (0.9, 0.95), 1e-8)
+    for xs, ys, zs in zip(inf, plain, chain if mt == dtype else plain):
+        for x, y, z in zip(xs, ys, zs):
+            assert _same(x, y) and _same(x, z)
+    for x, y in zip(ps2 + vs2, ps + vs):
+        assert torch.equal(x, y)
