@@ -110,7 +110,7 @@ class FusedMuon(Optimizer):
             parameters.
         adamw_state_dtype: type of the AdamW moments: ``None`` (default) is the
             gradient's, as the reference; ``torch.float32`` keeps them in fp32
-            beside 16-bit parameters.
+            beside 16-bit parameters (and changes nothing for wider ones).
     """
 
     def __init__(
@@ -422,6 +422,13 @@ class FusedMuon(Optimizer):
         sharding.run_sharded(plan, rank, pg, dev, compute, apply)
 
     # ------------------------------------------------------------------ AdamW
+    def _moment_dtype(self, t: torch.Tensor) -> torch.dtype:
+        """Type of the moments of a gradient (or parameter) like ``t``: fp32 state is for
+        16-bit ones, and nothing wider is cut down to it."""
+        if self._adamw_state_dtype is None:
+            return t.dtype
+        return torch.promote_types(t.dtype, self._adamw_state_dtype)
+
     @staticmethod
     def _adamw_kind(p, g, buf1, buf2):
         """What the fused kernel groups these tensors by; None where it does not take them."""
@@ -452,8 +459,9 @@ class FusedMuon(Optimizer):
             state = self.state[p]
             if "step" not in state:
                 state["step"] = 0
-                state["moment1"] = torch.zeros_like(g, dtype=self._adamw_state_dtype)
-                state["moment2"] = torch.zeros_like(g, dtype=self._adamw_state_dtype)
+                dtype = self._moment_dtype(g)
+                state["moment1"] = torch.zeros_like(g, dtype=dtype)
+                state["moment2"] = torch.zeros_like(g, dtype=dtype)
             state["step"] += 1
             item = p, g, state["moment1"], state["moment2"], state["step"]
             items.append(item)
@@ -562,9 +570,9 @@ class FusedMuon(Optimizer):
         for i, p in zip(ids, params):
             saved = state_dict["state"].get(i, {})
             for key in keys:
-                if key in saved and self.state[p][key].dtype != torch.float32:
-                    self.state[p][key] = saved[key].to(device=p.device, dtype=torch.float32,
-                                                       copy=True)
+                dtype = torch.float32 if key == "row_moment" else self._moment_dtype(p)
+                if key in saved and self.state[p][key].dtype != dtype:
+                    self.state[p][key] = saved[key].to(device=p.device, dtype=dtype, copy=True)
 
     def step(self, closure=None):
         """One optimisation step (optimizer.py:99-202)."""

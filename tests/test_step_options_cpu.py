@@ -220,3 +220,25 @@ def test_adamw_groups_need_neither_the_library_nor_an_sm100_device(monkeypatch):
         assert not step_ops.adamw_ready.__wrapped__(0)
     capability[0] = (9, 0)
     assert not step_ops.adamw_ready.__wrapped__(0)
+
+
+@pytest.mark.parametrize("dtype", [torch.float64, torch.complex64, torch.float32])
+def test_fp32_state_option_changes_nothing_for_wider_parameters(dtype):
+    """fp64 and complex parameters keep moments of their own type, through a checkpoint too."""
+    g = torch.Generator().manual_seed(0)
+    p0 = torch.randn(20, generator=g, dtype=dtype)
+    grads = [torch.randn(20, generator=g, dtype=dtype) for _ in range(3)]
+    runs = []
+    for state_dtype in (None, torch.float32):
+        p = torch.nn.Parameter(p0.clone())
+        opt = FusedMuon([p], lr=0.01, adamw_state_dtype=state_dtype)
+        for step, grad in enumerate(grads):
+            p.grad = grad.clone()
+            opt.step()
+            if step == 1:
+                saved = copy.deepcopy(opt.state_dict())
+                opt = FusedMuon([p], lr=0.01, adamw_state_dtype=state_dtype)
+                opt.load_state_dict(saved)
+        runs.append((p.detach(), opt.state[p]["moment1"], opt.state[p]["moment2"]))
+    for a, b in zip(*runs):
+        assert a.dtype == b.dtype == dtype and torch.equal(a, b)
