@@ -561,7 +561,18 @@ class FusedMuon(Optimizer):
         """As ``Optimizer.load_state_dict``, which casts state to the parameter's
         type, but the fp32 statistics stay fp32: ``row_moment``, and the AdamW
         moments where ``adamw_state_dtype`` asks for it."""
-        super().load_state_dict(state_dict)
+        seen = [state_dict]
+        # after the user's pre-hooks, which may replace the dict, and before the post-hooks
+        hooks = [self.register_load_state_dict_pre_hook(lambda _, sd: seen.append(sd)),
+                 self.register_load_state_dict_post_hook(lambda opt: opt._restore_fp32(seen[-1]),
+                                                         prepend=True)]
+        try:
+            super().load_state_dict(state_dict)
+        finally:
+            for hook in hooks:
+                hook.remove()
+
+    def _restore_fp32(self, state_dict) -> None:
         keys = ["row_moment"]
         if self._adamw_state_dtype is not None:
             keys += ["moment1", "moment2"]

@@ -242,3 +242,33 @@ def test_fp32_state_option_changes_nothing_for_wider_parameters(dtype):
         runs.append((p.detach(), opt.state[p]["moment1"], opt.state[p]["moment2"]))
     for a, b in zip(*runs):
         assert a.dtype == b.dtype == dtype and torch.equal(a, b)
+
+
+def test_loading_hooks_see_and_replace_the_state(patched):
+    """What a pre-hook puts in the place of the dict is loaded, in fp32 where that is kept,
+    and a post-hook has the last word."""
+    w = torch.nn.Parameter((torch.randn(32, 48) * 0.02).bfloat16())
+    e = torch.nn.Parameter((torch.randn(7, 5) * 0.02).bfloat16())
+    opt = FusedMuon([{"params": [w], "use_muon": True, "normed_beta2": 0.9}, {"params": [e]}],
+                    adamw_state_dtype=torch.float32)
+    w.grad, e.grad = torch.randn_like(w) * 1e-3, torch.randn_like(e) * 1e-3
+    opt.step()
+    saved = copy.deepcopy(opt.state_dict())
+    doubled = copy.deepcopy(saved)
+    for st in doubled["state"].values():
+        for key in ("row_moment", "moment1"):
+            if key in st:
+                st[key] = st[key] * 2 + 1e-4
+    seen = []
+    opt.register_load_state_dict_pre_hook(lambda o, sd: doubled)
+    opt.register_load_state_dict_post_hook(
+        lambda o: seen.append((o.state[w]["row_moment"].dtype, o.state[e]["moment1"].dtype))
+        or o.state[e]["moment2"].zero_())
+    for _ in range(2):
+        opt.load_state_dict(saved)
+        assert torch.equal(opt.state[w]["row_moment"], doubled["state"][0]["row_moment"])
+        assert torch.equal(opt.state[e]["moment1"], doubled["state"][1]["moment1"])
+        assert not opt.state[e]["moment2"].any()
+    assert seen == [(torch.float32, torch.float32)] * 2
+    assert len(opt._optimizer_load_state_dict_pre_hooks) == 1
+    assert len(opt._optimizer_load_state_dict_post_hooks) == 1
