@@ -138,19 +138,39 @@ class FusedMuon(Optimizer):
             adamw_betas=adamw_betas, adamw_eps=adamw_eps,
         )
         super().__init__(param_groups, defaults)
-        self._workspaces: dict[tuple, torch.Tensor] = {}
         self._process_group = process_group
         self._bucket_bytes = int(bucket_bytes)
         self._batch_bytes = int(batch_bytes)
-        self._plans: dict[tuple, Any] = {}
-        self._arena: dict[torch.device, torch.Tensor] = {}
         if collective not in ("nccl", "param_gather"):
             raise ValueError(f"collective must be 'nccl' or 'param_gather', got {collective!r}")
         self._collective = collective
+        self._init_caches()
+
+    def _init_caches(self) -> None:
+        """What the steps keep beside the state; a copy starts without it."""
+        self._workspaces: dict[tuple, torch.Tensor] = {}
+        self._plans: dict[tuple, Any] = {}
+        self._arena: dict[torch.device, torch.Tensor] = {}
         self._stores: dict[tuple, Any] = {}
         # id(group) -> (params, owner rank per param, momentum dtype per param)
         # of the group's last sharded step (consolidate_state_dict)
         self._owners: dict[int, tuple] = {}
+
+    # Constructor options that a copy keeps (a process group cannot be copied: the copy
+    # uses the world group), with their defaults for optimizers pickled without them.
+    _COPIED = {"_adamw_state_dtype": None, "_bucket_bytes": 256 << 20, "_batch_bytes": 4 << 30,
+               "_collective": "nccl"}
+
+    def __getstate__(self):
+        return {**super().__getstate__(), **{name: getattr(self, name) for name in self._COPIED}}
+
+    def __setstate__(self, state) -> None:
+        super().__setstate__(state)  # load_state_dict comes here too, with a live optimizer
+        for name, value in self._COPIED.items():
+            self.__dict__.setdefault(name, value)
+        if "_owners" not in self.__dict__:
+            self._process_group = None
+            self._init_caches()
 
     def add_param_group(self, param_group) -> None:
         """As ``Optimizer.add_param_group``, checking a Muon group's options first."""

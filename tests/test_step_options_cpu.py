@@ -4,6 +4,7 @@ the CPU: option checks, formulas, checkpoints, and the sharded step on gloo."""
 import copy
 import math
 import os
+import pickle
 import tempfile
 
 import pytest
@@ -272,3 +273,40 @@ def test_loading_hooks_see_and_replace_the_state(patched):
     assert seen == [(torch.float32, torch.float32)] * 2
     assert len(opt._optimizer_load_state_dict_pre_hooks) == 1
     assert len(opt._optimizer_load_state_dict_post_hooks) == 1
+
+
+@pytest.mark.parametrize("how", [copy.deepcopy, lambda o: pickle.loads(pickle.dumps(o))])
+def test_copies_of_the_optimizer(patched, how):
+    """A copy keeps the options, steps as the original does and loads its checkpoints."""
+    def make():
+        g = torch.Generator().manual_seed(3)
+        w = torch.nn.Parameter(torch.randn(32, 48, generator=g) * 0.02)
+        e = torch.nn.Parameter((torch.randn(7, generator=g) * 0.02).bfloat16())
+        return FusedMuon([{"params": [w], "use_muon": True, "heads": 4, "normed_beta2": 0.9},
+                          {"params": [e]}], lr=0.02, adamw_state_dtype=torch.float32)
+
+    def step(opt, seed):
+        g = torch.Generator().manual_seed(seed)
+        for group in opt.param_groups:
+            for p in group["params"]:
+                p.grad = (torch.randn(p.shape, generator=g) * 1e-3).to(p.dtype)
+        opt.step()
+        return [p.detach() for group in opt.param_groups for p in group["params"]]
+
+    def values(opt):
+        return [t for st in opt.state_dict()["state"].values() for t in st.values()
+                if isinstance(t, torch.Tensor)]
+
+    opt = make()
+    fresh = how(opt)  # before the first step: it makes its own state
+    for seed in (1, 2):
+        want = step(opt, seed)
+        for a, b in zip(want + values(opt), step(fresh, seed) + values(fresh)):
+            assert a.dtype == b.dtype and torch.equal(a, b)
+    later = how(opt)
+    other = make()
+    other.load_state_dict(copy.deepcopy(later.state_dict()))
+    later.load_state_dict(copy.deepcopy(opt.state_dict()))
+    assert all(t.dtype == torch.float32 for t in values(other)[1:])
+    for a, b in zip(step(opt, 3) + values(opt), step(later, 3) + values(later)):
+        assert a.dtype == b.dtype and torch.equal(a, b)
