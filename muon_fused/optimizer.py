@@ -155,6 +155,8 @@ class FusedMuon(Optimizer):
         # id(group) -> (params, owner rank per param, momentum dtype per param)
         # of the group's last sharded step (consolidate_state_dict)
         self._owners: dict[int, tuple] = {}
+        # parameter -> the one rank that holds its row_moment (after owner-applied steps)
+        self._row_owner: dict[torch.Tensor, int] = {}
 
     # Constructor options that a copy keeps (a process group cannot be copied: the copy
     # uses the world group), with their defaults for optimizers pickled without them.
@@ -414,8 +416,13 @@ class FusedMuon(Optimizer):
         for p, r in zip(params, plan.owner):
             if r != rank and p in self.state:  # e.g. after loading a consolidated checkpoint
                 self.state[p].pop("momentum_buffer", None)
-                if self._collective == "param_gather":  # only the owner applies updates
-                    self.state[p].pop("row_moment", None)
+        store = self._stores.get(key)
+        # supports() is checked before the store exists: afterwards the parameters
+        # deliberately share the store's flat buffers
+        gather = self._collective == "param_gather" and (store is not None
+                                                         or sharding.ParamStore.supports(params))
+        if group.get("normed_beta2") is not None:
+            self._place_row_moments(params, plan.owner if gather else None, pg, rank)
 
         def compute(indices, out) -> None:
             rows, cols = out.shape[1], out.shape[2]
@@ -428,11 +435,7 @@ class FusedMuon(Optimizer):
             self._apply_updates(group, [params[i]], [u])
 
         dev = params[0].device
-        store = self._stores.get(key)
-        if self._collective == "param_gather" and (store is not None
-                                                   or sharding.ParamStore.supports(params)):
-            # supports() is checked before the store exists: afterwards the
-            # parameters deliberately share the store's flat buffers
+        if gather:
             if store is None:
                 store = sharding.ParamStore(plan, params, dev)
                 self._stores[key] = store
@@ -440,6 +443,28 @@ class FusedMuon(Optimizer):
             sharding.run_sharded_param_gather(store, rank, pg, compute, apply)
             return
         sharding.run_sharded(plan, rank, pg, dev, compute, apply)
+
+    def _place_row_moments(self, params, owner, pg, rank: int) -> None:
+        """Row moments to where a sharded step applies updates: to each parameter's owner, or
+        to every rank (``owner`` None).  Every rank takes the same broadcasts."""
+        for i, p in enumerate(params):
+            had = self._row_owner.get(p)
+            if had is not None and (owner is None or owner[i] != had):
+                self._broadcast_row_moment(p, had, pg)
+                del self._row_owner[p]
+            if owner is not None:
+                self._row_owner[p] = owner[i]
+                if owner[i] != rank and p in self.state:
+                    self.state[p].pop("row_moment", None)
+
+    def _broadcast_row_moment(self, p, r: int, pg) -> None:
+        import torch.distributed as dist
+
+        st = self.state[p]
+        if "row_moment" not in st:
+            st["row_moment"] = torch.zeros(p.shape[0], dtype=torch.float32, device=p.device)
+        dist.broadcast(st["row_moment"], src=dist.get_global_rank(pg, r) if pg is not None else r,
+                       group=pg)
 
     # ------------------------------------------------------------------ AdamW
     def _moment_dtype(self, t: torch.Tensor) -> torch.dtype:
@@ -571,11 +596,11 @@ class FusedMuon(Optimizer):
                 src = dist.get_global_rank(pg, r) if pg is not None else r
                 dist.broadcast(buf, src=src, group=pg)
                 if group.get("normed_beta2") is not None:
-                    v = st.get("row_moment")
-                    if v is None:
-                        v = torch.zeros(p.shape[0], dtype=torch.float32, device=p.device)
-                        st["row_moment"] = v
-                    dist.broadcast(v, src=src, group=pg)
+                    self._broadcast_row_moment(p, self._row_owner.get(p, r), pg)
+            last = set(params)
+            for p in group["params"]:  # without a gradient in the last step
+                if p not in last and p in self._row_owner:
+                    self._broadcast_row_moment(p, self._row_owner[p], pg)
 
     def load_state_dict(self, state_dict) -> None:
         """As ``Optimizer.load_state_dict``, which casts state to the parameter's

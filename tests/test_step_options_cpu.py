@@ -310,3 +310,53 @@ def test_copies_of_the_optimizer(patched, how):
     assert all(t.dtype == torch.float32 for t in values(other)[1:])
     for a, b in zip(step(opt, 3) + values(opt), step(later, 3) + values(later)):
         assert a.dtype == b.dtype and torch.equal(a, b)
+
+
+def _run_uneven(case, **kw):
+    """Three steps of a normalised group that param_gather cannot serve in all of them: two
+    matrices that are slices of one tensor, or a step in which the lightest has no gradient
+    (afterwards the parameters live in the gather's flat buffers)."""
+    params = _params()[0]
+    if case == "shared":
+        base = torch.cat([params[0].detach(), params[1].detach()])
+        params[:2] = [torch.nn.Parameter(base[:32]), torch.nn.Parameter(base[32:])]
+    opt = FusedMuon([{"params": params, "use_muon": True, "normed_beta2": 0.9}], lr=0.02, **kw)
+    for s in range(4):
+        _set_grads([params], s)
+        if case == "missing" and s in (1, 3):
+            params[2].grad = None
+        opt.step()
+    return params, opt
+
+
+def _uneven_worker(rank, world, port, outdir, case):
+    os.environ["MASTER_ADDR"] = "127.0.0.1"
+    os.environ["MASTER_PORT"] = str(port)
+    import datetime
+
+    dist.init_process_group("gloo", rank=rank, world_size=world,
+                            timeout=datetime.timedelta(seconds=60))
+    _patch()
+    try:
+        params, opt = _run_uneven(case, bucket_bytes=8192, collective="param_gather")
+        opt.consolidate_state_dict()
+        torch.save({"params": [p.detach() for p in params], "state": opt.state_dict()["state"]},
+                   os.path.join(outdir, f"rank{rank}.pt"))
+    finally:
+        dist.destroy_process_group()
+
+
+@pytest.mark.parametrize("case", ["shared", "missing"])
+def test_row_moments_where_param_gather_falls_back(patched, case):
+    """A step that falls back to the update all-gather applies every update on every rank, so
+    every rank needs every row moment."""
+    params, opt = _run_uneven(case)
+    state = opt.state_dict()["state"]
+    outdir = tempfile.mkdtemp()
+    mp.spawn(_uneven_worker, args=(2, _free_port(), outdir, case), nprocs=2, join=True)
+    for r in range(2):
+        res = torch.load(os.path.join(outdir, f"rank{r}.pt"))
+        for i, (a, p) in enumerate(zip(res["params"], params)):
+            assert torch.equal(a, p.detach()), (r, i)
+        for k, v in state.items():
+            assert torch.equal(res["state"][k]["row_moment"], v["row_moment"]), (r, k)
