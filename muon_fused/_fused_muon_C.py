@@ -53,18 +53,24 @@ def workspace_size(m: int, n: int) -> int:
     return _lib.workspace_bytes(m, n)
 
 
+def workspace_for(G: torch.Tensor, need: int, workspace) -> torch.Tensor:
+    """``workspace``, or a buffer of ``need`` bytes on G's device where none is given.
+
+    Same policy as the reference (torch_binding.cu:95-102): a too-small workspace is
+    replaced by a fresh allocation.  So is one that is not contiguous: its ``nbytes`` do
+    not lie behind its first one, or belong to others."""
+    if workspace is not None:
+        _check_cuda(workspace, "workspace")
+        if workspace.device != G.device:
+            raise RuntimeError("workspace must be on the same device as the input")
+        if workspace.nbytes >= need and workspace.is_contiguous():
+            return workspace
+    return torch.empty(need, dtype=torch.uint8, device=G.device)
+
+
 def _workspace(G: torch.Tensor, rows: int, cols: int, workspace):
-    need = _lib.workspace_bytes(rows, cols)
-    if workspace is None:
-        return torch.empty(need, dtype=torch.uint8, device=G.device), need
-    _check_cuda(workspace, "workspace")
-    if workspace.device != G.device:
-        raise RuntimeError("workspace must be on the same device as the input")
-    if workspace.nbytes < need:
-        # Same policy as the reference (torch_binding.cu:95-102): a too-small
-        # workspace is replaced by a fresh allocation.
-        return torch.empty(need, dtype=torch.uint8, device=G.device), need
-    return workspace, workspace.nbytes
+    ws = workspace_for(G, _lib.workspace_bytes(rows, cols), workspace)
+    return ws, ws.nbytes
 
 
 def fused_newton_schulz(G: torch.Tensor, steps: int = 5, workspace=None) -> torch.Tensor:
@@ -119,9 +125,7 @@ def fused_newton_schulz_batched(G: torch.Tensor, steps: int = 5, workspace=None,
         raise RuntimeError("out must be a contiguous bf16 tensor shaped like G on its device")
     if G.numel() == 0:
         return out
-    need = _lib.workspace_bytes_batched(batch, rows, cols)
-    if workspace is None or workspace.nbytes < need:
-        workspace = torch.empty(need, dtype=torch.uint8, device=G.device)
+    workspace = workspace_for(G, _lib.workspace_bytes_batched(batch, rows, cols), workspace)
     with torch.cuda.device(G.device):
         _lib.check(
             _lib.load().fm_fused_newton_schulz_batched(
@@ -169,15 +173,8 @@ def newton_schulz_heads(G: torch.Tensor, heads: int, steps: int = 5, dim: int = 
         G = G.contiguous()
         ld = cols
     bs = G.stride(0) if G.dim() == 3 else 0
-    need = _lib.workspace_bytes_heads(batch, rows, cols, heads, dim)
-    if workspace is None:
-        workspace = torch.empty(need, dtype=torch.uint8, device=G.device)
-    else:
-        _check_cuda(workspace, "workspace")
-        if workspace.device != G.device:
-            raise RuntimeError("workspace must be on the same device as the input")
-        if workspace.nbytes < need:
-            workspace = torch.empty(need, dtype=torch.uint8, device=G.device)
+    workspace = workspace_for(G, _lib.workspace_bytes_heads(batch, rows, cols, heads, dim),
+                              workspace)
     with _on_device(G):
         _lib.check(
             _lib.load().fm_newton_schulz_heads(

@@ -24,7 +24,7 @@ import torch
 from torch.autograd.graph import increment_version
 
 from muon_fused import _lib
-from muon_fused._fused_muon_C import _check_cuda, _on_device, _stream
+from muon_fused._fused_muon_C import _check_cuda, _on_device, _stream, workspace_for
 
 STEP_DTYPES = {torch.float32: _lib.FM_DT_F32, torch.bfloat16: _lib.FM_DT_BF16,
                torch.float16: _lib.FM_DT_F16}
@@ -281,15 +281,7 @@ def fused_normed_update(
             _refuse_normed(p0, p, u, v, rows)
     if numel == 0:
         return
-    need = normed_workspace_size(n, rows)
-    if workspace is None:
-        workspace = torch.empty(need, dtype=torch.uint8, device=p0.device)
-    else:
-        _check_cuda(workspace, "workspace")
-        if workspace.device != p0.device:
-            raise RuntimeError("workspace must be on the same device as the input")
-        if workspace.nbytes < need:  # as everywhere: too small is replaced
-            workspace = torch.empty(need, dtype=torch.uint8, device=p0.device)
+    workspace = workspace_for(p0, normed_workspace_size(n, rows), workspace)
     ptr = torch.Tensor.data_ptr
     table = b"".join(map(_lib.NORMED_MATRIX.pack, map(ptr, params), map(ptr, updates),
                          map(ptr, row_moments)))
