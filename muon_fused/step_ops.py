@@ -18,7 +18,7 @@ import functools
 import math
 import operator
 import warnings
-from collections.abc import Sequence
+from collections.abc import Iterable, Sequence
 
 import torch
 from torch.autograd.graph import increment_version
@@ -34,9 +34,12 @@ _DTYPE = operator.attrgetter("dtype")
 
 
 def _check_list(tensors, name: str, count: int | None = None) -> list[torch.Tensor]:
-    if isinstance(tensors, torch.Tensor):
+    if isinstance(tensors, torch.Tensor) or not isinstance(tensors, Iterable):
         raise RuntimeError(f"{name} must be a list of tensors")
     tensors = list(tensors)
+    for t in tensors:
+        if not isinstance(t, torch.Tensor):
+            raise RuntimeError(f"{name} must be a list of tensors, got {type(t).__name__} in it")
     if count is not None and len(tensors) != count:
         raise RuntimeError(f"{name} must have one tensor per parameter, got {len(tensors)} "
                            f"for {count}")
@@ -258,8 +261,8 @@ def fused_normed_update(
         return
     params = _check_list(params, "params")
     n = len(params)
-    updates = list(updates.unbind(0)) if isinstance(updates, torch.Tensor) else list(updates)
-    updates = _check_list(updates, "updates", n)
+    updates = _check_list(updates.unbind(0) if isinstance(updates, torch.Tensor) else updates,
+                          "updates", n)
     row_moments = _check_list(row_moments, "row_moments", n)
     if n == 0:
         return

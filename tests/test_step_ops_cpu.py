@@ -110,3 +110,20 @@ def test_overlap_of_written_and_read_tensors():
     assert _overlap([x[:16], x[15:32].view(torch.bfloat16)], [])
     assert _overlap([x[:16]], [x[15:]])
     assert _overlap([x[40:41]], [x[:64], x[2:3]])  # inside a longer span before its neighbour
+
+
+@pytest.mark.parametrize("which", range(4))
+@pytest.mark.parametrize("bad", [None, [None], [1.0], 3])
+def test_lists_of_something_else_are_refused(which, bad):
+    """A gradient that is None, a number, no list at all: a RuntimeError that names the list."""
+    name = ("params", "grads", "moments1", "moments2")[which]
+    args = _four()
+    args[which] = bad
+    with pytest.raises(RuntimeError, match=name + " must be a list of tensors"):
+        fused_adamw(*args, 1, lr=0.1)
+    if which < 3:
+        name = ("params", "updates", "row_moments")[which]
+        args = [[torch.zeros(4, 6)], [torch.zeros(4, 6, dtype=torch.bfloat16)], [torch.zeros(4)]]
+        args[which] = bad
+        with pytest.raises(RuntimeError, match=name + " must be a list of tensors"):
+            fused_normed_update(*args, lr=0.1)
