@@ -30,6 +30,11 @@ STEP_DTYPES = {torch.float32: _lib.FM_DT_F32, torch.bfloat16: _lib.FM_DT_BF16,
                torch.float16: _lib.FM_DT_F16}
 
 
+class UnfitTensors(_lib.FusedMuonError):
+    """Tensors that torch's ops take and the kernel does not: they share memory or are
+    negative views.  Nothing was written."""
+
+
 _DTYPE = operator.attrgetter("dtype")
 
 
@@ -75,7 +80,7 @@ def _check_adamw(params, grads, moments1, moments2) -> list[tuple]:
     if not all(all(map(torch.Tensor.is_contiguous, ts)) for ts in lists):
         raise RuntimeError("fused_adamw needs contiguous tensors")
     if any(any(map(torch.Tensor.is_neg, ts)) for ts in lists):
-        raise RuntimeError("fused_adamw needs tensors that are not negative views")
+        raise UnfitTensors("fused_adamw needs tensors that are not negative views")
     if not all(all(map(torch.Tensor.is_same_size, params, ts)) for ts in lists[1:]):
         raise RuntimeError("params, grads and moments must have the same shapes")
     types = list(zip(*(map(_DTYPE, ts) for ts in lists)))
@@ -109,7 +114,7 @@ def adamw_launch(params, grads, moments1, moments2, alphas, lr: float, wd: float
     rc = _lib.step_ext().adamw(params, grads, moments1, moments2, alphas, float(1 - lr * wd),
                                1 - betas[0], 1 - betas[1], float(eps), False)
     if rc is not None:
-        _lib.check(rc, "fm_adamw")
+        _check_adamw_status(rc)
         return
     _check_adamw(params, grads, moments1, moments2)
     ptr = torch.Tensor.data_ptr
@@ -118,9 +123,15 @@ def adamw_launch(params, grads, moments1, moments2, alphas, lr: float, wd: float
                          map(torch.Tensor.numel, params), alphas))
     p0 = params[0]
     with _on_device(p0):
-        _lib.check(_lib.load().fm_adamw(
+        _check_adamw_status(_lib.load().fm_adamw(
             table, len(params), STEP_DTYPES[p0.dtype], STEP_DTYPES[moments1[0].dtype],
-            float(1 - lr * wd), 1 - betas[0], 1 - betas[1], float(eps), _stream(p0)), "fm_adamw")
+            float(1 - lr * wd), 1 - betas[0], 1 - betas[1], float(eps), _stream(p0)))
+
+
+def _check_adamw_status(rc: int) -> None:
+    if rc == _lib.FM_E_INVALID and b"overlap" in _lib.load().fm_last_error():
+        raise UnfitTensors("fused_adamw: tensors overlap in memory")
+    _lib.check(rc, "fm_adamw")
 
 
 def adamw_alpha(lr: float, betas, step: int) -> float:

@@ -360,3 +360,13 @@ def test_row_moments_where_param_gather_falls_back(patched, case):
             assert torch.equal(a, p.detach()), (r, i)
         for k, v in state.items():
             assert torch.equal(res["state"][k]["row_moment"], v["row_moment"]), (r, k)
+
+
+def test_which_parameters_reach_into_the_same_memory():
+    x = torch.zeros(64)
+    for yes in ([x[:32], x[31:]], [x.view(8, 8).T, x[63:]], [x[:48], x[2:3], x[40:]]):
+        assert opt_mod._overlapping(yes) and opt_mod._overlapping(yes[:1], yes[1:])
+    assert opt_mod._overlapping([], [x[:32], x[31:]])
+    for no in ([x[:32], x[32:]], [x[5:5], x], [x, x[5:5]], [x[:1].expand(9), x[1:]],
+               [x[:32].view(4, 8).T, x[32:]], [torch.zeros(3, 0).T, x]):
+        assert not opt_mod._overlapping(no) and not opt_mod._overlapping(no[:1], no[1:])
