@@ -83,9 +83,10 @@ def fused_newton_schulz(G: torch.Tensor, steps: int = 5, workspace=None) -> torc
     if G.dtype not in _DTYPE_CODE:
         raise RuntimeError(f"unsupported dtype {G.dtype}; expected a floating type")
     G = G.resolve_neg()  # the kernels read memory as it is
-    if G.stride(1) != 1:
-        G = G.contiguous()
     rows, cols = G.shape
+    ld = G.stride(0)
+    if G.stride(1) != 1 or ld < cols:
+        G, ld = G.contiguous(), cols  # strides of a size of one say nothing
     out = torch.empty((rows, cols), dtype=torch.bfloat16, device=G.device)
     if G.numel() == 0:
         return out
@@ -93,7 +94,7 @@ def fused_newton_schulz(G: torch.Tensor, steps: int = 5, workspace=None) -> torc
     with torch.cuda.device(G.device):
         _lib.check(
             _lib.load().fm_fused_newton_schulz(
-                G.data_ptr(), _DTYPE_CODE[G.dtype], rows, cols, G.stride(0), out.data_ptr(),
+                G.data_ptr(), _DTYPE_CODE[G.dtype], rows, cols, ld, out.data_ptr(),
                 int(steps), ws.data_ptr(), ws_bytes, _stream(G)),
             "fm_fused_newton_schulz")
     return out
@@ -115,9 +116,10 @@ def fused_newton_schulz_batched(G: torch.Tensor, steps: int = 5, workspace=None,
     if G.dtype not in _DTYPE_CODE:
         raise RuntimeError(f"unsupported dtype {G.dtype}; expected a floating type")
     G = G.resolve_neg()
-    if G.stride(2) != 1 or G.stride(0) < G.shape[1] * G.stride(1):
-        G = G.contiguous()
     batch, rows, cols = G.shape
+    bs, ld = G.stride(0), G.stride(1)
+    if G.stride(2) != 1 or ld < cols or bs < rows * ld:
+        G, bs, ld = G.contiguous(), rows * cols, cols
     if out is None:
         out = torch.empty((batch, rows, cols), dtype=torch.bfloat16, device=G.device)
     elif (out.shape != G.shape or out.dtype != torch.bfloat16 or not out.is_contiguous()
@@ -129,7 +131,7 @@ def fused_newton_schulz_batched(G: torch.Tensor, steps: int = 5, workspace=None,
     with torch.cuda.device(G.device):
         _lib.check(
             _lib.load().fm_fused_newton_schulz_batched(
-                G.data_ptr(), _DTYPE_CODE[G.dtype], batch, rows, cols, G.stride(1), G.stride(0),
+                G.data_ptr(), _DTYPE_CODE[G.dtype], batch, rows, cols, ld, bs,
                 out.data_ptr(), rows * cols, int(steps), workspace.data_ptr(), workspace.nbytes,
                 _stream(G)),
             "fm_fused_newton_schulz_batched")

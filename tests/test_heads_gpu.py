@@ -466,3 +466,30 @@ def test_negative_views(cuda_lib, shape, heads, steps, dim):
     assert torch.equal(fused_newton_schulz(neg), fused_newton_schulz(-G))
     with pytest.raises(RuntimeError, match="out must be"):
         fused_newton_schulz_heads(G, heads, steps, dim=dim, out=torch._neg_view(want))
+
+
+@pytest.mark.parametrize("steps", [0, 5, 6])
+@pytest.mark.parametrize("d", [40, 200])
+def test_one_row_and_repeated_rows(cuda_lib, d, steps):
+    """Heads of a single row (or column) on the long side, and inputs whose rows or columns
+    are one expanded in memory, on every route: what contiguous copies give."""
+    from muon_fused import fused_newton_schulz, fused_newton_schulz_heads
+
+    x = rand((1, 4 * d), d)
+    cases = [(x, 4, 1), (x.T, 4, 0), (x.T.contiguous().T, 4, 1), (rand((3, 1, 4 * d), 1), 4, 1),
+             (rand((300, 1), 2).expand(300, 4 * d), 4, 1), (rand((1, 300), 3).expand(4 * d, 300), 4, 0),
+             (rand((1, 2 * d, 64), 4).expand(3, 2 * d, 64), 2, 0)]
+    for G, heads, dim in cases:
+        plain = torch.empty(G.shape, dtype=G.dtype, device=DEV).copy_(G)
+        out = fused_newton_schulz_heads(G, heads, steps, dim=dim)
+        assert torch.equal(out, fused_newton_schulz_heads(plain, heads, steps, dim=dim))
+        if G.shape[-1 - dim] == 1:  # a head is a vector v, and its iterates are s_k·v/|v|
+            for h, o in zip(plain.double().chunk(heads, -2 + dim), out.double().chunk(heads, -2 + dim)):
+                s = 1.0
+                for _ in range(steps):
+                    s = A * s + B * s ** 3 + C * s ** 5
+                want = s * h / h.flatten(-2).norm(dim=-1)[..., None, None]
+                # the bf16 path rounds every iterate, A and the factor: 1e-2 as in its own tests
+                assert float((o - want).norm()) <= 1e-2 * float(want.norm())
+        if G.dim() == 2:
+            assert torch.equal(fused_newton_schulz(G, steps), fused_newton_schulz(plain, steps))
