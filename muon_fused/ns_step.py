@@ -108,7 +108,9 @@ def fused_newton_schulz_heads(
     the exact one up to its bf16 rounding, on ill-conditioned heads too; the
     error of heads whose long side has rank 1 to 4 only is 0.7 to 0.25 % after
     five steps.  Wider heads, and more steps, run as a batch of matrices on the
-    bf16 path of ``fused_newton_schulz``.
+    bf16 path of ``fused_newton_schulz``, with its error.  Both that route and the
+    one for heads wider than long copy G (unless the heads lie in it as a batch) and
+    the result with torch, beside the workspace.
 
     Args:
         G: CUDA tensor (rows, cols), or (batch, rows, cols) for same-shape

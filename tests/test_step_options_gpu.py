@@ -322,19 +322,21 @@ def test_adamw_tensors_that_share_memory(cuda_lib):
         assert torch.equal(p.detach(), r.detach()), i
 
 
-def test_adamw_group_without_the_extension(cuda_lib, monkeypatch):
+@pytest.mark.parametrize("dtype,state", [(torch.float32, None), (torch.bfloat16, None),
+                                         (torch.bfloat16, torch.float32), (torch.float16, torch.float32)])
+def test_adamw_group_without_the_extension(cuda_lib, monkeypatch, dtype, state):
     """The torch ops where the kernels cannot run, the same values."""
     from muon_fused import FusedMuon, _lib, step_ops
 
     def missing():
         raise ImportError("not built")
 
-    a = [torch.nn.Parameter(_rand(s, i, 0.02)) for i, s in enumerate([(33, 17), (9,), (4, 5, 6)])]
+    a = [torch.nn.Parameter(_rand(s, i, 0.02, dtype)) for i, s in enumerate([(33, 17), (9,), (4, 5, 6)])]
     b = [torch.nn.Parameter(p.detach().clone()) for p in a]
-    opts = [FusedMuon([{"params": ps}], lr=0.01) for ps in (a, b)]
+    opts = [FusedMuon([{"params": ps}], lr=0.01, adamw_state_dtype=state) for ps in (a, b)]
     for step in range(2):
         for i, (p, q) in enumerate(zip(a, b)):
-            p.grad = _rand(p.shape, 10 * step + i, 1e-3)
+            p.grad = _rand(p.shape, 10 * step + i, 1e-3, dtype)
             q.grad = p.grad.clone()
         opts[0].step()
         with monkeypatch.context() as m:
